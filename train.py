@@ -74,12 +74,8 @@ def train(config, exp_name, work_dir, synthetic, max_updates, log_interval, val_
         sharding.bind_rank_to_cores(local, int(os.environ.get('LOCAL_WORLD_SIZE', world)))       # loader threads stay next to this rank's GPU
         backend = os.environ.get('SOME_AMD_DIST_BACKEND', 'nccl')
         if backend == 'nccl':
-            # RCCL's stream on HIGH priority: the HIP runtime keeps separate hardware queues per priority level, so the collectives of the
-            # bucketed all-reduce cannot land on a queue one of the step's compute streams (two lanes + two weight-gradient side streams +
-            # the loader's copy stream on 4 normal-priority queues) already occupies - modelled on one GPU, the all-reduce is 35 - 50 %
-            # exposed that way and 90 - 130 % when it shares a queue (tools/ddp_overlap_bench.py)
-            opts = torch.distributed.ProcessGroupNCCL.Options(is_high_priority_stream=True)
-            torch.distributed.init_process_group('nccl', pg_options=opts, device_id=torch.device('cuda', dev))
+            # (RCCL's stream keeps the default priority: streams of different priorities working side by side have hung on this part)
+            torch.distributed.init_process_group('nccl', device_id=torch.device('cuda', dev))
         else:
             torch.distributed.init_process_group(backend)
     if rank == 0:
