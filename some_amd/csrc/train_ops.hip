@@ -747,20 +747,27 @@ __global__ __launch_bounds__(256) void emd_kernel(const float* __restrict__ pred
     }
 }
 
-// AdamW (torch.optim.AdamW semantics, amsgrad off): decoupled decay, bias-corrected moments
-__global__ __launch_bounds__(256) void adamw_kernel(float* __restrict__ p, const float* __restrict__ g, float* __restrict__ m, float* __restrict__ v,
-                                                     int64_t n, float lr, float beta1, float beta2, float eps, float weight_decay,
-                                                     float bc1, float bc2_sqrt, float grad_scale) {
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (i >= n) return;
+// AdamW (torch.optim.AdamW semantics, amsgrad off): decoupled decay, bias-corrected moments.  One function for both kernels below, its products not
+// fused into the sums: left to the compiler, the two kernels fused different ones and an update's bits depended on where its clip factor was computed
+__device__ __forceinline__ void adamw_update(float* __restrict__ p, const float* __restrict__ g, float* __restrict__ m, float* __restrict__ v, int64_t i,
+                                             float lr, float beta1, float beta2, float eps, float weight_decay, float bc1, float bc2_sqrt,
+                                             float grad_scale) {
+#pragma clang fp contract(off)
     const float gi = g[i] * grad_scale;
-    float pi = p[i] * (1.f - lr * weight_decay);
+    const float pi = p[i] * fmaf(-lr, weight_decay, 1.f);
     const float mi = beta1 * m[i] + (1.f - beta1) * gi;
     const float vi = beta2 * v[i] + (1.f - beta2) * gi * gi;
     m[i] = mi;
     v[i] = vi;
     const float denom = sqrtf(vi) / bc2_sqrt + eps;
     p[i] = pi - (lr / bc1) * (mi / denom);
+}
+
+__global__ __launch_bounds__(256) void adamw_kernel(float* __restrict__ p, const float* __restrict__ g, float* __restrict__ m, float* __restrict__ v,
+                                                     int64_t n, float lr, float beta1, float beta2, float eps, float weight_decay,
+                                                     float bc1, float bc2_sqrt, float grad_scale) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i < n) adamw_update(p, g, m, v, i, lr, beta1, beta2, eps, weight_decay, bc1, bc2_sqrt, grad_scale);
 }
 
 // The same update with the gradient scale taken from DEVICE memory: grad_scale = min(1, clip / (sqrt(sumsq) / denom + 1e-6)) / denom - the
@@ -776,14 +783,7 @@ __global__ __launch_bounds__(256) void adamw_clip_kernel(float* __restrict__ p, 
     const double norm = sqrt(ss) / denom;
     const double coef = clip > 0.0 ? fmin(1.0, clip / (norm + 1e-6)) : 1.0;
     const float grad_scale = (float)(coef / denom);
-    const float gi = g[i] * grad_scale;
-    float pi = p[i] * (1.f - lr * weight_decay);
-    const float mi = beta1 * m[i] + (1.f - beta1) * gi;
-    const float vi = beta2 * v[i] + (1.f - beta2) * gi * gi;
-    m[i] = mi;
-    v[i] = vi;
-    const float den = sqrtf(vi) / bc2_sqrt + eps;
-    p[i] = pi - (lr / bc1) * (mi / den);
+    adamw_update(p, g, m, v, i, lr, beta1, beta2, eps, weight_decay, bc1, bc2_sqrt, grad_scale);
 }
 
 }  // namespace
