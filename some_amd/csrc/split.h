@@ -18,6 +18,11 @@ typedef _Float16 half4 __attribute__((ext_vector_type(4)));
 typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
 
 __host__ __device__ inline void split_f16(float x, half_t& hi, half_t& lo) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    // x is rounded to f32 before it is split.  Without this hipcc may fold the product that made x into ONE of the uses below (v_fma_mixlo_f16: one
+    // rounding instead of two): the stored hi and the hi that lo was taken from then differ by a f16 step where the two disagree
+    asm("" : "+v"(x));
+#endif
     hi = (half_t)x;
     lo = (half_t)(x - (float)hi);
 }
