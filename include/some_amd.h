@@ -522,6 +522,62 @@ int some_op_dwconv_silu(SomeHandle* h, const float* x_dev, const float* taps_dev
                         const int32_t* frame_offsets_dev, int32_t B, int32_t max_frames, float* y_dev,
                         int32_t out_split, void* stream);
 
+/* ---- causal attention over packed clips --------------------------------------------------------------- */
+/* Attention that looks back only: for live transcription (frame by frame over a cache) and for training the models that do it.  Arrays are
+ * [rows, heads, head_dim] with head_dim (64 or 128) contiguous and the row and head strides given in elements, so slices of a fused
+ * projection are read where they lie: 16-byte aligned, strides non-negative multiples of 16 bytes, rows less than 16 MiB apart.  All arrays of
+ * a call have one dtype; sums, softmax statistics and norms are 32-bit, f32 products exact.  heads is a multiple of kv_heads: query head h
+ * reads kv head h / (heads / kv_heads).  Rows are packed clip by clip (int32 device offsets, B + 1 entries); rows behind the last clip are
+ * neither read nor written.  Fewer than 2^29 rows. */
+#define SOME_DTYPE_F32 0
+#define SOME_DTYPE_F16 1
+#define SOME_DTYPE_BF16 2
+
+/* Norm of queries and keys per head and the position rotation in one pass: z = x rsqrt(mean(x^2) + eps) gamma, then channel i and i + head_dim / 2
+ * are rotated by positions[row] theta^(-2 i / head_dim) (the angle reduced in 64 bits).  gamma: fp32 [head_dim]; positions: device int32 (or, with
+ * positions64 != 0, int64) [rows], any sign.  The outputs may be the inputs. */
+int some_op_qk_norm_rope(SomeHandle* h, int32_t dtype, int32_t head_dim, const void* q_dev, int64_t q_row, int64_t q_head, int32_t heads,
+                         const void* k_dev, int64_t k_row, int64_t k_head, int32_t kv_heads, int64_t rows, const float* gamma_q_dev,
+                         const float* gamma_k_dev, const void* positions_dev, int32_t positions64, double theta, float eps, void* q_out_dev,
+                         int64_t qo_row, int64_t qo_head, void* k_out_dev, int64_t ko_row, int64_t ko_head, void* stream);
+/* Its gradients: q / k are the forward's inputs, dqo / dko the gradients of its outputs; writes dq, dk (which may be dqo, dko) and - added to their
+ * contents if accumulate != 0 - the fp32 gain gradients, summed in a fixed order.  scratch_dev: some_train_qk_norm_rope_bytes. */
+size_t some_train_qk_norm_rope_bytes(const SomeHandle* h, int64_t rows, int32_t heads, int32_t kv_heads, int32_t head_dim);
+int some_train_qk_norm_rope_bwd(SomeHandle* h, int32_t dtype, int32_t head_dim, const void* q_dev, int64_t q_row, int64_t q_head, int32_t heads,
+                                const void* k_dev, int64_t k_row, int64_t k_head, int32_t kv_heads, int64_t rows, const float* gamma_q_dev,
+                                const float* gamma_k_dev, const void* positions_dev, int32_t positions64, double theta, float eps,
+                                const void* dqo_dev, int64_t dqo_row, int64_t dqo_head, const void* dko_dev, int64_t dko_row, int64_t dko_head,
+                                void* dq_dev, int64_t dq_row, int64_t dq_head, void* dk_dev, int64_t dk_row, int64_t dk_head,
+                                float* dgamma_q_dev, float* dgamma_k_dev, int32_t accumulate, void* scratch_dev, size_t scratch_bytes, void* stream);
+
+/* out = softmax(scale q k^T) v per clip.  Clip b's queries are rows [q_offsets[b], q_offsets[b + 1]) and its keys rows [k_offsets[b], ...): with
+ * causal != 0 the queries are the clip's LAST frames, i.e. query i of Tq sees keys j <= i + Tk - Tq (a chunk over what is cached already); with
+ * causal = 0 every key.  A query that sees no key gets 0, and nothing in a masked place - infinities and NaN included - reaches an output.
+ * scale > 0.  lse_dev: NULL, or fp32 [heads, q_rows] for the backward (base-2 log-sum-exp, -inf where no key is seen). */
+int some_op_causal_attention(SomeHandle* h, int32_t dtype, int32_t head_dim, const void* q_dev, int64_t q_row, int64_t q_head, int32_t heads,
+                             const void* k_dev, int64_t k_row, int64_t k_head, const void* v_dev, int64_t v_row, int64_t v_head, int32_t kv_heads,
+                             const int32_t* q_offsets_dev, const int32_t* k_offsets_dev, int32_t B, int64_t q_rows, int64_t k_rows, int32_t causal,
+                             float scale, void* out_dev, int64_t o_row, int64_t o_head, float* lse_dev, void* stream);
+/* Its gradients (dk, dv summed over the heads of a group), without atomics: the same bits every time.  out_dev, lse_dev: the forward's;
+ * dsum_dev: fp32 [heads, q_rows] scratch.  Here too nothing in a masked place reaches an output. */
+int some_train_causal_attention_bwd(SomeHandle* h, int32_t dtype, int32_t head_dim, const void* q_dev, int64_t q_row, int64_t q_head, int32_t heads,
+                                    const void* k_dev, int64_t k_row, int64_t k_head, const void* v_dev, int64_t v_row, int64_t v_head,
+                                    int32_t kv_heads, const int32_t* q_offsets_dev, const int32_t* k_offsets_dev, int32_t B, int64_t q_rows,
+                                    int64_t k_rows, int32_t causal, float scale, const void* out_dev, int64_t o_row, int64_t o_head,
+                                    const float* lse_dev, const void* dout_dev, int64_t do_row, int64_t do_head, void* dq_dev, int64_t dq_row,
+                                    int64_t dq_head, void* dk_dev, int64_t dk_row, int64_t dk_head, void* dv_dev, int64_t dv_row, int64_t dv_head,
+                                    float* dsum_dev, void* stream);
+
+/* The next frame of B live streams: out[b, h] = attention of q[b, h] over the first lengths[b] rows (device int32, cut to [0, max_length]; 0: zeros) of
+ * stream b's cache, k_dev + b k_batch and v_dev + b v_batch.  Rows from lengths[b] on are not read.  max_length: an upper bound of the lengths the
+ * caller knows (at most the cache's capacity); it sizes the launch.  workspace_dev: some_op_attention_step_bytes bytes, 16-byte aligned, not shared
+ * with a call that may run at the same time. */
+size_t some_op_attention_step_bytes(const SomeHandle* h, int32_t B, int32_t heads, int32_t kv_heads, int32_t head_dim, int32_t max_length);
+int some_op_attention_step(SomeHandle* h, int32_t dtype, int32_t head_dim, const void* q_dev, int64_t q_row, int64_t q_head, int32_t heads,
+                           const void* k_dev, int64_t k_batch, int64_t k_row, int64_t k_head, const void* v_dev, int64_t v_batch, int64_t v_row,
+                           int64_t v_head, int32_t kv_heads, const int32_t* lengths_dev, int32_t B, int32_t max_length, float scale,
+                           void* out_dev, int64_t o_row, int64_t o_head, void* workspace_dev, size_t workspace_bytes, void* stream);
+
 /* ---- per-kernel timing (measurement only; off by default) ----------------------------------------- */
 
 typedef struct SomeKernelStat {

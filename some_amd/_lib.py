@@ -23,6 +23,7 @@ SAMPLE_F32, SAMPLE_PCM16 = 0, 1
  ELT_AXPY_DROP) = range(9)
 GEMM_SPLIT_IN, GEMM_SPLIT_OUT, GEMM_HI_ONLY, GEMM_HI_BF16 = 1, 2, 4, 8
 OPERAND_F16X2, OPERAND_BF16 = 0, 1
+DTYPE_F32, DTYPE_F16, DTYPE_BF16 = 0, 1, 2
 
 
 class SomeConfig(C.Structure):
@@ -134,6 +135,20 @@ SYMBOLS = {
     'some_op_qkv_attention_f16x3_bytes': (C.c_size_t, [C.c_int32, C.c_int32]),
     'some_op_qkv_attention_f16x3': (C.c_int, [_P, _P, _P, _P, C.c_int32, C.c_int32, C.c_int32, _P, _P, C.c_size_t, _P]),
     'some_op_dwconv_silu': (C.c_int, [_P, _P, _P, _P, _P, C.c_int32, C.c_int32, _P, C.c_int32, _P]),
+    'some_op_qk_norm_rope': (C.c_int, [_P, C.c_int32, C.c_int32, _P, C.c_int64, C.c_int64, C.c_int32, _P, C.c_int64, C.c_int64, C.c_int32, C.c_int64, _P, _P, _P, C.c_int32,
+                                       C.c_double, C.c_float, _P, C.c_int64, C.c_int64, _P, C.c_int64, C.c_int64, _P]),
+    'some_train_qk_norm_rope_bytes': (C.c_size_t, [_P, C.c_int64, C.c_int32, C.c_int32, C.c_int32]),
+    'some_train_qk_norm_rope_bwd': (C.c_int, [_P, C.c_int32, C.c_int32, _P, C.c_int64, C.c_int64, C.c_int32, _P, C.c_int64, C.c_int64, C.c_int32, C.c_int64, _P, _P, _P, C.c_int32,
+                                              C.c_double, C.c_float, _P, C.c_int64, C.c_int64, _P, C.c_int64, C.c_int64, _P, C.c_int64, C.c_int64, _P, C.c_int64, C.c_int64,
+                                              _P, _P, C.c_int32, _P, C.c_size_t, _P]),
+    'some_op_causal_attention': (C.c_int, [_P, C.c_int32, C.c_int32, _P, C.c_int64, C.c_int64, C.c_int32, _P, C.c_int64, C.c_int64, _P, C.c_int64, C.c_int64, C.c_int32, _P, _P, C.c_int32,
+                                           C.c_int64, C.c_int64, C.c_int32, C.c_float, _P, C.c_int64, C.c_int64, _P, _P]),
+    'some_train_causal_attention_bwd': (C.c_int, [_P, C.c_int32, C.c_int32, _P, C.c_int64, C.c_int64, C.c_int32, _P, C.c_int64, C.c_int64, _P, C.c_int64, C.c_int64, C.c_int32, _P, _P,
+                                                  C.c_int32, C.c_int64, C.c_int64, C.c_int32, C.c_float, _P, C.c_int64, C.c_int64, _P, _P, C.c_int64, C.c_int64, _P, C.c_int64, C.c_int64, _P, C.c_int64, C.c_int64,
+                                                  _P, C.c_int64, C.c_int64, _P, _P]),
+    'some_op_attention_step_bytes': (C.c_size_t, [_P, C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_int32]),
+    'some_op_attention_step': (C.c_int, [_P, C.c_int32, C.c_int32, _P, C.c_int64, C.c_int64, C.c_int32, _P, C.c_int64, C.c_int64, C.c_int64, _P, C.c_int64, C.c_int64,
+                                         C.c_int64, C.c_int32, _P, C.c_int32, C.c_int32, C.c_float, _P, C.c_int64, C.c_int64, _P, C.c_size_t, _P]),
     'some_profile_enable': (C.c_int, [_P, C.c_int32]),
     'some_profile_collect': (C.c_int, [_P, C.POINTER(SomeKernelStat), C.c_int32, C.POINTER(C.c_int32)]),
     'some_box_calibrate': (C.c_int, [C.c_double, _P, _P, _P, _P]),

@@ -16,8 +16,9 @@ HERE = pathlib.Path(__file__).resolve().parent
 CSRC = HERE / 'csrc'
 OBJ = CSRC / 'build'
 LIB = HERE / 'libsome_amd.so'
-SOURCES = ['api.hip', 'gemm.hip', 'gemm_f16x3.hip', 'rowops.hip', 'attention.hip', 'attention_f16x3.hip', 'dwconv.hip', 'logmel.hip', 'logmel_shift.hip', 'decode.hip', 'ingest.hip', 'train_ops.hip', 'train_attention.hip', 'train_attention_f16x3.hip', 'train_gemm16s.hip', 'train_api.hip', 'calibrate.hip']
-HEADERS = [CSRC / 'internal.h', CSRC / 'fft_core.h', CSRC / 'split.h', CSRC / 'rms_core.h', HERE.parent / 'include' / 'some_amd.h']
+SOURCES = ['api.hip', 'gemm.hip', 'gemm_f16x3.hip', 'rowops.hip', 'attention.hip', 'attention_f16x3.hip', 'dwconv.hip', 'logmel.hip', 'logmel_shift.hip', 'decode.hip', 'ingest.hip', 'train_ops.hip', 'train_attention.hip', 'train_attention_f16x3.hip', 'train_gemm16s.hip', 'train_api.hip', 'norm_rope.hip', 'causal_fwd.hip',
+           'causal_bwd.hip', 'attention_step.hip', 'causal_api.hip', 'calibrate.hip']
+HEADERS = [CSRC / 'internal.h', CSRC / 'fft_core.h', CSRC / 'split.h', CSRC / 'rms_core.h', CSRC / 'causal_core.h', HERE.parent / 'include' / 'some_amd.h']
 ARCH = 'gfx950'
 # per-source additions.  attention_f16x3.hip: without SLP vectorisation hipcc keeps the softmax's fp32 adds / multiplies scalar -
 # packed v_pk_* instructions beside MFMAs cost more than the two plain ones they replace (MI355X_MICROARCH.md, cost table)

@@ -1,0 +1,196 @@
+// Attention of ONE new frame per stream over its cache: out[b, h] = sum_j softmax_j(scale q_bh . k_j) v_j over the first lengths[b] rows of the cache of kv
+// head h / group.  Bound by reading the live rows of K and V once, so the keys are cut into chunks that fill the machine whatever the batch is:
+//   step_kernel     block = (stream, kv head, chunk).  A wave takes every NW-th 32 keys of the chunk through its own double-buffered LDS tiles (DMA, no
+//                   barrier in the loop); the heads of a group are the columns of its products, so a key is read once for all of them.  Running maximum
+//                   and sum per wave, the waves of a block joined through LDS; one chunk in all: the output, otherwise a partial (O, m, l).
+//   join_kernel     joins a stream's chunks in chunk order (the result does not depend on which block finished first).
+#include "causal_core.h"
+
+namespace {
+using namespace causal;
+
+template <typename T, int D> struct StepShape {
+    static constexpr int NW = (sizeof(T) == 4 && D == 128) ? 2 : 4;       // waves
+    static constexpr int TILE_B = 32 * D * (int)sizeof(T);
+    static constexpr int WAVE_B = 4 * TILE_B;                              // two stages of K | V
+    static constexpr int LDS_B = NW * WAVE_B;                              // >= NW * 32 * (D + 2) * 4, what the join inside a block needs
+    static_assert(LDS_B >= NW * 32 * (D + 2) * 4, "join space");
+};
+
+template <typename T, int D>
+__global__ __launch_bounds__((StepShape<T, D>::NW * 64)) void step_kernel(StepArgs a) {
+    constexpr int NW = StepShape<T, D>::NW, TILE_B = StepShape<T, D>::TILE_B, KS = D / 16, DB = D / 32;
+    typedef Tile<T, D> TL;
+    typedef typename Frag<T>::type frag;
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    const int hgs = (a.group + 31) / 32;                                   // blocks of 32 heads of a group
+    const int chunk = blockIdx.x, kvh = blockIdx.y / hgs, hg = blockIdx.y % hgs, b = blockIdx.z;
+    const int len = min(max(a.lengths[b], 0), a.capacity);
+    const int lo = chunk * a.chunk, hi_key = min(len, lo + a.chunk);
+    if (chunk > 0 && lo >= len) return;                                    // (chunk 0 of an empty stream writes its zeros)
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int l31 = lane & 31, hi = lane >> 5;
+    const int heads = min(32, a.group - 32 * hg), head0 = kvh * a.group + 32 * hg;
+    const T* qrow = static_cast<const T*>(a.q.p) + (int64_t)b * a.q.row + (int64_t)(head0 + min(l31, heads - 1)) * a.q.head + 8 * hi;
+    frag qfr[KS];
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) qfr[ks] = load8<T>(qrow + 16 * ks);
+
+    const int64_t kbytes = a.k.row * (int64_t)sizeof(T), vbytes = a.v.row * (int64_t)sizeof(T);
+    const char* kbase = reinterpret_cast<const char*>(static_cast<const T*>(a.k.p) + (int64_t)b * a.k_batch + (int64_t)kvh * a.k.head);
+    const char* vbase = reinterpret_cast<const char*>(static_cast<const T*>(a.v.p) + (int64_t)b * a.v_batch + (int64_t)kvh * a.v.head);
+    Copier<T, D, 32, 64> ck, cv;
+    ck.init(kbytes, lane);
+    cv.init(vbytes, lane);
+    char* own = lds + wave * StepShape<T, D>::WAVE_B;
+    const int ntiles = (max(0, hi_key - lo) + 31) / 32;
+    auto fetch = [&](int t, int stage) {
+        char* st = own + stage * 2 * TILE_B;
+        const int key0 = lo + t * 32;
+        ck.run(st, kbase + (int64_t)key0 * kbytes, hi_key - key0, lane);
+        cv.run(st + TILE_B, vbase + (int64_t)key0 * vbytes, hi_key - key0, lane);
+    };
+    constexpr int PER_TILE = 2 * Copier<T, D, 32, 64>::PASSES;
+
+    f32x16 o[DB];
+#pragma unroll
+    for (int d = 0; d < DB; ++d) o[d] = zero16();
+    float m = -INFINITY, l = 0.f;
+    const float c2 = a.scale * 1.4426950408889634f;
+
+    if (wave < ntiles) fetch(wave, 0);
+    int stage = 0;
+    for (int t = wave; t < ntiles; t += NW, stage ^= 1) {
+        // the tile being read next was last touched one iteration ago, by this wave alone: its reads must have returned before the copy starts
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        if (t + NW < ntiles) {
+            fetch(t + NW, stage ^ 1);
+            wait_vm<PER_TILE>();
+        } else {
+            wait_vm<0>();
+        }
+        const char* kt = own + stage * 2 * TILE_B;
+        const char* vt = kt + TILE_B;
+        f32x16 s = zero16();
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) s = mma<T>(TL::row_frag(kt, l31, ks, hi), qfr[ks], s);
+        const int key0 = lo + t * 32;
+        if (key0 + 32 > hi_key) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[r] = key0 + crow(r, hi) < hi_key ? s[r] : -INFINITY;
+        }
+        float mx = s[0];
+#pragma unroll
+        for (int r = 1; r < 16; ++r) mx = fmaxf(mx, s[r]);
+        mx = fmaxf(mx, other_half(mx));
+        if (__any(mx > m)) {
+            const float mn = fmaxf(m, mx);
+            const float f = m == -INFINITY ? 0.f : exp2_((m - mn) * c2);
+            m = mn;
+            l *= f;
+#pragma unroll
+            for (int d = 0; d < DB; ++d)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) o[d][r] *= f;
+        }
+        const float mc = m == -INFINITY ? 0.f : m * c2;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] = exp2_(fmaf(s[r], c2, -mc));
+#pragma unroll
+        for (int r = 0; r < 16; ++r) l += s[r];
+#pragma unroll
+        for (int s2 = 0; s2 < 2; ++s2) {
+            const frag p = pack8<T>(s, s2);
+#pragma unroll
+            for (int d = 0; d < DB; ++d) o[d] = mma<T>(TL::col_frag(vt, 16 * s2, d, lane), p, o[d]);
+        }
+    }
+    l += other_half(l);
+
+    // join the waves: O [wave][head][D], then m and l [wave][head]
+    __syncthreads();
+    float* ow = reinterpret_cast<float*>(lds);
+    float* ml = ow + NW * 32 * D;
+    if (l31 < heads) {
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+            for (int r4 = 0; r4 < 4; ++r4)
+                *reinterpret_cast<f32x4*>(ow + (wave * 32 + l31) * D + 32 * d + 8 * r4 + 4 * hi) = (f32x4){o[d][4 * r4], o[d][4 * r4 + 1], o[d][4 * r4 + 2], o[d][4 * r4 + 3]};
+        if (hi == 0) {
+            ml[wave * 32 + l31] = m;
+            ml[(NW + wave) * 32 + l31] = l;
+        }
+    }
+    __syncthreads();
+    for (int i = tid; i < heads * D; i += NW * 64) {
+        const int h = i / D, d = i % D;
+        float mm = -INFINITY;
+#pragma unroll
+        for (int x = 0; x < NW; ++x) mm = fmaxf(mm, ml[x * 32 + h]);
+        float acc = 0.f, ll = 0.f;
+#pragma unroll
+        for (int x = 0; x < NW; ++x) {
+            const float mx = ml[x * 32 + h];
+            const float f = mx == -INFINITY ? (ml[(NW + x) * 32 + h] == 0.f ? 0.f : 1.f) : exp2_((mx - mm) * c2);
+            acc = fmaf(ow[(x * 32 + h) * D + d], f, acc);
+            ll = fmaf(ml[(NW + x) * 32 + h], f, ll);
+        }
+        if (a.chunks == 1) {
+            const float v = len > 0 ? acc / ll : 0.f;
+            static_cast<T*>(a.out.p)[(int64_t)b * a.out.row + (int64_t)(head0 + h) * a.out.head + d] = (T)v;
+        } else {
+            const int64_t slot = ((int64_t)b * a.kv_heads * a.group + head0 + h) * a.chunks + chunk;
+            a.part_o[slot * D + d] = acc;
+            if (d == 0) {
+                a.part_ml[2 * slot] = mm * c2;
+                a.part_ml[2 * slot + 1] = ll;
+            }
+        }
+    }
+}
+
+template <typename T, int D> __global__ __launch_bounds__(D) void join_kernel(StepArgs a) {
+    const int heads = a.kv_heads * a.group, h = blockIdx.x, b = blockIdx.y, d = threadIdx.x;
+    const int len = min(max(a.lengths[b], 0), a.capacity), n = (len + a.chunk - 1) / a.chunk;
+    const int64_t slot = ((int64_t)b * heads + h) * a.chunks;
+    float mm = -INFINITY, acc = 0.f, ll = 0.f;
+    for (int i = 0; i < n; ++i) mm = fmaxf(mm, a.part_ml[2 * (slot + i)]);
+    for (int i = 0; i < n; ++i) {
+        const float mx = a.part_ml[2 * (slot + i)], lx = a.part_ml[2 * (slot + i) + 1];
+        const float f = mx == -INFINITY ? (lx == 0.f ? 0.f : 1.f) : exp2_(mx - mm);
+        acc = fmaf(a.part_o[(slot + i) * D + d], f, acc);
+        ll = fmaf(lx, f, ll);
+    }
+    static_cast<T*>(a.out.p)[(int64_t)b * a.out.row + (int64_t)h * a.out.head + d] = (T)(len > 0 ? acc / ll : 0.f);
+}
+
+template <typename T, int D> hipError_t run(const StepArgs& a, hipStream_t s) {
+    constexpr int lds = StepShape<T, D>::LDS_B;
+    static DeviceOnce once;
+    if (once.need()) {
+        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(&step_kernel<T, D>), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+        if (e != hipSuccess) return e;
+        once.mark();
+    }
+    const unsigned hgs = (unsigned)((a.group + 31) / 32);
+    hipLaunchKernelGGL((step_kernel<T, D>), dim3((unsigned)a.chunks, (unsigned)a.kv_heads * hgs, (unsigned)a.B), dim3(StepShape<T, D>::NW * 64), lds, s, a);
+    if (a.chunks > 1) hipLaunchKernelGGL((join_kernel<T, D>), dim3((unsigned)(a.kv_heads * a.group), (unsigned)a.B), dim3(D), 0, s, a);
+    return hipGetLastError();
+}
+
+}  // namespace
+
+// Chunk length: enough blocks for the machine (about 4 per CU) but no less than 128 keys, one tile per wave, and at most 1024.
+int step_chunk(int B, int kv_heads, int group, int max_len) {
+    const int64_t units = (int64_t)B * kv_heads * ((group + 31) / 32);
+    int c = 128;
+    while (c < 1024 && units * ((max_len + 2 * c - 1) / (2 * c)) >= 1024) c *= 2;
+    return c;
+}
+
+hipError_t launch_attention_step(int dtype, int head_dim, const StepArgs& a, hipStream_t s) {
+    if (a.B <= 0) return hipSuccess;
+    if (head_dim == 64) return dtype == 0 ? run<float, 64>(a, s) : dtype == 1 ? run<f16_t, 64>(a, s) : run<bf16_t, 64>(a, s);
+    return dtype == 0 ? run<float, 128>(a, s) : dtype == 1 ? run<f16_t, 128>(a, s) : run<bf16_t, 128>(a, s);
+}

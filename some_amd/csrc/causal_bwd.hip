@@ -1,0 +1,352 @@
+// Causal attention over packed clips, backward (causal_fwd.hip's mask, groups and layouts).  With s2 = scale log2(e) q.k, P = exp2(s2 - lse) is recomputed
+// tile by tile:
+//     D_i = sum_d dO O,   dV = P^T dO,   dP = dO V^T,   dS = P (dP - D),   dQ = scale dS K,   dK = scale dS^T Q     (dK, dV summed over a group's heads)
+// Two kernels, no atomics, so the gradients do not depend on the order blocks run in:
+//   causal_dq_kernel   a wave owns 32 queries (a lane's column is a query), loops over the keys they see; writes D on the way in
+//   causal_dkv_kernel  a wave owns 32 keys of one kv head (a lane's column is a key), loops over the group's heads and the queries that see them
+// In both, the recomputed tile's registers are the B operand of the products that follow (causal_core.h).
+#include "causal_core.h"
+
+namespace {
+using namespace causal;
+
+// f16 only: dS has the gradient's scale, which may lie far below (or above) f16's range.  A column's values are multiplied by a power of two F of its
+// own - constant over the contraction, so the accumulators simply carry it - that is lowered (accumulators rescaled) when a block would pass 2^14.
+template <int DB> __device__ __forceinline__ void fit_column(const f32x16& ds, float& F, f32x16 (&acc)[DB]) {
+    float mx = 0.f;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) mx = fmaxf(mx, __builtin_fabsf(ds[r]));
+    mx = fmaxf(mx, other_half(mx));
+    if (__any(mx * F > 16384.f)) {
+        if (mx * F > 16384.f) {
+            const float f = __builtin_ldexpf(1.f, min(100, max(-126, 5 - __builtin_amdgcn_frexp_expf(mx))));
+            const float ratio = f / F;
+            F = f;
+#pragma unroll
+            for (int d = 0; d < DB; ++d)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) acc[d][r] *= ratio;
+        }
+    }
+}
+constexpr float kFitStart = 0x1p100f;
+// f16 only: probabilities of long clips (about 1 / T) would be subnormal; they enter the products as 2^10 P
+template <typename T> constexpr float kProbLog2 = __is_same(T, f16_t) ? 10.f : 0.f;
+
+template <typename T> __device__ __forceinline__ void store4(T* p, float a, float b, float c, float d) {
+    if constexpr (sizeof(T) == 4) {
+        *reinterpret_cast<f32x4*>(p) = (f32x4){a, b, c, d};
+    } else {
+        *reinterpret_cast<s16x4*>(p) = (s16x4){__builtin_bit_cast(short, (T)a), __builtin_bit_cast(short, (T)b), __builtin_bit_cast(short, (T)c), __builtin_bit_cast(short, (T)d)};
+    }
+}
+
+// ---- dQ (and D) ----------------------------------------------------------------------------------------------------------------------------
+constexpr int QB = 128;
+template <typename T, int D> struct DqShape {
+    static constexpr int KT = (sizeof(T) == 4 && D == 128) ? 32 : 64;
+    static constexpr int TILE_B = KT * D * (int)sizeof(T);
+    static constexpr int LDS_B = 2 * 2 * TILE_B;
+};
+
+template <typename T, int D>
+__global__ __launch_bounds__(256, (D == 128 ? 1 : 2)) void causal_dq_kernel(CausalBwdArgs b, int nsub, int slots) {
+    constexpr int KT = DqShape<T, D>::KT, NB = KT / 32, KS = D / 16, DB = D / 32, TILE_B = DqShape<T, D>::TILE_B;
+    constexpr bool F16 = __is_same(T, f16_t);
+    typedef Tile<T, D> TL;
+    typedef typename Frag<T>::type frag;
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    const CausalArgs& a = b.f;
+
+    const Work w = find_work(a.kv_heads, nsub, a.group, slots);
+    if (w.slot < 0) return;
+    const Place pl = find_clip<QB>(a.q_offsets, a.B, w.slot);
+    const int qf = a.q_offsets[pl.b], Tq = a.q_offsets[pl.b + 1] - qf;
+    const int kf = a.k_offsets[pl.b], Tk = a.k_offsets[pl.b + 1] - kf;
+    const int q0 = pl.tile * QB;
+    if (q0 >= Tq) return;
+    const int shift = a.causal ? Tk - Tq : 0x3fffffff;
+
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int l31 = lane & 31, hi = lane >> 5;
+    const int head = w.kvh * a.group + w.g;
+    const int qw = q0 + wave * 32, q = qw + l31;
+    const int64_t qr = qf + min(q, Tq - 1);
+    const T* qrow = static_cast<const T*>(a.q.p) + qr * a.q.row + (int64_t)head * a.q.head + 8 * hi;
+    const T* grow = static_cast<const T*>(b.dout.p) + qr * b.dout.row + (int64_t)head * b.dout.head + 8 * hi;
+    const T* orow = static_cast<const T*>(a.out.p) + qr * a.out.row + (int64_t)head * a.out.head + 8 * hi;
+    frag qfr[KS], gfr[KS];
+    float dsum = 0.f;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+        qfr[ks] = load8<T>(qrow + 16 * ks);
+        gfr[ks] = load8<T>(grow + 16 * ks);
+        const frag of = load8<T>(orow + 16 * ks);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            if constexpr (sizeof(T) == 4) dsum = fmaf(gfr[ks][j], of[j], dsum);
+            else dsum = fmaf((float)__builtin_bit_cast(T, (short)gfr[ks][j]), (float)__builtin_bit_cast(T, (short)of[j]), dsum);
+        }
+    }
+    dsum += other_half(dsum);
+    const float lse = a.lse[(int64_t)head * a.q_rows + qr];
+    if (q < Tq && hi == 0) b.dsum[(int64_t)head * a.q_rows + qf + q] = dsum;
+
+    const int last_q = min(q0 + QB, Tq) - 1;
+    const int nkeys = min(Tk, max(0, last_q + shift + 1));
+    const int ntiles = (nkeys + KT - 1) / KT;
+    const int seen_w = min(Tk, max(0, min(qw + 31, Tq - 1) + shift + 1));
+    const int limit = min(q + shift, Tk - 1);
+    const int full_w = min(Tk, max(0, qw + shift + 1));
+
+    const char* kbase = reinterpret_cast<const char*>(static_cast<const T*>(a.k.p) + (int64_t)kf * a.k.row + (int64_t)w.kvh * a.k.head);
+    const char* vbase = reinterpret_cast<const char*>(static_cast<const T*>(a.v.p) + (int64_t)kf * a.v.row + (int64_t)w.kvh * a.v.head);
+    const int64_t kbytes = a.k.row * (int64_t)sizeof(T), vbytes = a.v.row * (int64_t)sizeof(T);
+    Copier<T, D, KT, 256> ck, cv;
+    ck.init(kbytes, tid);
+    cv.init(vbytes, tid);
+    auto fetch = [&](int t) {
+        char* st = lds + (t & 1) * 2 * TILE_B;
+        const int left = Tk - t * KT;
+        ck.run(st, kbase + (int64_t)(t * KT) * kbytes, left, tid);
+        cv.run(st + TILE_B, vbase + (int64_t)(t * KT) * vbytes, left, tid);
+    };
+
+    f32x16 acc[DB];
+#pragma unroll
+    for (int d = 0; d < DB; ++d) acc[d] = zero16();
+    float F = F16 ? kFitStart : 1.f;
+    const float c2 = a.scale * 1.4426950408889634f;
+
+    if (ntiles > 0) fetch(0);
+    for (int t = 0; t < ntiles; ++t) {
+        wait_vm<0>();
+        __syncthreads();
+        if (t + 1 < ntiles) fetch(t + 1);
+        const char* kt = lds + (t & 1) * 2 * TILE_B;
+        const char* vt = kt + TILE_B;
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+            const int key0 = t * KT + nb * 32;
+            if (key0 >= seen_w) break;
+            f32x16 s = zero16(), dp = zero16();
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                s = mma<T>(TL::row_frag(kt, nb * 32 + l31, ks, hi), qfr[ks], s);
+                dp = mma<T>(TL::row_frag(vt, nb * 32 + l31, ks, hi), gfr[ks], dp);
+            }
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[r] = exp2_(fmaf(s[r], c2, -lse)) * (dp[r] - dsum);
+            const bool edge = key0 + 32 > full_w;
+            if (edge) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) s[r] = key0 + crow(r, hi) <= limit ? s[r] : 0.f;
+            }
+            if constexpr (F16) {
+                fit_column<DB>(s, F, acc);
+#pragma unroll
+                for (int r = 0; r < 16; ++r) s[r] *= F;
+            }
+            if (edge && block_not_finite<T, D>(kt, nb * 32)) {
+                add_by_hand<T, D>(acc, s, kt, nb * 32, [&](int j) { return key0 + j <= limit; });
+                continue;
+            }
+#pragma unroll
+            for (int s2 = 0; s2 < 2; ++s2) {
+                const frag p = pack8<T>(s, s2);
+#pragma unroll
+                for (int d = 0; d < DB; ++d) acc[d] = mma<T>(TL::col_frag(kt, nb * 32 + 16 * s2, d, lane), p, acc[d]);
+            }
+        }
+    }
+
+    if (q < Tq) {
+        const float f = a.scale / F;
+        T* dst = static_cast<T*>(b.dq.p) + (int64_t)(qf + q) * b.dq.row + (int64_t)head * b.dq.head + 4 * hi;
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+            for (int r4 = 0; r4 < 4; ++r4) store4<T>(dst + 32 * d + 8 * r4, acc[d][4 * r4] * f, acc[d][4 * r4 + 1] * f, acc[d][4 * r4 + 2] * f, acc[d][4 * r4 + 3] * f);
+    }
+}
+
+// ---- dK, dV --------------------------------------------------------------------------------------------------------------------------------
+constexpr int KB = 128;                          // keys per workgroup
+template <typename T, int D> struct DkvShape {
+    static constexpr int QT = sizeof(T) == 4 ? 32 : 64;                    // queries per tile
+    static constexpr int TILE_B = QT * D * (int)sizeof(T);
+    static constexpr int STAGE_B = 2 * TILE_B + 2 * 64 * 4;                // Q, dO, lse, D
+    static constexpr int LDS_B = 2 * STAGE_B;
+};
+
+template <typename T, int D>
+__global__ __launch_bounds__(256, (D == 128 || sizeof(T) == 4 ? 1 : 2)) void causal_dkv_kernel(CausalBwdArgs b, int nsub, int slots) {
+    constexpr int QT = DkvShape<T, D>::QT, NB = QT / 32, KS = D / 16, DB = D / 32, TILE_B = DkvShape<T, D>::TILE_B, STAGE_B = DkvShape<T, D>::STAGE_B;
+    constexpr bool F16 = __is_same(T, f16_t);
+    typedef Tile<T, D> TL;
+    typedef typename Frag<T>::type frag;
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    const CausalArgs& a = b.f;
+
+    const Work w = find_work(a.kv_heads, nsub, 1, slots);
+    if (w.slot < 0) return;
+    const Place pl = find_clip<KB>(a.k_offsets, a.B, slots - 1 - w.slot);        // the first keys of a clip are seen by most queries: first slots first
+    const int qf = a.q_offsets[pl.b], Tq = a.q_offsets[pl.b + 1] - qf;
+    const int kf = a.k_offsets[pl.b], Tk = a.k_offsets[pl.b + 1] - kf;
+    const int k0 = pl.tile * KB;
+    if (k0 >= Tk) return;
+    const int shift = a.causal ? Tk - Tq : 0x3fffffff;
+
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int l31 = lane & 31, hi = lane >> 5;
+    const int kw = k0 + wave * 32, key = kw + l31;
+    const int64_t kr = kf + min(key, Tk - 1);
+    const T* krow = static_cast<const T*>(a.k.p) + kr * a.k.row + (int64_t)w.kvh * a.k.head + 8 * hi;
+    const T* vrow = static_cast<const T*>(a.v.p) + kr * a.v.row + (int64_t)w.kvh * a.v.head + 8 * hi;
+    frag kfr[KS], vfr[KS];
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+        kfr[ks] = load8<T>(krow + 16 * ks);
+        vfr[ks] = load8<T>(vrow + 16 * ks);
+    }
+
+    // the first query that sees key k0 is k0 - shift
+    const int t0 = max(0, k0 - shift) / QT, nt = max(0, (Tq + QT - 1) / QT - t0);
+    const int total = nt * a.group;
+    const int64_t qbytes = a.q.row * (int64_t)sizeof(T), gbytes = b.dout.row * (int64_t)sizeof(T);
+    const char* qbase = reinterpret_cast<const char*>(static_cast<const T*>(a.q.p) + (int64_t)qf * a.q.row + (int64_t)w.kvh * a.group * a.q.head);
+    const char* gbase = reinterpret_cast<const char*>(static_cast<const T*>(b.dout.p) + (int64_t)qf * b.dout.row + (int64_t)w.kvh * a.group * b.dout.head);
+    const float* lbase = a.lse + (int64_t)w.kvh * a.group * a.q_rows + qf;
+    const float* dbase = b.dsum + (int64_t)w.kvh * a.group * a.q_rows + qf;
+    Copier<T, D, QT, 256> cq, cg;
+    cq.init(qbytes, tid);
+    cg.init(gbytes, tid);
+    auto fetch = [&](int it, int g, int t) {
+        char* st = lds + (it & 1) * STAGE_B;
+        const int left = Tq - t * QT;
+        cq.run(st, qbase + (int64_t)g * a.q.head * (int64_t)sizeof(T) + (int64_t)(t * QT) * qbytes, left, tid);
+        cg.run(st + TILE_B, gbase + (int64_t)g * b.dout.head * (int64_t)sizeof(T) + (int64_t)(t * QT) * gbytes, left, tid);
+        const int row = min(lane, left - 1);
+        if (wave == 0) dma4(reinterpret_cast<const char*>(lbase + (int64_t)g * a.q_rows + t * QT + row), st + 2 * TILE_B);
+        if (wave == 1) dma4(reinterpret_cast<const char*>(dbase + (int64_t)g * a.q_rows + t * QT + row), st + 2 * TILE_B + 64 * 4);
+    };
+
+    f32x16 dk[DB], dv[DB];
+#pragma unroll
+    for (int d = 0; d < DB; ++d) {
+        dk[d] = zero16();
+        dv[d] = zero16();
+    }
+    float F = F16 ? kFitStart : 1.f;
+    const float c2 = a.scale * 1.4426950408889634f;
+
+    if (total > 0) fetch(0, 0, t0);
+    int g = 0, t = t0;
+    for (int it = 0; it < total; ++it) {
+        int gn = g, tn = t + 1;
+        if (tn == t0 + nt) { tn = t0; ++gn; }
+        wait_vm<0>();
+        __syncthreads();
+        if (it + 1 < total) fetch(it + 1, gn, tn);
+        const char* qt = lds + (it & 1) * STAGE_B;
+        const char* gt = qt + TILE_B;
+        const float* lt = reinterpret_cast<const float*>(qt + 2 * TILE_B);
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+            const int qb0 = t * QT + nb * 32;
+            if (qb0 >= Tq || qb0 + 31 + shift < kw) continue;             // nobody here / nobody sees this wave's first key
+            f32x16 s = zero16(), dp = zero16();
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                s = mma<T>(TL::row_frag(qt, nb * 32 + l31, ks, hi), kfr[ks], s);
+                dp = mma<T>(TL::row_frag(gt, nb * 32 + l31, ks, hi), vfr[ks], dp);
+            }
+            const bool edge = qb0 + shift < kw + 31 || qb0 + 32 > Tq || kw + 32 > Tk;
+#pragma unroll
+            for (int r4 = 0; r4 < 4; ++r4) {
+                const f32x4 lv = *reinterpret_cast<const f32x4*>(lt + nb * 32 + 8 * r4 + 4 * hi);
+                const f32x4 dv4 = *reinterpret_cast<const f32x4*>(lt + 64 + nb * 32 + 8 * r4 + 4 * hi);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int r = 4 * r4 + i;
+                    float p = exp2_(fmaf(s[r], c2, kProbLog2<T> - lv[i]));
+                    float d = p * (dp[r] - dv4[i]);
+                    if (edge) {
+                        const int qi = qb0 + crow(r, hi);
+                        const bool see = qi < Tq && key < Tk && key <= qi + shift;
+                        p = see ? p : 0.f;
+                        d = see ? d : 0.f;
+                    }
+                    s[r] = p;
+                    dp[r] = d;
+                }
+            }
+            if constexpr (F16) {
+                fit_column<DB>(dp, F, dk);
+#pragma unroll
+                for (int r = 0; r < 16; ++r) dp[r] *= F;
+            }
+            if (edge && (block_not_finite<T, D>(qt, nb * 32) || block_not_finite<T, D>(gt, nb * 32))) {
+                const auto see = [&](int j) { return qb0 + j < Tq && key <= qb0 + j + shift; };
+                add_by_hand<T, D>(dv, s, gt, nb * 32, see);
+                add_by_hand<T, D>(dk, dp, qt, nb * 32, see);
+                continue;
+            }
+#pragma unroll
+            for (int s2 = 0; s2 < 2; ++s2) {
+                const frag pf = pack8<T>(s, s2), df = pack8<T>(dp, s2);
+#pragma unroll
+                for (int d = 0; d < DB; ++d) {
+                    dv[d] = mma<T>(TL::col_frag(gt, nb * 32 + 16 * s2, d, lane), pf, dv[d]);
+                    dk[d] = mma<T>(TL::col_frag(qt, nb * 32 + 16 * s2, d, lane), df, dk[d]);
+                }
+            }
+        }
+        g = gn;
+        t = tn;
+    }
+
+    if (key < Tk) {
+        const float pf = F16 ? 0x1p-10f : 1.f;
+        const float fk = a.scale / F * pf;
+        T* dkd = static_cast<T*>(b.dk.p) + (int64_t)(kf + key) * b.dk.row + (int64_t)w.kvh * b.dk.head + 4 * hi;
+        T* dvd = static_cast<T*>(b.dv.p) + (int64_t)(kf + key) * b.dv.row + (int64_t)w.kvh * b.dv.head + 4 * hi;
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+            for (int r4 = 0; r4 < 4; ++r4) {
+                store4<T>(dkd + 32 * d + 8 * r4, dk[d][4 * r4] * fk, dk[d][4 * r4 + 1] * fk, dk[d][4 * r4 + 2] * fk, dk[d][4 * r4 + 3] * fk);
+                store4<T>(dvd + 32 * d + 8 * r4, dv[d][4 * r4] * pf, dv[d][4 * r4 + 1] * pf, dv[d][4 * r4 + 2] * pf, dv[d][4 * r4 + 3] * pf);
+            }
+    }
+}
+
+template <typename T, int D> hipError_t run(const CausalBwdArgs& b, hipStream_t s) {
+    const CausalArgs& a = b.f;
+    static DeviceOnce once;
+    if (once.need()) {
+        hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(&causal_dq_kernel<T, D>), hipFuncAttributeMaxDynamicSharedMemorySize, DqShape<T, D>::LDS_B);
+        if (e != hipSuccess) return e;
+        e = hipFuncSetAttribute(reinterpret_cast<const void*>(&causal_dkv_kernel<T, D>), hipFuncAttributeMaxDynamicSharedMemorySize, DkvShape<T, D>::LDS_B);
+        if (e != hipSuccess) return e;
+        once.mark();
+    }
+    const int nsub = work_subs(a.kv_heads);
+    if (a.q_rows > 0) {
+        const int slots = (int)(a.q_rows / QB) + a.B;
+        hipLaunchKernelGGL((causal_dq_kernel<T, D>), dim3((unsigned)work_blocks(a.kv_heads, a.group, slots)), dim3(256), (DqShape<T, D>::LDS_B), s, b, nsub, slots);
+    }
+    if (b.k_rows > 0) {
+        const int slots = (int)(b.k_rows / KB) + a.B;
+        hipLaunchKernelGGL((causal_dkv_kernel<T, D>), dim3((unsigned)work_blocks(a.kv_heads, 1, slots)), dim3(256), (DkvShape<T, D>::LDS_B), s, b, nsub, slots);
+    }
+    return hipGetLastError();
+}
+
+}  // namespace
+
+hipError_t launch_causal_bwd(int dtype, int head_dim, const CausalBwdArgs& b, hipStream_t s) {
+    if (b.f.B <= 0) return hipSuccess;
+    if (head_dim == 64) return dtype == 0 ? run<float, 64>(b, s) : dtype == 1 ? run<f16_t, 64>(b, s) : run<bf16_t, 64>(b, s);
+    return dtype == 0 ? run<float, 128>(b, s) : dtype == 1 ? run<f16_t, 128>(b, s) : run<bf16_t, 128>(b, s);
+}

@@ -1,0 +1,254 @@
+// Shared pieces of the causal attention kernels over packed clips (causal_fwd.hip, causal_bwd.hip, attention_step.hip): element types, the
+// LDS tile format with its two fragment reads, the global -> LDS copy and the block -> (clip, tile, head) map.
+//
+// All matrix products are 32 x 32 tiles with a contraction of 16 (v_mfma_f32_32x32x16 for f16 / bf16; for f32 eight v_mfma_f32_32x32x2_f32 on the
+// same fragments).  Lane l = (l31 = l & 31, hi = l >> 5):
+//     A / B fragment: 8 values, row (column) l31, contraction slots 8 hi + j          C / D register r: column l31, row crow(r, hi)
+// A contraction may run in any order as long as both operands agree, so the C registers 8 s .. 8 s + 7 of one product ARE the B fragment of the
+// next one when its A fragment takes the rows 16 s + (j & 3) + 8 (j >> 2) + 4 hi in slot j: probabilities never leave their registers.
+#pragma once
+#include "internal.h"
+
+namespace causal {
+
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x8 __attribute__((ext_vector_type(8)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16_t;
+typedef _Float16 f16_t;
+
+template <typename T> struct Frag { typedef s16x8 type; };
+template <> struct Frag<float> { typedef f32x8 type; };
+
+__device__ __forceinline__ int crow(int r, int hi) { return (r & 3) + 8 * (r >> 2) + 4 * hi; }
+
+// (plain functions: hipcc drops the host stub of a kernel template that holds these builtins in a dependent context)
+__device__ __forceinline__ f32x16 mma_bf16(s16x8 a, s16x8 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x16 mma_f16(s16x8 a, s16x8 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x16 mma_f32(f32x8 a, f32x8 b, f32x16 c) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[j], b[j], c, 0, 0, 0);
+    return c;
+}
+template <typename T> __device__ __forceinline__ f32x16 mma(typename Frag<T>::type a, typename Frag<T>::type b, f32x16 c) {
+    if constexpr (sizeof(T) == 4) return mma_f32(a, b, c);
+    else if constexpr (__is_same(T, bf16_t)) return mma_bf16(a, b, c);
+    else return mma_f16(a, b, c);
+}
+__device__ __forceinline__ s16x4 tr_read(const char* p) {
+    typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+    return __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(uintptr_t)p);
+}
+__device__ __forceinline__ void dma16(const char* src, char* lds_dst) {
+    typedef __attribute__((address_space(3))) void lds_void;
+    __builtin_amdgcn_global_load_lds(src, (lds_void*)(uintptr_t)lds_dst, 16, 0, 0);
+}
+__device__ __forceinline__ void dma4(const char* src, char* lds_dst) {
+    typedef __attribute__((address_space(3))) void lds_void;
+    __builtin_amdgcn_global_load_lds(src, (lds_void*)(uintptr_t)lds_dst, 4, 0, 0);
+}
+template <int N> __device__ __forceinline__ void wait_vm() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
+__device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
+__device__ __forceinline__ float log2_(float x) { return __builtin_amdgcn_logf(x); }
+__device__ __forceinline__ float other_half(float x) { return __shfl_xor(x, 32, 64); }
+__device__ __forceinline__ f32x16 zero16() {
+    f32x16 z;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) z[r] = 0.f;
+    return z;
+}
+
+// registers 8 s .. 8 s + 7 of a product as a fragment, rounded to the operand type (16-bit: half an ulp, 2^-9 / 2^-12 of the value)
+template <typename T> __device__ __forceinline__ typename Frag<T>::type pack8(const f32x16& x, int s) {
+    typename Frag<T>::type f;
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) f[j] = x[8 * s + j];
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) f[j] = __builtin_bit_cast(short, (T)x[8 * s + j]);
+    }
+    return f;
+}
+template <typename T> __device__ __forceinline__ float to_f32(T x) { return (float)x; }
+
+// 8 consecutive values of a row in global memory as a fragment
+template <typename T> __device__ __forceinline__ typename Frag<T>::type load8(const T* p) {
+    if constexpr (sizeof(T) == 4) {
+        const f32x4 a = *reinterpret_cast<const f32x4*>(p), b = *reinterpret_cast<const f32x4*>(p + 4);
+        return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+    } else {
+        return *reinterpret_cast<const s16x8*>(p);
+    }
+}
+template <typename T> __device__ __forceinline__ typename Frag<T>::type zero8() {
+    typename Frag<T>::type f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) f[j] = 0;
+    return f;
+}
+
+// ---- LDS tiles: ROWS rows of D values, row pitch D sizeof(T) bytes, 16-byte chunk c of row r stored at chunk c ^ swz(r) --------------------
+// The copy global -> LDS writes lane-linear chunks, so the permutation is applied to its per-lane source address.  swz is chosen so that both
+// reads touch every LDS bank equally often: row fragments (32 rows, one chunk) and column fragments (ds_read_b64_tr_b16: 8 rows x 64 bytes; f32:
+// rows r and r + 4 x 128 bytes).
+template <typename T, int D> struct Tile {
+    static constexpr int PITCH = D * (int)sizeof(T);
+    static constexpr int CHUNKS = PITCH / 16;
+
+    static __device__ __forceinline__ int swz(int r) {
+        if constexpr (sizeof(T) == 4) return ((r & 4) << 1) | ((r & 3) << 1) | ((r >> 3) & 1);
+        else if constexpr (CHUNKS == 8) return r & 7;
+        else return ((r & 3) << 2) | ((r >> 2) & 3);
+    }
+    // fragment of row `row` (any row = 32 n + l31): values 16 ks + 8 hi .. + 7
+    static __device__ __forceinline__ typename Frag<T>::type row_frag(const char* tile, int row, int ks, int hi) {
+        const char* p = tile + row * PITCH;
+        const int x = swz(row);
+        if constexpr (sizeof(T) == 4) {
+            const f32x4 a = *reinterpret_cast<const f32x4*>(p + (((4 * ks + 2 * hi) ^ x) << 4));
+            const f32x4 b = *reinterpret_cast<const f32x4*>(p + (((4 * ks + 2 * hi + 1) ^ x) << 4));
+            return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+        } else {
+            return *reinterpret_cast<const s16x8*>(p + (((2 * ks + hi) ^ x) << 4));
+        }
+    }
+    // fragment of column 32 db + l31: slot j holds row r0 + (j & 3) + 8 (j >> 2) + 4 hi (r0 a multiple of 16)
+    static __device__ __forceinline__ typename Frag<T>::type col_frag(const char* tile, int r0, int db, int lane) {
+        const int hi = lane >> 5;
+        typename Frag<T>::type f;
+        if constexpr (sizeof(T) == 4) {
+            const int c = 8 * db + ((lane & 31) >> 2);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int row = r0 + (j & 3) + 8 * (j >> 2) + 4 * hi;
+                f[j] = *reinterpret_cast<const float*>(tile + row * PITCH + ((c ^ swz(row)) << 4) + (lane & 3) * 4);
+            }
+        } else {
+            // 16 lanes read a 4 x 16 block transposed: lane i supplies 4 values of row i >> 2, receives column i
+            const int row = r0 + 4 * hi + ((lane & 15) >> 2), c = 4 * db + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
+            const s16x4 a = tr_read(tile + row * PITCH + ((c ^ swz(row)) << 4) + (lane & 1) * 8);
+            const s16x4 b = tr_read(tile + (row + 8) * PITCH + ((c ^ swz(row + 8)) << 4) + (lane & 1) * 8);
+            f = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+        }
+        return f;
+    }
+};
+
+// Copy of ROWS consecutive rows (one tile) global -> LDS by NT threads.  The tile's first row is a wave-uniform pointer, a lane's place in the tile
+// a 32-bit offset that never changes (the host refuses row strides whose tile would not fit 31 bits).  Rows at or past `rows` are copies of the
+// last real one: finite or not, whoever reads them masks them, and no address leaves the matrix.
+template <typename T, int D, int ROWS, int NT> struct Copier {
+    typedef Tile<T, D> TL;
+    static constexpr int PASSES = ROWS * TL::CHUNKS / NT;
+    static_assert(PASSES * NT == ROWS * TL::CHUNKS, "whole passes");
+    uint32_t off[PASSES];
+    uint32_t row_bytes;
+
+    __device__ __forceinline__ void init(int64_t stride_bytes, int tid) {
+        row_bytes = (uint32_t)stride_bytes;
+#pragma unroll
+        for (int p = 0; p < PASSES; ++p) off[p] = place(p * NT + tid, ROWS);
+    }
+    __device__ __forceinline__ uint32_t place(int L, int rows) const {
+        const int row = L / TL::CHUNKS, slot = L % TL::CHUNKS;
+        return (uint32_t)min(row, rows - 1) * row_bytes + (uint32_t)((slot ^ TL::swz(row)) << 4);
+    }
+    __device__ __forceinline__ void run(char* tile, const char* first, int rows, int tid) const {
+        const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+#pragma unroll
+        for (int p = 0; p < PASSES; ++p) {
+            const uint32_t o = rows >= ROWS ? off[p] : place(p * NT + tid, rows);
+            dma16(first + o, tile + (p * NT + wave * 64) * 16);
+        }
+    }
+};
+
+// ---- not-a-number and infinities in masked places ----------------------------------------------------------------------------------------------
+// A masked weight is 0, and 0 * inf would reach the sum.  Only a 32 x 32 block on the diagonal (or at a clip's end) mixes masked and visible places;
+// if the 32 tile rows it contracts over hold such a value, the block's product is summed by hand over the visible ones.
+template <typename T, int D> __device__ __noinline__ bool block_not_finite(const char* tile, int r0) {
+    typedef Tile<T, D> TL;
+    const int lane = threadIdx.x & 63;
+    bool bad = false;
+    for (int i = lane; i < 32 * TL::CHUNKS; i += 64) {
+        const uint4 w = *reinterpret_cast<const uint4*>(tile + (r0 + i / TL::CHUNKS) * TL::PITCH + (i % TL::CHUNKS) * 16);
+        const uint32_t x[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            if constexpr (sizeof(T) == 4) bad |= (x[k] & 0x7f800000u) == 0x7f800000u;
+            else {
+                constexpr uint32_t E = __is_same(T, bf16_t) ? 0x7f80u : 0x7c00u;
+                bad |= (x[k] & E) == E || ((x[k] >> 16) & E) == E;
+            }
+        }
+    }
+    return __any(bad);
+}
+// acc[column l31] += sum over the tile rows r0 + j the column sees of w[j] * row, w in the registers of a product (row crow(r, hi) <-> j)
+template <typename T, int D, typename See>
+__device__ __forceinline__ void add_by_hand(f32x16 (&acc)[D / 32], const f32x16& w, const char* tile, int r0, See see) {
+    typedef Tile<T, D> TL;
+    constexpr int PER = 16 / (int)sizeof(T);
+    const int lane = threadIdx.x & 63, l31 = lane & 31, hi = lane >> 5;
+    for (int j = 0; j < 32; ++j) {
+        const int r = (j & 3) + 4 * (j >> 3), h = (j >> 2) & 1;          // crow(r, h) == j
+        float p = 0.f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) p = i == r ? w[i] : p;
+        p = __shfl(p, l31 + 32 * h, 64);
+        const bool visible = see(j);
+        const int row = r0 + j;
+#pragma unroll
+        for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const int col = 32 * d + crow(i, hi);
+                const float v = to_f32(*reinterpret_cast<const T*>(tile + row * TL::PITCH + (((col / PER) ^ TL::swz(row)) << 4) + (col % PER) * (int)sizeof(T)));
+                if (visible) acc[d][i] = fmaf(p, v, acc[d][i]);
+            }
+    }
+}
+
+// ---- block map ------------------------------------------------------------------------------------------------------------------------
+// Rows are packed: clip b owns rows [off[b], off[b + 1]).  Tiles of TR rows: clip b's first tile sits in slot off[b] / TR + b, so `rows / TR + B` slots
+// hold every clip's tiles without a table, and a block finds its clip by counting the clips that begin at or before its slot (64 per step).
+struct Place { int b, tile; };
+template <int TR> __device__ __forceinline__ Place find_clip(const int32_t* __restrict__ off, int B, int slot) {
+    const int lane = threadIdx.x & 63;
+    int n = 0;
+    for (int base = 0; base < B; base += 64) {
+        const int b = base + lane;
+        const bool below = b < B && off[b] / TR + b <= slot;
+        const int c = __popcll(__ballot(below));
+        n += c;
+        if (c < 64) break;
+    }
+    const int b = n > 0 ? n - 1 : 0;
+    return {__builtin_amdgcn_readfirstlane(b), __builtin_amdgcn_readfirstlane(slot - (off[b] / TR + b))};
+}
+// blockIdx -> (kv head, slot, head of the group): the blocks of one kv head run on as few of the 8 XCDs as balance allows (they read the same K
+// and V through that XCD's L2), neighbouring slots at the same time, the last slot of the packed rows first (a clip's last tile sees most keys).
+struct Work { int kvh, slot, g; };
+inline int work_subs(int kv_heads) { return (kv_heads & 1) ? 8 : (kv_heads & 2) ? 4 : (kv_heads & 4) ? 2 : 1; }
+inline int64_t work_blocks(int kv_heads, int per_slot, int slots) {
+    const int nsub = work_subs(kv_heads);
+    return 8ll * (kv_heads * nsub / 8) * per_slot * ((slots + nsub - 1) / nsub);
+}
+__device__ __forceinline__ Work find_work(int kv_heads, int nsub, int per_slot, int slots) {
+    const int xcd = blockIdx.x & 7, j = blockIdx.x >> 3;
+    const int upx = kv_heads * nsub / 8;
+    const int g = j % per_slot, t = j / per_slot;
+    const int u = (t % upx) * 8 + xcd;
+    const int s = (t / upx) * nsub + u % nsub;
+    return {u / nsub, slots - 1 - s, g};
+}
+
+}  // namespace causal

@@ -169,6 +169,51 @@ constexpr int kClipAlign = SOME_CLIP_ALIGN;
 inline int64_t attn_rows_cover(int64_t M, int64_t B) { return (M + (kClipAlign - 1) * B + 63 + 63) / 64 * 64; }
 hipError_t launch_attn_plan(const int32_t* frame_offsets, int B, int rows_cover, int32_t* pad_offsets, int32_t* row_map, hipStream_t s);
 
+// ---- causal attention over packed clips (causal_fwd.hip, causal_bwd.hip, attention_step.hip) and the norm + rotation in front of it (norm_rope.hip) ----
+// dtype: 0 f32, 1 f16, 2 bf16 (SOME_DTYPE_*).  Rows3: [rows, heads, head_dim], head_dim contiguous; strides in elements.
+struct Rows3 { void* p; int64_t row, head; };
+struct CausalArgs {
+    Rows3 q, k, v, out;
+    float* lse;                    // optional [heads, q_rows]: base-2 log-sum-exp of the scaled scores (-inf: no visible key)
+    const int32_t* q_offsets; const int32_t* k_offsets;
+    int64_t q_rows;
+    int B, kv_heads, group, causal;
+    float scale;
+};
+struct CausalBwdArgs {
+    CausalArgs f;                  // as in the forward call (out and lse read)
+    Rows3 dout, dq, dk, dv;
+    float* dsum;                   // [heads, q_rows] scratch: rowsum(dout out)
+    int64_t k_rows;
+};
+struct StepArgs {
+    Rows3 q, k, v, out;            // q, out: row = stream; k, v: row = frame of a stream's cache, the streams k_batch / v_batch apart
+    int64_t k_batch, v_batch;
+    const int32_t* lengths;
+    float* part_o; float* part_ml; // chunks > 1: [B, heads, chunks, head_dim], [B, heads, chunks, 2] (base-2 maximum, sum)
+    int B, capacity, kv_heads, group, chunk, chunks;
+    float scale;
+};
+int step_chunk(int B, int kv_heads, int group, int max_len);
+hipError_t launch_attention_step(int dtype, int head_dim, const StepArgs& a, hipStream_t s);
+struct NormRopeArgs {
+    Rows3 q, k, q_out, k_out;      // forward: x -> y; backward: x, dx
+    Rows3 dq_in, dk_in;            // backward: dy
+    const float* gamma_q; const float* gamma_k;
+    const void* positions;         // [rows] int32, or int64 if positions64
+    float* partial;                // backward: [blocks, 2, head_dim]
+    int64_t rows;
+    int heads, kv_heads, positions64, parts;
+    float eps;
+    double turns[64];              // theta^(-2 i / head_dim) / (2 pi)
+};
+int norm_rope_bwd_blocks(int64_t rows, int heads, int head_dim);
+hipError_t launch_norm_rope(int dtype, int head_dim, NormRopeArgs a, hipStream_t s);
+hipError_t launch_norm_rope_bwd(int dtype, int head_dim, NormRopeArgs a, float* dgq, float* dgk, int accumulate, hipStream_t s);
+int64_t causal_fwd_blocks(const CausalArgs& a);
+hipError_t launch_causal_fwd(int dtype, int head_dim, const CausalArgs& a, hipStream_t s);
+hipError_t launch_causal_bwd(int dtype, int head_dim, const CausalBwdArgs& a, hipStream_t s);
+
 // ---- depthwise conv + folded BN + SiLU ------------------------------------------------------------
 struct DwArgs {
     const float* x[kStreams];      // [M, 512] (GLU output)

@@ -11,7 +11,7 @@ from typing import Dict, List, Mapping, Optional, Sequence
 import numpy as np
 import torch
 
-from . import _lib
+from . import _lib, causal
 
 
 def make_some_config(config: dict) -> _lib.SomeConfig:
@@ -312,6 +312,51 @@ class Engine:
             1 if quantized else 0, _ptr(out['note_midi']), _ptr(out['note_dur']), _ptr(out['note_rest']),
             _ptr(out['n_notes']), _ptr(f2i), _ptr(val), _ptr(rest), _ptr(sc), sc.numel(), self._stream()))
         return out
+
+    # ---- causal attention over packed clips (some_amd/causal.py; the differentiable forms are TrainOps') ----------------------------
+    def _raw_stream(self):
+        return torch.cuda.current_stream(self.device).cuda_stream
+
+    def _serve(self):
+        if self.host_only:
+            raise RuntimeError('a host-only engine runs no device operators')
+        return _lib.fast(), getattr(self.handle, 'value', self.handle)
+
+    def qk_norm_rope(self, q: torch.Tensor, k: torch.Tensor, gamma_q: torch.Tensor, gamma_k: torch.Tensor, positions: torch.Tensor,
+                     theta: float = 10000.0, eps: float = 1e-6):
+        """Norm of queries and keys for each head and the position rotation in one pass: q [rows, heads, D], k [rows, kv_heads, D] (or
+        [rows, heads * D]), gains fp32 [D], positions int32 / int64 [rows] (``causal.frame_positions(batch)`` for whole clips).  Channels i
+        and i + D / 2 of x rsqrt(mean(x^2) + eps) gamma are rotated by position theta^(-2 i / D).  Returns new (q, k) of the inputs' shapes."""
+        lib, h = self._serve()
+        q3, k3 = causal.check_norm_rope(self.device, q, k, gamma_q, gamma_k, positions)
+        causal.no_gradient_lost('Engine.qk_norm_rope', q, k, gamma_q, gamma_k)
+        with causal.on_device(q3):
+            yq, yk = causal.norm_rope_forward(lib, h, self._raw_stream(), q3, k3, gamma_q, gamma_k, positions, theta, eps)
+        return yq.view(q.shape), yk.view(k.shape)
+
+    def causal_attention(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, batch: ClipBatch, kv_batch: Optional[ClipBatch] = None,
+                         causal_mask: bool = True, scale: Optional[float] = None, head_dim: int = 0) -> torch.Tensor:
+        """Attention over packed clips that looks back only: q [total_frames, heads, D], k and v [.., kv_heads, D] (2-D with ``head_dim``), heads
+        a multiple of kv_heads.  ``kv_batch``: keys and values of another (longer) stretch of the same clips - the queries are then each
+        clip's last frames, e.g. a new chunk over what is cached.  ``causal_mask=False``: every frame of the clip.  A frame that sees no key
+        gets 0.  scale: default D ** -0.5."""
+        lib, h = self._serve()
+        q3, k3, v3, kv = causal.check_attention(self.device, q, k, v, batch, kv_batch, head_dim)
+        causal.no_gradient_lost('Engine.causal_attention', q, k, v)
+        scale = causal.default_scale(scale, q3.shape[2])
+        with causal.on_device(q3):
+            out, _ = causal.attention_forward(lib, h, self._raw_stream(), causal.readable(q3), causal.readable(k3), causal.readable(v3), batch, kv,
+                                              causal_mask, scale, False)
+        return out.view(q.shape)
+
+    def attention_step(self, q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, lengths: torch.Tensor,
+                       max_length: Optional[int] = None, scale: Optional[float] = None) -> torch.Tensor:
+        """The next frame of B live streams: q [B, heads, D] over the first lengths[b] (int32 [B], on the device) rows of the caches
+        [B, capacity, kv_heads, D] - the new frame's key and value among them.  ``max_length``: an upper bound of the lengths, if the caller
+        knows one below the capacity (lengths beyond it are cut).  Returns [B, heads, D]; a stream of length 0 gets 0."""
+        lib, h = self._serve()
+        causal.no_gradient_lost('Engine.attention_step', q, k_cache, v_cache)
+        return causal.attention_step(lib, h, self._raw_stream, self.device, q, k_cache, v_cache, lengths, max_length, scale)
 
     # ---- graph replay of a whole step ------------------------------------------------------------
     def graph_runner(self, audio: torch.Tensor, batch: ClipBatch, head_mode: int = _lib.HEAD_LOGITS, quantized: bool = False,

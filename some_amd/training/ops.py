@@ -9,8 +9,9 @@ from typing import Dict, Optional
 
 import numpy as np
 import torch
+from torch.autograd.function import once_differentiable
 
-from .. import _lib
+from .. import _lib, causal
 from ..engine import Engine
 
 
@@ -736,6 +737,19 @@ class TrainOps:
         """F.scaled_dot_product_attention on the fused projection qkv [M, 1536] -> merged heads [M, 512]."""
         return self._apply(_Attention, qkv, batch)
 
+    def qk_norm_rope(self, q, k, gamma_q, gamma_k, positions, theta: float = 10000.0, eps: float = 1e-6):
+        """Norm of queries and keys for each head and the position rotation in one pass (``Engine.qk_norm_rope``), differentiable in q, k and the
+        gains: -> (q, k) of the inputs' shapes."""
+        causal.check_norm_rope(self.device, q, k, gamma_q, gamma_k, positions)
+        return self._apply(_QkNormRope, q, k, gamma_q, gamma_k, positions, float(theta), float(eps))
+
+    def causal_attention(self, q, k, v, batch, kv_batch=None, causal_mask: bool = True, scale: Optional[float] = None, head_dim: int = 0):
+        """Attention over packed clips that looks back only, heads in groups (``Engine.causal_attention``), differentiable in q, k and v; takes and
+        returns float32, float16 or bfloat16 (in float16, gradients of any magnitude are carried at full precision)."""
+        q3, _, _, kv = causal.check_attention(self.device, q, k, v, batch, kv_batch, head_dim)
+        return self._apply(_CausalAttention, q, k, v, batch, kv, bool(causal_mask), causal.default_scale(scale, q3.shape[2]),
+                           q3.shape[2])
+
     def bce_with_logits(self, logits, target):
         return self._apply(_Bce, logits, target)
 
@@ -787,11 +801,13 @@ class Tape:
         ctx.needs_input_grad = needs = tuple(isinstance(a, torch.Tensor) and (a.requires_grad or id(a) in produced) for a in args)
         out = fn.forward(ctx, *args)
         ops._lane_version[lane] += 1
-        if ops.lanes == 2 and isinstance(out, torch.Tensor):
-            self.lane_of[id(out)] = (lane, ops._lane_version[lane])
+        for o in out if isinstance(out, tuple) else (out,):
+            if ops.lanes == 2 and isinstance(o, torch.Tensor):
+                self.lane_of[id(o)] = (lane, ops._lane_version[lane])
+            if True in needs:
+                produced.add(id(o))
         if True in needs:
             self.records.append((fn, ctx, args, out, lane))
-            produced.add(id(out))
         return out
 
     def backward(self, seeds):
@@ -817,15 +833,15 @@ class Tape:
     def _walk(records, ops, two, grads):
         while records:
             fn, ctx, args, out, lane = records.pop()            # releases the saved activations as the pass moves on
-            entry = grads.pop(id(out), None)
-            if entry is None:
+            entries = [grads.pop(id(o), None) for o in (out if isinstance(out, tuple) else (out,))]
+            if not any(entries):
                 continue                                        # an output nothing differentiable consumed
-            g, g_lane = entry
             if two and lane != ops._lane:
                 ops._enter_lane(lane)
-            if g_lane != lane and isinstance(g, torch.Tensor):
-                ops.adopt(g, g_lane)
-            results = fn.backward(ctx, g)
+            for e in entries:
+                if e is not None and e[1] != lane and isinstance(e[0], torch.Tensor):
+                    ops.adopt(*e)
+            results = fn.backward(ctx, *(None if e is None else e[0] for e in entries))
             ops._lane_version[lane] += 1
             for a, ga, need in zip(args, results, ctx.needs_input_grad):
                 if ga is None or not need:
@@ -1232,6 +1248,63 @@ def _attention_bwd16(ctx, dout):
     ops.check(ops.lib.some_train_attention_bwd_f16x3_auto16(ops.h, _p(R), _p(Rt), _p(out), _p(dout), _p(lse), _p(batch.frame_offsets_dev), batch.B,
                                                             batch.max_frames, M, Mp, ops._hi_mode, _p(dqkv16), _p(work), work.numel(), ops.stream()))
     return dqkv16
+
+
+class _QkNormRope(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, ops, q, k, gamma_q, gamma_k, positions, theta, eps):
+        D = gamma_q.shape[0]
+        q3, k3 = causal.heads_view(q, 'q', D), causal.heads_view(k, 'k', D)
+        with causal.on_device(q3):
+            yq, yk = causal.norm_rope_forward(ops.lib, ops.h, ops.stream(), q3, k3, gamma_q, gamma_k, positions, theta, eps)
+        ctx.ops, ctx.theta, ctx.eps = ops, theta, eps
+        ctx.gparams = gamma_q, gamma_k                            # identities only: looked up among the gradient sinks in backward
+        ctx.shapes = q.shape, k.shape
+        ctx.save_for_backward(q3, k3, gamma_q, gamma_k, positions)
+        return yq.view(q.shape), yk.view(k.shape)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dyq, dyk):
+        ops: TrainOps = ctx.ops
+        q, k, gamma_q, gamma_k, positions = ctx.saved_tensors
+        dyq = torch.zeros_like(q, memory_format=torch.contiguous_format) if dyq is None else dyq.reshape(q.shape)
+        dyk = torch.zeros_like(k, memory_format=torch.contiguous_format) if dyk is None else dyk.reshape(k.shape)
+        pq, pk = ctx.gparams
+        sq, sk = ops.sink(pq), ops.sink(pk)
+        sunk = sq is not None and sk is not None and sq is not sk and ctx.needs_input_grad[3] and ctx.needs_input_grad[4]
+        dgq, dgk = (sq, sk) if sunk else (torch.empty_like(gamma_q), torch.empty_like(gamma_k))
+        with causal.on_device(q):
+            dq, dk = causal.norm_rope_backward(ops.lib, ops.h, ops.stream(), q, k, gamma_q, gamma_k, positions, ctx.theta, ctx.eps, dyq, dyk, dgq, dgk, sunk)
+        if sunk:
+            ops.deposited(pq)
+            ops.deposited(pk)
+            dgq = dgk = None
+        return None, dq.view(ctx.shapes[0]), dk.view(ctx.shapes[1]), dgq, dgk, None, None, None
+
+
+class _CausalAttention(torch.autograd.Function):
+    """Forward keeps q, k, v, the output and the log-sum-exp; backward recomputes the probabilities (csrc/causal_bwd.hip)."""
+
+    @staticmethod
+    def forward(ctx, ops, q, k, v, batch, kv, causal_mask, scale, head_dim):
+        q3, k3, v3 = (causal.readable(causal.heads_view(t, n, head_dim)) for t, n in ((q, 'q'), (k, 'k'), (v, 'v')))
+        with causal.on_device(q3):
+            out, lse = causal.attention_forward(ops.lib, ops.h, ops.stream(), q3, k3, v3, batch, kv, causal_mask, scale, True)
+        ctx.ops, ctx.batch, ctx.kv, ctx.causal_mask, ctx.scale = ops, batch, kv, causal_mask, scale
+        ctx.shapes = q.shape, k.shape, v.shape
+        ctx.save_for_backward(q3, k3, v3, out, lse)
+        return out.view(q.shape)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout):
+        ops: TrainOps = ctx.ops
+        q, k, v, out, lse = ctx.saved_tensors
+        with causal.on_device(q):
+            dq, dk, dv = causal.attention_backward(ops.lib, ops.h, ops.stream(), q, k, v, ctx.batch, ctx.kv, ctx.causal_mask, ctx.scale, out, lse,
+                                                   dout.reshape(q.shape))
+        return (None, dq.view(ctx.shapes[0]), dk.view(ctx.shapes[1]), dv.view(ctx.shapes[2])) + (None,) * 5
 
 
 class _Bce(torch.autograd.Function):
