@@ -170,20 +170,22 @@ def attention_forward(lib, h, stream, q, k, v, batch, kv, causal, scale, want_ls
     """Launch on checked, readable views -> (out, lse or None)."""
     out = q.new_empty(q.shape)
     lse = torch.empty((q.shape[1], q.shape[0]), dtype=torch.float32, device=q.device) if want_lse else None
+    n = lib.some_op_causal_attention_bytes(h, q.shape[1], k.shape[1], q.shape[2], batch.B, q.shape[0], k.shape[0])
+    work = torch.empty(n, dtype=torch.uint8, device=q.device) if n else None
     _lib.check(h, lib.some_op_causal_attention(h, DTYPES[q.dtype], q.shape[2], *_rows(q), q.shape[1], *_rows(k), *_rows(v), k.shape[1],
                                                batch.frame_offsets_dev.data_ptr(), kv.frame_offsets_dev.data_ptr(), batch.B, q.shape[0], k.shape[0],
-                                               int(causal), scale, *_rows(out), lse.data_ptr() if want_lse else None, stream))
+                                               int(causal), scale, *_rows(out), lse.data_ptr() if want_lse else None, work.data_ptr() if n else None, n, stream))
     return out, lse
 
 
 def attention_backward(lib, h, stream, q, k, v, batch, kv, causal, scale, out, lse, dout):
     dout = readable(dout)
     dq, dk, dv = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
-    dsum = torch.empty_like(lse)
+    work = torch.empty(lib.some_train_causal_attention_bytes(h, q.shape[1], k.shape[1], q.shape[2], batch.B, q.shape[0], k.shape[0]), dtype=torch.uint8, device=q.device)
     _lib.check(h, lib.some_train_causal_attention_bwd(h, DTYPES[q.dtype], q.shape[2], *_rows(q), q.shape[1], *_rows(k), *_rows(v), k.shape[1],
                                                       batch.frame_offsets_dev.data_ptr(), kv.frame_offsets_dev.data_ptr(), batch.B, q.shape[0], k.shape[0],
                                                       int(causal), scale, *_rows(out), lse.data_ptr(), *_rows(dout), *_rows(dq), *_rows(dk), *_rows(dv),
-                                                      dsum.data_ptr(), stream))
+                                                      work.data_ptr(), work.numel(), stream))
     return dq, dk, dv
 
 

@@ -82,7 +82,7 @@ __global__ __launch_bounds__((StepShape<T, D>::NW * 64)) void step_kernel(StepAr
         float mx = s[0];
 #pragma unroll
         for (int r = 1; r < 16; ++r) mx = fmaxf(mx, s[r]);
-        mx = fmaxf(mx, other_half(mx));
+        mx = halves_max(mx);
         if (__any(mx > m)) {
             const float mn = fmaxf(m, mx);
             const float f = m == -INFINITY ? 0.f : exp2_((m - mn) * c2);
@@ -105,7 +105,7 @@ __global__ __launch_bounds__((StepShape<T, D>::NW * 64)) void step_kernel(StepAr
             for (int d = 0; d < DB; ++d) o[d] = mma<T>(TL::col_frag(vt, 16 * s2, d, lane), p, o[d]);
         }
     }
-    l += other_half(l);
+    l = halves_sum(l);
 
     // join the waves: O [wave][head][D], then m and l [wave][head]
     __syncthreads();

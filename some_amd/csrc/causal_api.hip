@@ -35,6 +35,8 @@ const char* kLayout = "arrays must be 16-byte aligned, strides non-negative mult
 
 Rows3 rows3(const void* p, int64_t row, int64_t head) { return {const_cast<void*>(p), row, head}; }
 
+size_t dsum_bytes(int heads, int64_t q_rows) { return ((size_t)heads * q_rows * sizeof(float) + 255) / 256 * 256 + 256; }
+
 bool fill_turns(NormRopeArgs& a, double theta, int head_dim) {
     if (!(theta > 0.0) || !std::isfinite(theta)) return false;
     for (int i = 0; i < head_dim / 2; ++i) a.turns[i] = std::pow(theta, -2.0 * i / head_dim) / 6.283185307179586476925286766559;
@@ -109,10 +111,25 @@ int some_train_qk_norm_rope_bwd(SomeHandle* h, int32_t dtype, int32_t head_dim, 
     return SOME_OK;
 }
 
+size_t some_op_causal_attention_bytes(const SomeHandle* h, int32_t heads, int32_t kv_heads, int32_t head_dim, int32_t B, int64_t q_rows, int64_t k_rows) {
+    (void)h;
+    if (!heads_ok(heads, kv_heads) || head_dim <= 0 || B <= 0 || q_rows <= 0 || k_rows <= 0 || q_rows >= kMaxRows || k_rows >= kMaxRows) return 0;
+    const int parts = causal_fwd_parts(q_rows, k_rows, B, heads);
+    return parts > 1 ? (size_t)parts * q_rows * heads * (head_dim + 2) * sizeof(float) : 0;
+}
+
+size_t some_train_causal_attention_bytes(const SomeHandle* h, int32_t heads, int32_t kv_heads, int32_t head_dim, int32_t B, int64_t q_rows, int64_t k_rows) {
+    (void)h;
+    if (!heads_ok(heads, kv_heads) || head_dim <= 0 || B <= 0 || q_rows < 0 || k_rows < 0 || q_rows >= kMaxRows || k_rows >= kMaxRows) return 256;
+    const int parts = causal_bwd_parts(q_rows, k_rows, B, heads, kv_heads);
+    return dsum_bytes(heads, q_rows) + (parts > 1 ? (size_t)parts * k_rows * kv_heads * head_dim * 2 * sizeof(float) : 0);
+}
+
 int some_op_causal_attention(SomeHandle* h, int32_t dtype, int32_t head_dim, const void* q_dev, int64_t q_row, int64_t q_head, int32_t heads,
                              const void* k_dev, int64_t k_row, int64_t k_head, const void* v_dev, int64_t v_row, int64_t v_head, int32_t kv_heads,
                              const int32_t* q_offsets_dev, const int32_t* k_offsets_dev, int32_t B, int64_t q_rows, int64_t k_rows, int32_t causal,
-                             float scale, void* out_dev, int64_t o_row, int64_t o_head, float* lse_dev, void* stream) {
+                             float scale, void* out_dev, int64_t o_row, int64_t o_head, float* lse_dev, void* workspace_dev, size_t workspace_bytes,
+                             void* stream) {
     if (!h) return SOME_EINVAL;
     C_CHECK(type_ok(dtype, head_dim), kType);
     C_CHECK(heads_ok(heads, kv_heads), kHeadsMsg);
@@ -125,6 +142,14 @@ int some_op_causal_attention(SomeHandle* h, int32_t dtype, int32_t head_dim, con
     C_CHECK(laid_out(dtype, a.q) && laid_out(dtype, a.k) && laid_out(dtype, a.v) && laid_out(dtype, a.out), kLayout);
     a.lse = lse_dev; a.q_offsets = q_offsets_dev; a.k_offsets = k_offsets_dev; a.q_rows = q_rows;
     a.B = B; a.kv_heads = kv_heads; a.group = heads / kv_heads; a.causal = causal; a.scale = scale;
+    a.parts = k_rows > 0 ? causal_fwd_parts(q_rows, k_rows, B, heads) : 1;
+    if (a.parts > 1) {
+        if (!workspace_dev || workspace_bytes < some_op_causal_attention_bytes(h, heads, kv_heads, head_dim, B, q_rows, k_rows))
+            return cfail(h, SOME_ENOMEM, __func__, "workspace too small (some_op_causal_attention_bytes)");
+        C_CHECK((reinterpret_cast<uintptr_t>(workspace_dev) & 15) == 0, "workspace must be 16-byte aligned");
+        a.part_o = static_cast<float*>(workspace_dev);
+        a.part_ml = a.part_o + (int64_t)a.parts * q_rows * heads * head_dim;
+    }
     C_CHECK(causal_fwd_blocks(a) < 0x7fffffffll, "too many rows, clips and heads for one launch");
     C_TRY(launch_causal_fwd(dtype, head_dim, a, static_cast<hipStream_t>(stream)));
     return SOME_OK;
@@ -135,15 +160,15 @@ int some_train_causal_attention_bwd(SomeHandle* h, int32_t dtype, int32_t head_d
                                     const int32_t* q_offsets_dev, const int32_t* k_offsets_dev, int32_t B, int64_t q_rows, int64_t k_rows, int32_t causal,
                                     float scale, const void* out_dev, int64_t o_row, int64_t o_head, const float* lse_dev, const void* dout_dev,
                                     int64_t do_row, int64_t do_head, void* dq_dev, int64_t dq_row, int64_t dq_head, void* dk_dev, int64_t dk_row,
-                                    int64_t dk_head, void* dv_dev, int64_t dv_row, int64_t dv_head, float* dsum_dev, void* stream) {
+                                    int64_t dk_head, void* dv_dev, int64_t dv_row, int64_t dv_head, void* workspace_dev, size_t workspace_bytes, void* stream) {
     if (!h) return SOME_EINVAL;
     C_CHECK(type_ok(dtype, head_dim), kType);
     C_CHECK(heads_ok(heads, kv_heads), kHeadsMsg);
     C_CHECK(B >= 0 && q_rows >= 0 && k_rows >= 0 && q_rows < kMaxRows && k_rows < kMaxRows && B < kMaxRows, "clips and rows must be below 2^29");
     C_CHECK(scale > 0.f && std::isfinite(scale), "scale must be finite and positive");
     if (B == 0 || (q_rows == 0 && k_rows == 0)) return SOME_OK;
-    C_CHECK(q_offsets_dev && k_offsets_dev, "null pointer");
-    C_CHECK(q_rows == 0 || (q_dev && out_dev && lse_dev && dout_dev && dq_dev && dsum_dev), "null pointer");
+    C_CHECK(q_offsets_dev && k_offsets_dev && workspace_dev, "null pointer");
+    C_CHECK(q_rows == 0 || (q_dev && out_dev && lse_dev && dout_dev && dq_dev), "null pointer");
     C_CHECK(k_rows == 0 || (k_dev && v_dev && dk_dev && dv_dev), "null pointer");
     CausalBwdArgs b{};
     CausalArgs& a = b.f;
@@ -153,8 +178,16 @@ int some_train_causal_attention_bwd(SomeHandle* h, int32_t dtype, int32_t head_d
             laid_out(dtype, b.dk) && laid_out(dtype, b.dv), kLayout);
     a.lse = const_cast<float*>(lse_dev); a.q_offsets = q_offsets_dev; a.k_offsets = k_offsets_dev; a.q_rows = q_rows;
     a.B = B; a.kv_heads = kv_heads; a.group = heads / kv_heads; a.causal = causal; a.scale = scale;
-    b.dsum = dsum_dev; b.k_rows = k_rows;
-    C_CHECK(causal_fwd_blocks(a) < 0x7fffffffll && (k_rows / 64 + B) * (int64_t)heads * 8 < 0x7fffffffll, "too many rows, clips and heads for one launch");
+    a.parts = 1;
+    b.k_rows = k_rows;
+    b.parts = causal_bwd_parts(q_rows, k_rows, B, heads, kv_heads);
+    if (workspace_bytes < some_train_causal_attention_bytes(h, heads, kv_heads, head_dim, B, q_rows, k_rows))
+        return cfail(h, SOME_ENOMEM, __func__, "workspace too small (some_train_causal_attention_bytes)");
+    C_CHECK((reinterpret_cast<uintptr_t>(workspace_dev) & 15) == 0, "workspace must be 16-byte aligned");
+    b.dsum = static_cast<float*>(workspace_dev);
+    b.part_k = reinterpret_cast<float*>(static_cast<char*>(workspace_dev) + dsum_bytes(heads, q_rows));
+    b.part_v = b.part_k + (int64_t)b.parts * k_rows * kv_heads * head_dim;
+    C_CHECK(causal_fwd_blocks(a) < 0x7fffffffll && causal_bwd_blocks(b) < 0x7fffffffll && k_rows * kv_heads * (head_dim / 4) / 256 < 0x7ffffff0ll, "too many rows, clips and heads for one launch");
     C_TRY(launch_causal_bwd(dtype, head_dim, b, static_cast<hipStream_t>(stream)));
     return SOME_OK;
 }

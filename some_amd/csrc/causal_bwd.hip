@@ -16,7 +16,7 @@ template <int DB> __device__ __forceinline__ void fit_column(const f32x16& ds, f
     float mx = 0.f;
 #pragma unroll
     for (int r = 0; r < 16; ++r) mx = fmaxf(mx, __builtin_fabsf(ds[r]));
-    mx = fmaxf(mx, other_half(mx));
+    mx = halves_max(mx);
     if (__any(mx * F > 16384.f)) {
         if (mx * F > 16384.f) {
             const float f = __builtin_ldexpf(1.f, min(100, max(-126, 5 - __builtin_amdgcn_frexp_expf(mx))));
@@ -33,14 +33,6 @@ constexpr float kFitStart = 0x1p100f;
 // f16 only: probabilities of long clips (about 1 / T) would be subnormal; they enter the products as 2^10 P
 template <typename T> constexpr float kProbLog2 = __is_same(T, f16_t) ? 10.f : 0.f;
 
-template <typename T> __device__ __forceinline__ void store4(T* p, float a, float b, float c, float d) {
-    if constexpr (sizeof(T) == 4) {
-        *reinterpret_cast<f32x4*>(p) = (f32x4){a, b, c, d};
-    } else {
-        *reinterpret_cast<s16x4*>(p) = (s16x4){__builtin_bit_cast(short, (T)a), __builtin_bit_cast(short, (T)b), __builtin_bit_cast(short, (T)c), __builtin_bit_cast(short, (T)d)};
-    }
-}
-
 // ---- dQ (and D) ----------------------------------------------------------------------------------------------------------------------------
 constexpr int QB = 128;
 template <typename T, int D> struct DqShape {
@@ -50,7 +42,7 @@ template <typename T, int D> struct DqShape {
 };
 
 template <typename T, int D>
-__global__ __launch_bounds__(256, (D == 128 ? 1 : 2)) void causal_dq_kernel(CausalBwdArgs b, int nsub, int slots) {
+__global__ __launch_bounds__(256, (D == 128 && sizeof(T) == 4 ? 1 : 2)) void causal_dq_kernel(CausalBwdArgs b, int nsub, int slots) {
     constexpr int KT = DqShape<T, D>::KT, NB = KT / 32, KS = D / 16, DB = D / 32, TILE_B = DqShape<T, D>::TILE_B;
     constexpr bool F16 = __is_same(T, f16_t);
     typedef Tile<T, D> TL;
@@ -88,7 +80,7 @@ __global__ __launch_bounds__(256, (D == 128 ? 1 : 2)) void causal_dq_kernel(Caus
             else dsum = fmaf((float)__builtin_bit_cast(T, (short)gfr[ks][j]), (float)__builtin_bit_cast(T, (short)of[j]), dsum);
         }
     }
-    dsum += other_half(dsum);
+    dsum = halves_sum(dsum);
     const float lse = a.lse[(int64_t)head * a.q_rows + qr];
     if (q < Tq && hi == 0) b.dsum[(int64_t)head * a.q_rows + qf + q] = dsum;
 
@@ -117,6 +109,7 @@ __global__ __launch_bounds__(256, (D == 128 ? 1 : 2)) void causal_dq_kernel(Caus
     for (int d = 0; d < DB; ++d) acc[d] = zero16();
     float F = F16 ? kFitStart : 1.f;
     const float c2 = a.scale * 1.4426950408889634f;
+    bool bad = false;
 
     if (ntiles > 0) fetch(0);
     for (int t = 0; t < ntiles; ++t) {
@@ -147,10 +140,7 @@ __global__ __launch_bounds__(256, (D == 128 ? 1 : 2)) void causal_dq_kernel(Caus
 #pragma unroll
                 for (int r = 0; r < 16; ++r) s[r] *= F;
             }
-            if (edge && block_not_finite<T, D>(kt, nb * 32)) {
-                add_by_hand<T, D>(acc, s, kt, nb * 32, [&](int j) { return key0 + j <= limit; });
-                continue;
-            }
+            if (edge) bad |= block_not_finite<T, D>(kt, nb * 32);
 #pragma unroll
             for (int s2 = 0; s2 < 2; ++s2) {
                 const frag p = pack8<T>(s, s2);
@@ -160,6 +150,24 @@ __global__ __launch_bounds__(256, (D == 128 ? 1 : 2)) void causal_dq_kernel(Caus
         }
     }
 
+    if (bad) {                                               // (wave-uniform; causal_core.h, "not-a-number and infinities")
+        const T* kp = reinterpret_cast<const T*>(kbase);
+        const T* vp = reinterpret_cast<const T*>(vbase);
+        for (int n = 0; n < 32 && qw + n < Tq; ++n) {
+            const int64_t row = qf + qw + n;
+            const T* qp = static_cast<const T*>(a.q.p) + row * a.q.row + (int64_t)head * a.q.head;
+            const T* gp = static_cast<const T*>(b.dout.p) + row * b.dout.row + (int64_t)head * b.dout.head;
+            const float lse_n = __shfl(lse, n, 64), dsum_n = __shfl(dsum, n, 64);
+            float x[(D + 63) / 64] = {};
+            solo_column<T, D>(x, 0, min(qw + n + shift, Tk - 1) + 1, kp, a.k.row, [&](int j) {
+                return exp2_(fmaf(dot_rows<T, D>(qp, kp + (int64_t)j * a.k.row), c2, -lse_n)) * (dot_rows<T, D>(gp, vp + (int64_t)j * a.v.row) - dsum_n);
+            });
+            T* dst = static_cast<T*>(b.dq.p) + row * b.dq.row + (int64_t)head * b.dq.head;
+#pragma unroll
+            for (int e = 0; e < (D + 63) / 64; ++e) dst[lane + 64 * e] = (T)(x[e] * a.scale);
+        }
+        return;
+    }
     if (q < Tq) {
         const float f = a.scale / F;
         T* dst = static_cast<T*>(b.dq.p) + (int64_t)(qf + q) * b.dq.row + (int64_t)head * b.dq.head + 4 * hi;
@@ -180,7 +188,7 @@ template <typename T, int D> struct DkvShape {
 };
 
 template <typename T, int D>
-__global__ __launch_bounds__(256, (D == 128 || sizeof(T) == 4 ? 1 : 2)) void causal_dkv_kernel(CausalBwdArgs b, int nsub, int slots) {
+__global__ __launch_bounds__(256, (D == 128 ? 1 : 2)) void causal_dkv_kernel(CausalBwdArgs b, int nsub, int slots) {
     constexpr int QT = DkvShape<T, D>::QT, NB = QT / 32, KS = D / 16, DB = D / 32, TILE_B = DkvShape<T, D>::TILE_B, STAGE_B = DkvShape<T, D>::STAGE_B;
     constexpr bool F16 = __is_same(T, f16_t);
     typedef Tile<T, D> TL;
@@ -188,7 +196,7 @@ __global__ __launch_bounds__(256, (D == 128 || sizeof(T) == 4 ? 1 : 2)) void cau
     extern __shared__ __attribute__((aligned(16))) char lds[];
     const CausalArgs& a = b.f;
 
-    const Work w = find_work(a.kv_heads, nsub, 1, slots);
+    const Work w = find_work(a.kv_heads, nsub, b.parts, slots);
     if (w.slot < 0) return;
     const Place pl = find_clip<KB>(a.k_offsets, a.B, slots - 1 - w.slot);        // the first keys of a clip are seen by most queries: first slots first
     const int qf = a.q_offsets[pl.b], Tq = a.q_offsets[pl.b + 1] - qf;
@@ -212,7 +220,8 @@ __global__ __launch_bounds__(256, (D == 128 || sizeof(T) == 4 ? 1 : 2)) void cau
 
     // the first query that sees key k0 is k0 - shift
     const int t0 = max(0, k0 - shift) / QT, nt = max(0, (Tq + QT - 1) / QT - t0);
-    const int total = nt * a.group;
+    const int total = nt * a.group;                          // (head, tile) pairs; this part's share of them:
+    const int it0 = (int)((int64_t)total * w.g / b.parts), it1 = (int)((int64_t)total * (w.g + 1) / b.parts);
     const int64_t qbytes = a.q.row * (int64_t)sizeof(T), gbytes = b.dout.row * (int64_t)sizeof(T);
     const char* qbase = reinterpret_cast<const char*>(static_cast<const T*>(a.q.p) + (int64_t)qf * a.q.row + (int64_t)w.kvh * a.group * a.q.head);
     const char* gbase = reinterpret_cast<const char*>(static_cast<const T*>(b.dout.p) + (int64_t)qf * b.dout.row + (int64_t)w.kvh * a.group * b.dout.head);
@@ -239,15 +248,16 @@ __global__ __launch_bounds__(256, (D == 128 || sizeof(T) == 4 ? 1 : 2)) void cau
     }
     float F = F16 ? kFitStart : 1.f;
     const float c2 = a.scale * 1.4426950408889634f;
+    bool bad = false;
 
-    if (total > 0) fetch(0, 0, t0);
-    int g = 0, t = t0;
-    for (int it = 0; it < total; ++it) {
+    int g = nt > 0 ? it0 / nt : 0, t = nt > 0 ? t0 + it0 % nt : 0;
+    if (it0 < it1) fetch(it0, g, t);
+    for (int it = it0; it < it1; ++it) {
         int gn = g, tn = t + 1;
         if (tn == t0 + nt) { tn = t0; ++gn; }
         wait_vm<0>();
         __syncthreads();
-        if (it + 1 < total) fetch(it + 1, gn, tn);
+        if (it + 1 < it1) fetch(it + 1, gn, tn);
         const char* qt = lds + (it & 1) * STAGE_B;
         const char* gt = qt + TILE_B;
         const float* lt = reinterpret_cast<const float*>(qt + 2 * TILE_B);
@@ -286,12 +296,7 @@ __global__ __launch_bounds__(256, (D == 128 || sizeof(T) == 4 ? 1 : 2)) void cau
 #pragma unroll
                 for (int r = 0; r < 16; ++r) dp[r] *= F;
             }
-            if (edge && (block_not_finite<T, D>(qt, nb * 32) || block_not_finite<T, D>(gt, nb * 32))) {
-                const auto see = [&](int j) { return qb0 + j < Tq && key <= qb0 + j + shift; };
-                add_by_hand<T, D>(dv, s, gt, nb * 32, see);
-                add_by_hand<T, D>(dk, dp, qt, nb * 32, see);
-                continue;
-            }
+            if (edge) bad |= block_not_finite<T, D>(qt, nb * 32) || block_not_finite<T, D>(gt, nb * 32);
 #pragma unroll
             for (int s2 = 0; s2 < 2; ++s2) {
                 const frag pf = pack8<T>(s, s2), df = pack8<T>(dp, s2);
@@ -306,19 +311,78 @@ __global__ __launch_bounds__(256, (D == 128 || sizeof(T) == 4 ? 1 : 2)) void cau
         t = tn;
     }
 
+    const int64_t prow = (int64_t)w.g * b.k_rows;
+    if (bad) {                                               // (wave-uniform; causal_core.h, "not-a-number and infinities")
+        for (int n = 0; n < 32 && kw + n < Tk; ++n) {
+            const int kn = kw + n;
+            const int64_t row = kf + kn;
+            const T* kp = static_cast<const T*>(a.k.p) + row * a.k.row + (int64_t)w.kvh * a.k.head;
+            const T* vp = static_cast<const T*>(a.v.p) + row * a.v.row + (int64_t)w.kvh * a.v.head;
+            float xk[(D + 63) / 64] = {}, xv[(D + 63) / 64] = {};
+            for (int gg = it0 / nt; gg <= (it1 - 1) / nt; ++gg) {
+                const int r0 = max(max(max(it0, gg * nt) - gg * nt + t0, 0) * QT, kn - shift), r1 = min((min(it1, (gg + 1) * nt) - gg * nt + t0) * QT, Tq);
+                const T* qp = reinterpret_cast<const T*>(qbase) + (int64_t)gg * a.q.head;
+                const T* gp = reinterpret_cast<const T*>(gbase) + (int64_t)gg * b.dout.head;
+                const float* lp = lbase + (int64_t)gg * a.q_rows;
+                const float* dp = dbase + (int64_t)gg * a.q_rows;
+                const auto prob = [&](int i) { return exp2_(fmaf(dot_rows<T, D>(qp + (int64_t)i * a.q.row, kp), c2, -lp[i])); };
+                solo_column<T, D>(xv, r0, r1, gp, b.dout.row, prob);
+                solo_column<T, D>(xk, r0, r1, qp, a.q.row, [&](int i) { return prob(i) * (dot_rows<T, D>(gp + (int64_t)i * b.dout.row, vp) - dp[i]); });
+            }
+#pragma unroll
+            for (int e = 0; e < (D + 63) / 64; ++e) {
+                const int d = lane + 64 * e;
+                if (b.parts > 1) {
+                    const int64_t i = ((prow + row) * a.kv_heads + w.kvh) * D + d;
+                    b.part_k[i] = xk[e] * a.scale;
+                    b.part_v[i] = xv[e];
+                } else {
+                    static_cast<T*>(b.dk.p)[row * b.dk.row + (int64_t)w.kvh * b.dk.head + d] = (T)(xk[e] * a.scale);
+                    static_cast<T*>(b.dv.p)[row * b.dv.row + (int64_t)w.kvh * b.dv.head + d] = (T)xv[e];
+                }
+            }
+        }
+        return;
+    }
     if (key < Tk) {
         const float pf = F16 ? 0x1p-10f : 1.f;
         const float fk = a.scale / F * pf;
+        const int64_t i = ((prow + kf + key) * a.kv_heads + w.kvh) * D + 4 * hi;
         T* dkd = static_cast<T*>(b.dk.p) + (int64_t)(kf + key) * b.dk.row + (int64_t)w.kvh * b.dk.head + 4 * hi;
         T* dvd = static_cast<T*>(b.dv.p) + (int64_t)(kf + key) * b.dv.row + (int64_t)w.kvh * b.dv.head + 4 * hi;
 #pragma unroll
         for (int d = 0; d < DB; ++d)
 #pragma unroll
             for (int r4 = 0; r4 < 4; ++r4) {
-                store4<T>(dkd + 32 * d + 8 * r4, dk[d][4 * r4] * fk, dk[d][4 * r4 + 1] * fk, dk[d][4 * r4 + 2] * fk, dk[d][4 * r4 + 3] * fk);
-                store4<T>(dvd + 32 * d + 8 * r4, dv[d][4 * r4] * pf, dv[d][4 * r4 + 1] * pf, dv[d][4 * r4 + 2] * pf, dv[d][4 * r4 + 3] * pf);
+                const f32x4 x = {dk[d][4 * r4] * fk, dk[d][4 * r4 + 1] * fk, dk[d][4 * r4 + 2] * fk, dk[d][4 * r4 + 3] * fk};
+                const f32x4 y = {dv[d][4 * r4] * pf, dv[d][4 * r4 + 1] * pf, dv[d][4 * r4 + 2] * pf, dv[d][4 * r4 + 3] * pf};
+                if (b.parts > 1) {
+                    *reinterpret_cast<f32x4*>(b.part_k + i + 32 * d + 8 * r4) = x;
+                    *reinterpret_cast<f32x4*>(b.part_v + i + 32 * d + 8 * r4) = y;
+                } else {
+                    store4<T>(dkd + 32 * d + 8 * r4, x[0], x[1], x[2], x[3]);
+                    store4<T>(dvd + 32 * d + 8 * r4, y[0], y[1], y[2], y[3]);
+                }
             }
     }
+}
+
+// dK and dV: the parts summed in order, four channels a thread (blockIdx.y: 0 dK, 1 dV)
+template <typename T, int D> __global__ __launch_bounds__(256) void causal_sum_kernel(CausalBwdArgs b) {
+    const int G = b.f.kv_heads;
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, plane = b.k_rows * G * D;
+    const int64_t row = i / (G * (D / 4));
+    if (row < b.f.k_offsets[0] || row >= b.f.k_offsets[b.f.B]) return;
+    const int h = (int)(i % (G * (D / 4))) / (D / 4), d = (int)(i % (D / 4)) * 4;
+    const float* src = (blockIdx.y ? b.part_v : b.part_k) + i * 4;
+    f32x4 x = *reinterpret_cast<const f32x4*>(src);
+    for (int p = 1; p < b.parts; ++p) {
+        const f32x4 y = *reinterpret_cast<const f32x4*>(src + p * plane);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) x[k] += y[k];
+    }
+    const Rows3& out = blockIdx.y ? b.dv : b.dk;
+    store4<T>(static_cast<T*>(out.p) + row * out.row + (int64_t)h * out.head + d, x[0], x[1], x[2], x[3]);
 }
 
 template <typename T, int D> hipError_t run(const CausalBwdArgs& b, hipStream_t s) {
@@ -338,12 +402,26 @@ template <typename T, int D> hipError_t run(const CausalBwdArgs& b, hipStream_t 
     }
     if (b.k_rows > 0) {
         const int slots = (int)(b.k_rows / KB) + a.B;
-        hipLaunchKernelGGL((causal_dkv_kernel<T, D>), dim3((unsigned)work_blocks(a.kv_heads, 1, slots)), dim3(256), (DkvShape<T, D>::LDS_B), s, b, nsub, slots);
+        hipLaunchKernelGGL((causal_dkv_kernel<T, D>), dim3((unsigned)work_blocks(a.kv_heads, b.parts, slots)), dim3(256), (DkvShape<T, D>::LDS_B), s, b, nsub,
+                           slots);
+        if (b.parts > 1)
+            hipLaunchKernelGGL((causal_sum_kernel<T, D>), dim3((unsigned)((b.k_rows * a.kv_heads * (D / 4) + 255) / 256), 2), dim3(256), 0, s, b);
     }
     return hipGetLastError();
 }
 
 }  // namespace
+
+// Parts the queries (and heads of a group) that a key tile meets are cut into: as many as bring the launch to 6 workgroups per CU, at least 4 tiles of 64
+// queries each.  Lengths are on the device, so the averages over the batch decide.
+int causal_bwd_parts(int64_t q_rows, int64_t k_rows, int B, int heads, int kv_heads) {
+    if (B <= 0 || q_rows <= 0 || k_rows <= 0) return 1;
+    const int64_t tiles = (k_rows + KB - 1) / KB > B ? (k_rows + KB - 1) / KB : B;
+    const int64_t want = (1536 + tiles * kv_heads - 1) / (tiles * kv_heads), room = (q_rows / B + 63) / 64 * (heads / kv_heads) / 4;
+    const int64_t p = want < room ? want : room;
+    return p < 1 ? 1 : p > 16 ? 16 : (int)p;
+}
+int64_t causal_bwd_blocks(const CausalBwdArgs& b) { return causal::work_blocks(b.f.kv_heads, b.parts, (int)(b.k_rows / KB) + b.f.B); }
 
 hipError_t launch_causal_bwd(int dtype, int head_dim, const CausalBwdArgs& b, hipStream_t s) {
     if (b.f.B <= 0) return hipSuccess;

@@ -57,7 +57,13 @@ __device__ __forceinline__ void dma4(const char* src, char* lds_dst) {
 template <int N> __device__ __forceinline__ void wait_vm() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
 __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
 __device__ __forceinline__ float log2_(float x) { return __builtin_amdgcn_logf(x); }
-__device__ __forceinline__ float other_half(float x) { return __shfl_xor(x, 32, 64); }
+// a value and its counterpart in the other half of the wave (the same pair in both halves, so both compute the same bits)
+__device__ __forceinline__ f32x2 both_halves(float x) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, x), __builtin_bit_cast(uint32_t, x), false, false);
+    return (f32x2){__builtin_bit_cast(float, (uint32_t)r[0]), __builtin_bit_cast(float, (uint32_t)r[1])};
+}
+__device__ __forceinline__ float halves_max(float x) { const f32x2 b = both_halves(x); return fmaxf(b[0], b[1]); }
+__device__ __forceinline__ float halves_sum(float x) { const f32x2 b = both_halves(x); return b[0] + b[1]; }
 __device__ __forceinline__ f32x16 zero16() {
     f32x16 z;
 #pragma unroll
@@ -93,6 +99,15 @@ template <typename T> __device__ __forceinline__ typename Frag<T>::type zero8() 
 #pragma unroll
     for (int j = 0; j < 8; ++j) f[j] = 0;
     return f;
+}
+
+// four neighbouring values of a row, rounded to the type once
+template <typename T> __device__ __forceinline__ void store4(T* p, float a, float b, float c, float d) {
+    if constexpr (sizeof(T) == 4) {
+        *reinterpret_cast<f32x4*>(p) = (f32x4){a, b, c, d};
+    } else {
+        *reinterpret_cast<s16x4*>(p) = (s16x4){__builtin_bit_cast(short, (T)a), __builtin_bit_cast(short, (T)b), __builtin_bit_cast(short, (T)c), __builtin_bit_cast(short, (T)d)};
+    }
 }
 
 // ---- LDS tiles: ROWS rows of D values, row pitch D sizeof(T) bytes, 16-byte chunk c of row r stored at chunk c ^ swz(r) --------------------
@@ -172,9 +187,11 @@ template <typename T, int D, int ROWS, int NT> struct Copier {
 };
 
 // ---- not-a-number and infinities in masked places ----------------------------------------------------------------------------------------------
-// A masked weight is 0, and 0 * inf would reach the sum.  Only a 32 x 32 block on the diagonal (or at a clip's end) mixes masked and visible places;
-// if the 32 tile rows it contracts over hold such a value, the block's product is summed by hand over the visible ones.
-template <typename T, int D> __device__ __noinline__ bool block_not_finite(const char* tile, int r0) {
+// A masked weight is 0, and 0 * inf would reach the sum.  Only a 32 x 32 block on the diagonal (or at a clip's end) mixes masked and visible places.
+// If the 32 tile rows such a block contracts over hold a value that is not finite, the wave remembers it and, when its loop is done, computes its
+// 32 columns anew one by one over the visible rows alone (solo_column).  The check is a few LDS reads per such block; the redo is slow and rare, and
+// stands behind the loop where its registers cost nothing.
+template <typename T, int D> __device__ __forceinline__ bool block_not_finite(const char* tile, int r0) {
     typedef Tile<T, D> TL;
     const int lane = threadIdx.x & 63;
     bool bad = false;
@@ -192,28 +209,22 @@ template <typename T, int D> __device__ __noinline__ bool block_not_finite(const
     }
     return __any(bad);
 }
-// acc[column l31] += sum over the tile rows r0 + j the column sees of w[j] * row, w in the registers of a product (row crow(r, hi) <-> j)
-template <typename T, int D, typename See>
-__device__ __forceinline__ void add_by_hand(f32x16 (&acc)[D / 32], const f32x16& w, const char* tile, int r0, See see) {
-    typedef Tile<T, D> TL;
-    constexpr int PER = 16 / (int)sizeof(T);
-    const int lane = threadIdx.x & 63, l31 = lane & 31, hi = lane >> 5;
-    for (int j = 0; j < 32; ++j) {
-        const int r = (j & 3) + 4 * (j >> 3), h = (j >> 2) & 1;          // crow(r, h) == j
-        float p = 0.f;
+template <typename T, int D> __device__ __forceinline__ float dot_rows(const T* x, const T* y) {
+    float s = 0.f;
+    for (int d = 0; d < D; ++d) s = fmaf(to_f32(x[d]), to_f32(y[d]), s);
+    return s;
+}
+// acc[e] (+)= sum over rows r in [r0, r1) of weight(r) * m[r][lane + 64 e]; the wave's lanes compute 64 weights side by side, then share them
+template <typename T, int D, typename Weight>
+__device__ __forceinline__ void solo_column(float (&acc)[(D + 63) / 64], int r0, int r1, const T* m, int64_t stride, Weight weight) {
+    const int lane = threadIdx.x & 63;
+    for (int base = r0; base < r1; base += 64) {
+        const float w = base + lane < r1 ? weight(base + lane) : 0.f;
+        for (int j = 0; j < min(64, r1 - base); ++j) {
+            const float wj = __shfl(w, j, 64);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) p = i == r ? w[i] : p;
-        p = __shfl(p, l31 + 32 * h, 64);
-        const bool visible = see(j);
-        const int row = r0 + j;
-#pragma unroll
-        for (int d = 0; d < D / 32; ++d)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const int col = 32 * d + crow(i, hi);
-                const float v = to_f32(*reinterpret_cast<const T*>(tile + row * TL::PITCH + (((col / PER) ^ TL::swz(row)) << 4) + (col % PER) * (int)sizeof(T)));
-                if (visible) acc[d][i] = fmaf(p, v, acc[d][i]);
-            }
+            for (int e = 0; e < (D + 63) / 64; ++e) acc[e] = fmaf(wj, to_f32(m[(int64_t)(base + j) * stride + lane + 64 * e]), acc[e]);
+        }
     }
 }
 
@@ -233,6 +244,19 @@ template <int TR> __device__ __forceinline__ Place find_clip(const int32_t* __re
     }
     const int b = n > 0 ? n - 1 : 0;
     return {__builtin_amdgcn_readfirstlane(b), __builtin_amdgcn_readfirstlane(slot - (off[b] / TR + b))};
+}
+// the clip of a packed row (off[0] <= row < off[B])
+__device__ __forceinline__ Place find_row(const int32_t* __restrict__ off, int B, int row) {
+    const int lane = threadIdx.x & 63;
+    int n = 0;
+    for (int base = 0; base < B; base += 64) {
+        const int b = base + lane;
+        const int c = __popcll(__ballot(b < B && off[b] <= row));
+        n += c;
+        if (c < 64) break;
+    }
+    const int b = __builtin_amdgcn_readfirstlane(n - 1);
+    return {b, row - off[b]};
 }
 // blockIdx -> (kv head, slot, head of the group): the blocks of one kv head run on as few of the 8 XCDs as balance allows (they read the same K
 // and V through that XCD's L2), neighbouring slots at the same time, the last slot of the packed rows first (a clip's last tile sees most keys).

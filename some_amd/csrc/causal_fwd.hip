@@ -1,8 +1,8 @@
 // Causal attention over packed clips, forward: out[i] = sum_j softmax_j(scale q_i . k_j) v_j over the keys j <= i + Tk - Tq of the clip (rows aligned at
 // the end: the queries are the clip's last Tq frames), heads in groups that share keys and values.  A row that sees no key is 0 (log-sum -inf).
 //
-// One pass over the keys with a running maximum and sum (base 2, the scale folded into the exponent's multiplier).  A workgroup is 128 queries of one
-// head, a wave 32 of them; S^T = K Q^T puts a query in every lane's column, so its maximum and sum are the lane's own registers plus one exchange
+// One pass over the keys with a running maximum and sum (base 2, the scale folded into the exponent's multiplier).  A workgroup is 128 QN queries of one
+// head, a wave 32 QN of them; S^T = K Q^T puts a query in every lane's column, so its maximum and sum are the lane's own registers plus one exchange
 // with the other half, and P^T is already the B operand of O^T += V^T P^T (causal_core.h): no probability touches LDS.  K and V tiles go global ->
 // LDS by DMA into a ring; V is read transposed by ds_read_b64_tr_b16.
 #include "causal_core.h"
@@ -10,24 +10,51 @@
 namespace {
 using namespace causal;
 
-constexpr int QB = 128;                          // queries per workgroup
+// The running maximum only has to keep the exponentials in range, so it follows the true one lazily: it moves when a score passes it by 2^8.  P then
+// reaches 256, far inside every operand type, and the accumulators are rescaled once or twice per row instead of at every new maximum.
+constexpr float kSlack = 8.f;
 
-template <typename T, int D> struct Shape {
+template <typename T, int D, int QN> struct Shape {
     static constexpr int KT = (sizeof(T) == 4 && D == 128) ? 32 : 64;      // keys per tile
     static constexpr int TILE_B = KT * D * (int)sizeof(T);
     static constexpr int STAGES = 2;
     static constexpr int LDS_B = STAGES * 2 * TILE_B;
+    static constexpr int QB = 128 * QN;                                    // queries per workgroup
 };
 
+// one query, all its visible keys in [j0, j1) (causal_core.h, "not-a-number and infinities"): unnormalised sums, maximum and sum
 template <typename T, int D>
+__device__ __forceinline__ void solo_query(const CausalArgs& a, const T* q, const T* k, const T* v, int j0, int j1, float c2, float* m, float* l,
+                                        float* o0, float* o1) {
+    const int lane = threadIdx.x & 63;
+    float mx = -INFINITY;
+    for (int j = j0 + lane; j < j1; j += 64) mx = fmaxf(mx, dot_rows<T, D>(q, k + (int64_t)j * a.k.row));
+#pragma unroll
+    for (int x = 1; x < 64; x *= 2) mx = fmaxf(mx, __shfl_xor(mx, x, 64));
+    const float mc = mx == -INFINITY ? 0.f : mx * c2;
+    float sum = 0.f, acc[(D + 63) / 64] = {};
+    solo_column<T, D>(acc, j0, j1, v, a.v.row, [&](int j) {
+        const float p = exp2_(fmaf(dot_rows<T, D>(q, k + (int64_t)j * a.k.row), c2, -mc));
+        sum += p;
+        return p;
+    });
+#pragma unroll
+    for (int x = 1; x < 64; x *= 2) sum += __shfl_xor(sum, x, 64);
+    *m = mx;
+    *l = sum;
+    *o0 = acc[0];
+    *o1 = D > 64 ? acc[(D + 63) / 64 - 1] : 0.f;
+}
+
+template <typename T, int D, int QN>
 __global__ __launch_bounds__(256, 2) void causal_fwd_kernel(CausalArgs a, int nsub, int slots) {
-    constexpr int KT = Shape<T, D>::KT, NB = KT / 32, KS = D / 16, DB = D / 32;
-    constexpr int TILE_B = Shape<T, D>::TILE_B, STAGES = Shape<T, D>::STAGES;
+    typedef Shape<T, D, QN> SH;
+    constexpr int KT = SH::KT, NB = KT / 32, KS = D / 16, DB = D / 32, TILE_B = SH::TILE_B, STAGES = SH::STAGES, QB = SH::QB;
     typedef Tile<T, D> TL;
     typedef typename Frag<T>::type frag;
     extern __shared__ __attribute__((aligned(16))) char lds[];
 
-    const Work w = find_work(a.kv_heads, nsub, a.group, slots);
+    const Work w = find_work(a.kv_heads, nsub, a.group * a.parts, slots);
     if (w.slot < 0) return;
     const Place pl = find_clip<QB>(a.q_offsets, a.B, w.slot);
     const int qf = a.q_offsets[pl.b], Tq = a.q_offsets[pl.b + 1] - qf;
@@ -35,21 +62,24 @@ __global__ __launch_bounds__(256, 2) void causal_fwd_kernel(CausalArgs a, int ns
     const int q0 = pl.tile * QB;
     if (q0 >= Tq) return;
     const int shift = a.causal ? Tk - Tq : 0x3fffffff;       // query i sees keys j <= i + shift
+    const int head = w.kvh * a.group + w.g % a.group, part = w.g / a.group;
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int l31 = lane & 31, hi = lane >> 5;
-    const int head = w.kvh * a.group + w.g;
-    const int qw = q0 + wave * 32, q = qw + l31;
-    const T* qrow = static_cast<const T*>(a.q.p) + (int64_t)(qf + min(q, Tq - 1)) * a.q.row + (int64_t)head * a.q.head + 8 * hi;
-    frag qfr[KS];
+    const int qw = q0 + wave * 32 * QN;                      // the wave's first query; block n holds qw + 32 n ..
+    const T* qhead = static_cast<const T*>(a.q.p) + (int64_t)head * a.q.head;
+    frag qfr[QN][KS];
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks) qfr[ks] = load8<T>(qrow + 16 * ks);
+    for (int n = 0; n < QN; ++n)
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) qfr[n][ks] = load8<T>(qhead + (int64_t)(qf + min(qw + 32 * n + l31, Tq - 1)) * a.q.row + 8 * hi + 16 * ks);
 
     const int last_q = min(q0 + QB, Tq) - 1;
     const int nkeys = min(Tk, max(0, last_q + shift + 1));   // keys anybody here sees
     const int ntiles = (nkeys + KT - 1) / KT;
-    const int seen_w = min(Tk, max(0, min(qw + 31, Tq - 1) + shift + 1));        // ... this wave sees (0 or less: none)
-    const int limit = min(q + shift, Tk - 1);                // last key this lane's query sees
+    // this part's tiles
+    const int t_begin = (int)((int64_t)ntiles * part / a.parts), t_end = (int)((int64_t)ntiles * (part + 1) / a.parts);
+    const int seen_w = min(Tk, max(0, min(qw + 32 * QN - 1, Tq - 1) + shift + 1));        // keys this wave sees
     const int full_w = min(Tk, max(0, qw + shift + 1));      // keys every query of the wave sees
 
     const char* kbase = reinterpret_cast<const char*>(static_cast<const T*>(a.k.p) + (int64_t)kf * a.k.row + (int64_t)w.kvh * a.k.head);
@@ -65,104 +95,207 @@ __global__ __launch_bounds__(256, 2) void causal_fwd_kernel(CausalArgs a, int ns
         cv.run(st + TILE_B, vbase + (int64_t)(t * KT) * vbytes, left, tid);
     };
 
-    f32x16 o[DB];
+    f32x16 o[QN][DB];
+    float m[QN], l[QN];                                      // running maximum (of the raw products) and this half's share of the sum
 #pragma unroll
-    for (int d = 0; d < DB; ++d) o[d] = zero16();
-    float m = -INFINITY, l = 0.f;                            // running maximum (of the raw products) and this half's share of the sum
-    const float c2 = a.scale * 1.4426950408889634f;
+    for (int n = 0; n < QN; ++n) {
+        m[n] = -INFINITY;
+        l[n] = 0.f;
+#pragma unroll
+        for (int d = 0; d < DB; ++d) o[n][d] = zero16();
+    }
+    const float c2 = a.scale * 1.4426950408889634f, slack = kSlack / c2;
+    bool bad = false;
 
-    if (ntiles > 0) fetch(0);
-    for (int t = 0; t < ntiles; ++t) {
+    if (t_begin < t_end) fetch(t_begin);
+    for (int t = t_begin; t < t_end; ++t) {
         wait_vm<0>();
         __syncthreads();
-        if (t + 1 < ntiles) fetch(t + 1);
+        if (t + 1 < t_end) fetch(t + 1);
         const char* kt = lds + (t % STAGES) * 2 * TILE_B;
         const char* vt = kt + TILE_B;
+        const int key0 = t * KT;
+        if (key0 >= seen_w) continue;
+        f32x16 s[QN][NB];
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
-            const int key0 = t * KT + nb * 32;
-            if (key0 >= seen_w) break;
-            f32x16 s = zero16();
 #pragma unroll
-            for (int ks = 0; ks < KS; ++ks) s = mma<T>(TL::row_frag(kt, nb * 32 + l31, ks, hi), qfr[ks], s);
-            const bool edge = key0 + 32 > full_w;
-            if (edge) {
+            for (int n = 0; n < QN; ++n) s[n][nb] = zero16();
 #pragma unroll
-                for (int r = 0; r < 16; ++r) s[r] = key0 + crow(r, hi) <= limit ? s[r] : -INFINITY;
+            for (int ks = 0; ks < KS; ++ks) {
+                const frag kfr = TL::row_frag(kt, nb * 32 + l31, ks, hi);
+#pragma unroll
+                for (int n = 0; n < QN; ++n) s[n][nb] = mma<T>(kfr, qfr[n][ks], s[n][nb]);
             }
-            float mx = s[0];
+        }
+        if (key0 + KT > full_w) {                            // some masked place in here
 #pragma unroll
-            for (int r = 1; r < 16; ++r) mx = fmaxf(mx, s[r]);
-            mx = fmaxf(mx, other_half(mx));
-            if (__any(mx > m)) {
-                const float mn = fmaxf(m, mx);
-                const float f = m == -INFINITY ? 0.f : exp2_((m - mn) * c2);
-                m = mn;
-                l *= f;
+            for (int nb = 0; nb < NB; ++nb) {
+                bad |= block_not_finite<T, D>(vt, nb * 32);
+#pragma unroll
+                for (int n = 0; n < QN; ++n) {
+                    const int limit = min(qw + 32 * n + l31 + shift, Tk - 1);
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) s[n][nb][r] = key0 + nb * 32 + crow(r, hi) <= limit ? s[n][nb][r] : -INFINITY;
+                }
+            }
+        }
+#pragma unroll
+        for (int n = 0; n < QN; ++n) {
+            float mx = s[n][0][0];
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[n][nb][r]);
+            mx = halves_max(mx);
+            if (__any(mx > m[n] + slack)) {                  // (the first visible key passes -inf)
+                const float mn = mx > m[n] + slack ? mx : m[n];
+                const float f = m[n] == -INFINITY ? 0.f : exp2_((m[n] - mn) * c2);
+                m[n] = mn;
+                l[n] *= f;
 #pragma unroll
                 for (int d = 0; d < DB; ++d)
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) o[d][r] *= f;
+                    for (int r = 0; r < 16; ++r) o[n][d][r] *= f;
             }
-            const float mc = m == -INFINITY ? 0.f : m * c2;
+            const float mc = m[n] == -INFINITY ? 0.f : m[n] * c2;
 #pragma unroll
-            for (int r = 0; r < 16; ++r) s[r] = exp2_(fmaf(s[r], c2, -mc));
+            for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) l += s[r];
-            if (edge && block_not_finite<T, D>(vt, nb * 32)) {
-                add_by_hand<T, D>(o, s, vt, nb * 32, [&](int j) { return key0 + j <= limit; });
-                continue;
-            }
+                for (int r = 0; r < 16; ++r) {
+                    s[n][nb][r] = exp2_(fmaf(s[n][nb][r], c2, -mc));
+                    l[n] += s[n][nb][r];
+                }
+        }
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
             for (int s2 = 0; s2 < 2; ++s2) {
-                const frag p = pack8<T>(s, s2);
+                frag p[QN];
 #pragma unroll
-                for (int d = 0; d < DB; ++d) o[d] = mma<T>(TL::col_frag(vt, nb * 32 + 16 * s2, d, lane), p, o[d]);
-            }
-        }
-    }
-
-    if (q < Tq) {
-        l += other_half(l);
-        const float inv = limit >= 0 ? 1.f / l : 0.f;         // no visible key: zero
-        T* orow = static_cast<T*>(a.out.p) + (int64_t)(qf + q) * a.out.row + (int64_t)head * a.out.head;
+                for (int n = 0; n < QN; ++n) p[n] = pack8<T>(s[n][nb], s2);
 #pragma unroll
-        for (int d = 0; d < DB; ++d)
+                for (int d = 0; d < DB; ++d) {
+                    const frag vfr = TL::col_frag(vt, nb * 32 + 16 * s2, d, lane);
 #pragma unroll
-            for (int r4 = 0; r4 < 4; ++r4) {
-                T* p = orow + 32 * d + 8 * r4 + 4 * hi;
-                if constexpr (sizeof(T) == 4) {
-                    *reinterpret_cast<f32x4*>(p) = (f32x4){o[d][4 * r4] * inv, o[d][4 * r4 + 1] * inv, o[d][4 * r4 + 2] * inv, o[d][4 * r4 + 3] * inv};
-                } else {
-                    s16x4 x;
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) x[i] = __builtin_bit_cast(short, (T)(o[d][4 * r4 + i] * inv));
-                    *reinterpret_cast<s16x4*>(p) = x;
+                    for (int n = 0; n < QN; ++n) o[n][d] = mma<T>(vfr, p[n], o[n][d]);
                 }
             }
-        if (a.lse && hi == 0) a.lse[(int64_t)head * a.q_rows + qf + q] = limit >= 0 ? m * c2 + log2_(l) : -INFINITY;
+    }
+
+    const int64_t prow = (int64_t)part * a.q_rows * a.kv_heads * a.group;
+    if (bad) {                                               // (wave-uniform)
+        for (int n = 0; n < 32 * QN; ++n) {
+            const int q = qw + n, limit = min(q + shift, Tk - 1);
+            if (q >= Tq) break;
+            float mm, ll, o0, o1;
+            solo_query<T, D>(a, qhead + (int64_t)(qf + q) * a.q.row, reinterpret_cast<const T*>(kbase), reinterpret_cast<const T*>(vbase), t_begin * KT,
+                             min(t_end * KT, limit + 1), c2, &mm, &ll, &o0, &o1);
+            if (a.parts > 1) {
+                const int64_t i = prow + (int64_t)(qf + q) * a.kv_heads * a.group + head;
+                a.part_o[i * D + lane] = o0;
+                if (D > 64) a.part_o[i * D + 64 + lane] = o1;
+                if (lane == 0) *reinterpret_cast<f32x2*>(a.part_ml + 2 * i) = (f32x2){mm * c2, ll};
+            } else {
+                const float inv = limit >= 0 ? 1.f / ll : 0.f;
+                T* orow = static_cast<T*>(a.out.p) + (int64_t)(qf + q) * a.out.row + (int64_t)head * a.out.head;
+                orow[lane] = (T)(o0 * inv);
+                if (D > 64) orow[64 + lane] = (T)(o1 * inv);
+                if (a.lse && lane == 0) a.lse[(int64_t)head * a.q_rows + qf + q] = limit >= 0 ? mm * c2 + log2_(ll) : -INFINITY;
+            }
+        }
+        return;
+    }
+#pragma unroll
+    for (int n = 0; n < QN; ++n) {
+        const int q = qw + 32 * n + l31;
+        if (q >= Tq) continue;
+        const float sum = halves_sum(l[n]);
+        if (a.parts > 1) {
+            const int64_t i = prow + (int64_t)(qf + q) * a.kv_heads * a.group + head;
+#pragma unroll
+            for (int d = 0; d < DB; ++d)
+#pragma unroll
+                for (int r4 = 0; r4 < 4; ++r4)
+                    store4<float>(a.part_o + i * D + 32 * d + 8 * r4 + 4 * hi, o[n][d][4 * r4], o[n][d][4 * r4 + 1], o[n][d][4 * r4 + 2], o[n][d][4 * r4 + 3]);
+            if (hi == 0) *reinterpret_cast<f32x2*>(a.part_ml + 2 * i) = (f32x2){m[n] * c2, sum};
+        } else {
+            const bool any = q + shift >= 0 && Tk > 0;
+            const float inv = any ? 1.f / sum : 0.f;         // no visible key: zero
+            T* orow = static_cast<T*>(a.out.p) + (int64_t)(qf + q) * a.out.row + (int64_t)head * a.out.head;
+#pragma unroll
+            for (int d = 0; d < DB; ++d)
+#pragma unroll
+                for (int r4 = 0; r4 < 4; ++r4)
+                    store4<T>(orow + 32 * d + 8 * r4 + 4 * hi, o[n][d][4 * r4] * inv, o[n][d][4 * r4 + 1] * inv, o[n][d][4 * r4 + 2] * inv, o[n][d][4 * r4 + 3] * inv);
+            if (a.lse && hi == 0) a.lse[(int64_t)head * a.q_rows + qf + q] = any ? m[n] * c2 + log2_(sum) : -INFINITY;
+        }
     }
 }
 
-template <typename T, int D> hipError_t run(const CausalArgs& a, hipStream_t s) {
-    constexpr int lds = Shape<T, D>::LDS_B;
+// Joins the parts of the keys, in order: a block is one query row, its threads walk the heads' channels.
+template <typename T, int D> __global__ __launch_bounds__(256) void causal_join_kernel(CausalArgs a) {
+    const int heads = a.kv_heads * a.group;
+    const int64_t row = blockIdx.x;
+    if (row < a.q_offsets[0] || row >= a.q_offsets[a.B]) return;
+    const Place pl = find_row(a.q_offsets, a.B, (int)row);
+    const int i = (int)row - a.q_offsets[pl.b], Tq = a.q_offsets[pl.b + 1] - a.q_offsets[pl.b], Tk = a.k_offsets[pl.b + 1] - a.k_offsets[pl.b];
+    const bool any = Tk > 0 && (!a.causal || i + Tk - Tq >= 0);
+    const int64_t step = a.q_rows * heads;
+    for (int c = threadIdx.x; c < heads * (D / 4); c += 256) {
+        const int h = c / (D / 4), d = c % (D / 4) * 4;
+        const int64_t i0 = row * heads + h;
+        float mm = -INFINITY, sum = 0.f;
+        for (int p = 0; p < a.parts; ++p) mm = fmaxf(mm, a.part_ml[2 * (i0 + p * step)]);
+        f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+        for (int p = 0; p < a.parts; ++p) {
+            const f32x2 ml = *reinterpret_cast<const f32x2*>(a.part_ml + 2 * (i0 + p * step));
+            if (ml[1] == 0.f) continue;                      // nothing visible in this part
+            const float f = ml[0] == -INFINITY ? 1.f : exp2_(ml[0] - mm);
+            const f32x4 x = *reinterpret_cast<const f32x4*>(a.part_o + (i0 + p * step) * D + d);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) acc[k] = fmaf(x[k], f, acc[k]);
+            sum = fmaf(ml[1], f, sum);
+        }
+        const float inv = any ? 1.f / sum : 0.f;
+        store4<T>(static_cast<T*>(a.out.p) + row * a.out.row + (int64_t)h * a.out.head + d, acc[0] * inv, acc[1] * inv, acc[2] * inv, acc[3] * inv);
+        if (a.lse && d == 0) a.lse[(int64_t)h * a.q_rows + row] = any ? mm + log2_(sum) : -INFINITY;
+    }
+}
+
+template <typename T, int D, int QN> hipError_t run(const CausalArgs& a, hipStream_t s) {
+    typedef Shape<T, D, QN> SH;
     static DeviceOnce once;
     if (once.need()) {
-        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(&causal_fwd_kernel<T, D>), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(&causal_fwd_kernel<T, D, QN>), hipFuncAttributeMaxDynamicSharedMemorySize, SH::LDS_B);
         if (e != hipSuccess) return e;
         once.mark();
     }
-    const int slots = (int)(a.q_rows / QB) + a.B;
-    hipLaunchKernelGGL((causal_fwd_kernel<T, D>), dim3((unsigned)work_blocks(a.kv_heads, a.group, slots)), dim3(256), lds, s, a, work_subs(a.kv_heads), slots);
+    const int slots = (int)(a.q_rows / SH::QB) + a.B;
+    hipLaunchKernelGGL((causal_fwd_kernel<T, D, QN>), dim3((unsigned)work_blocks(a.kv_heads, a.group * a.parts, slots)), dim3(256), SH::LDS_B, s, a,
+                       work_subs(a.kv_heads), slots);
+    if (a.parts > 1) hipLaunchKernelGGL((causal_join_kernel<T, D>), dim3((unsigned)a.q_rows), dim3(256), 0, s, a);
     return hipGetLastError();
 }
 
+template <typename T, int D> hipError_t pick(const CausalArgs& a, hipStream_t s) { return run<T, D, 1>(a, s); }
+
 }  // namespace
 
-int64_t causal_fwd_blocks(const CausalArgs& a) { return causal::work_blocks(a.kv_heads, a.group, (int)(a.q_rows / QB) + a.B); }
+int64_t causal_fwd_blocks(const CausalArgs& a) { return causal::work_blocks(a.kv_heads, a.group * a.parts, (int)(a.q_rows / 128) + a.B); }
+
+// Parts the keys are cut into: 1 unless the queries alone give too few workgroups (below 3 per CU) AND the keys are long (256 of them per part at
+// least).  Lengths are on the device, so the averages over the batch decide.
+int causal_fwd_parts(int64_t q_rows, int64_t k_rows, int B, int heads) {
+    if (B <= 0 || q_rows <= 0) return 1;
+    const int64_t groups = (q_rows + 127) / 128 > B ? (q_rows + 127) / 128 : B;
+    const int64_t want = 768 / (groups * heads), room = k_rows / B / 256;
+    const int64_t p = want < room ? want : room;
+    return p < 1 ? 1 : p > 32 ? 32 : (int)p;
+}
 
 hipError_t launch_causal_fwd(int dtype, int head_dim, const CausalArgs& a, hipStream_t s) {
     if (a.B <= 0 || a.q_rows <= 0) return hipSuccess;
-    if (head_dim == 64) return dtype == 0 ? run<float, 64>(a, s) : dtype == 1 ? run<f16_t, 64>(a, s) : run<bf16_t, 64>(a, s);
-    return dtype == 0 ? run<float, 128>(a, s) : dtype == 1 ? run<f16_t, 128>(a, s) : run<bf16_t, 128>(a, s);
+    if (head_dim == 64) return dtype == 0 ? pick<float, 64>(a, s) : dtype == 1 ? pick<f16_t, 64>(a, s) : pick<bf16_t, 64>(a, s);
+    return dtype == 0 ? pick<float, 128>(a, s) : dtype == 1 ? pick<f16_t, 128>(a, s) : pick<bf16_t, 128>(a, s);
 }

@@ -177,14 +177,17 @@ struct CausalArgs {
     float* lse;                    // optional [heads, q_rows]: base-2 log-sum-exp of the scaled scores (-inf: no visible key)
     const int32_t* q_offsets; const int32_t* k_offsets;
     int64_t q_rows;
-    int B, kv_heads, group, causal;
+    float* part_o; float* part_ml; // parts > 1: [parts, q_rows, heads, head_dim] and [.., 2] (base-2 maximum, sum)
+    int B, kv_heads, group, causal, parts;
     float scale;
 };
 struct CausalBwdArgs {
     CausalArgs f;                  // as in the forward call (out and lse read)
     Rows3 dout, dq, dk, dv;
     float* dsum;                   // [heads, q_rows] scratch: rowsum(dout out)
+    float* part_k; float* part_v;  // parts > 1: [parts, k_rows, kv_heads, head_dim] each
     int64_t k_rows;
+    int parts;
 };
 struct StepArgs {
     Rows3 q, k, v, out;            // q, out: row = stream; k, v: row = frame of a stream's cache, the streams k_batch / v_batch apart
@@ -211,7 +214,10 @@ int norm_rope_bwd_blocks(int64_t rows, int heads, int head_dim);
 hipError_t launch_norm_rope(int dtype, int head_dim, NormRopeArgs a, hipStream_t s);
 hipError_t launch_norm_rope_bwd(int dtype, int head_dim, NormRopeArgs a, float* dgq, float* dgk, int accumulate, hipStream_t s);
 int64_t causal_fwd_blocks(const CausalArgs& a);
+int causal_fwd_parts(int64_t q_rows, int64_t k_rows, int B, int heads);
 hipError_t launch_causal_fwd(int dtype, int head_dim, const CausalArgs& a, hipStream_t s);
+int causal_bwd_parts(int64_t q_rows, int64_t k_rows, int B, int heads, int kv_heads);
+int64_t causal_bwd_blocks(const CausalBwdArgs& b);
 hipError_t launch_causal_bwd(int dtype, int head_dim, const CausalBwdArgs& a, hipStream_t s);
 
 // ---- depthwise conv + folded BN + SiLU ------------------------------------------------------------

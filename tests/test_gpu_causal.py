@@ -228,6 +228,29 @@ def test_attention_long_rows_past_32_bit_offsets(eng):
     oracle.check(got, *(x[99:] for x in oracle.attention(q, k, v, [100], [n])), 'step')
 
 
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('H,G,D', [(4, 1, 64), (2, 2, 128)])
+def test_few_queries_over_many_keys(ops, eng, dtype, H, G, D):
+    """The keys are cut into parts here (and the queries of a key tile in the backward): unequal clips, parts that see nothing, values that are not finite."""
+    import some_amd._lib as _lib
+    ql, kl = [130, 3, 1, 40], [3001, 2, 1500, 40]
+    assert _lib.load().some_op_causal_attention_bytes(None, H, G, D, 4, sum(ql), sum(kl)) > 0
+    q, k, v = _qkv(84, sum(ql), sum(kl), H, G, D, dtype)
+    dout = _normal(87, sum(ql), H, D, dtype=dtype)
+    leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+    out = ops.causal_attention(*leaves, _batch(ql), kv_batch=_batch(kl))
+    grads = torch.autograd.grad(out, leaves, dout)
+    w = oracle.attention(q, k, v, ql, kl, dout=dout)
+    for i, (name, got) in enumerate(zip(('out', 'dq', 'dk', 'dv'), (out.detach(), *grads))):
+        oracle.check(got, w[2 * i], w[2 * i + 1], name)
+    v2 = v.clone()
+    v2[2999] = math.nan                                            # seen by the clip's last two queries
+    got = eng.causal_attention(q, k, v2, _batch(ql), kv_batch=_batch(kl))
+    oracle.check(got[:128], w[0][:128], w[1][:128], 'before')
+    assert torch.isnan(got[128:130]).all()
+    oracle.check(got[130:], w[0][130:], w[1][130:], 'other clips')
+
+
 def test_rows_behind_the_last_clip_stay(eng):
     """Through the C ABI: offsets that end before the arrays do."""
     import some_amd._lib as _lib
@@ -241,13 +264,13 @@ def test_rows_behind_the_last_clip_stay(eng):
     st = torch.cuda.current_stream().cuda_stream
     s3 = lambda t: (t.data_ptr(), t.stride(0), t.stride(1))          # noqa: E731
     off = b.frame_offsets_dev.data_ptr()
-    _lib.check(h, lib.some_op_causal_attention(h, 2, D, *s3(q), H, *s3(k), *s3(v), G, off, off, b.B, M + extra, M + extra, 1, 0.125, *s3(out), lse.data_ptr(), st))
+    _lib.check(h, lib.some_op_causal_attention(h, 2, D, *s3(q), H, *s3(k), *s3(v), G, off, off, b.B, M + extra, M + extra, 1, 0.125, *s3(out), lse.data_ptr(), None, 0, st))
     assert (out[M:] == 7).all() and (lse[:, M:] == 7).all()
     assert torch.equal(out[:M], eng.causal_attention(q[:M], k[:M], v[:M], b))
-    dout, dsum = torch.ones_like(q), torch.full_like(lse, 7.0)
+    dout, work = torch.ones_like(q), torch.empty(1 << 24, dtype=torch.uint8, device='cuda')
     d = [torch.full_like(t, 7.0) for t in (q, k, v)]
     _lib.check(h, lib.some_train_causal_attention_bwd(h, 2, D, *s3(q), H, *s3(k), *s3(v), G, off, off, b.B, M + extra, M + extra, 1, 0.125, *s3(out), lse.data_ptr(),
-                                                      *s3(dout), *s3(d[0]), *s3(d[1]), *s3(d[2]), dsum.data_ptr(), st))
+                                                      *s3(dout), *s3(d[0]), *s3(d[1]), *s3(d[2]), work.data_ptr(), work.numel(), st))
     assert all((t[M:] == 7).all() for t in d) and not any((t[:M] == 7).all() for t in d)
 
 
