@@ -38,47 +38,59 @@ def heads_view(x: torch.Tensor, name: str, head_dim: int) -> torch.Tensor:
         if x.shape[1] == 0 or x.shape[1] % head_dim:
             raise ValueError(f'{name}: {x.shape[1]} columns are not a multiple of head_dim {head_dim}')
         x = x.unflatten(1, (x.shape[1] // head_dim, head_dim))
-    if x.dim() != 3 or x.shape[1] == 0 or (head_dim and x.shape[2] != head_dim):
-        raise ValueError(f'{name} must be [rows, heads, head_dim{"" if not head_dim else f" = {head_dim}"}], got {tuple(x.shape)}')
-    if x.shape[2] not in HEAD_DIMS:
-        raise ValueError(f'{name}: head_dim must be one of {HEAD_DIMS}, got {x.shape[2]}')
+    shape = x.shape
+    if len(shape) != 3 or shape[1] == 0 or (head_dim and shape[2] != head_dim):
+        raise ValueError(f'{name} must be [rows, heads, head_dim{"" if not head_dim else f" = {head_dim}"}], got {tuple(shape)}')
+    if shape[2] not in HEAD_DIMS:
+        raise ValueError(f'{name}: head_dim must be one of {HEAD_DIMS}, got {shape[2]}')
     return x
 
 
 def readable(x: torch.Tensor) -> torch.Tensor:
     """``x`` itself if the library reads its layout in place, else a contiguous copy."""
-    size = x.element_size()
-    if x.stride(-1) == 1 and not x.data_ptr() & 15:
-        for n, s in zip(x.shape[:-1], x.stride()[:-1]):
-            if n > 1 and (s < 0 or s * size & 15):
-                break
-        else:
-            if x.shape[-3] <= 1 or x.stride(-3) * size < _MAX_ROW_BYTES:
-                return x
+    return x if _place(x) is not None else aligned(x)
+
+
+def aligned(x: torch.Tensor) -> torch.Tensor:
     x = x.contiguous()
-    return x if not x.data_ptr() & 15 else x.clone()
+    return x.clone() if x.data_ptr() & 15 else x
 
 
-def _rows(x: torch.Tensor):
-    """(address, row stride, head stride) of a [..., rows, heads, head_dim] tensor; a dimension of one entry has no stride to speak of."""
-    return x.data_ptr(), x.stride(-3) if x.shape[-3] > 1 else 0, x.stride(-2) if x.shape[-2] > 1 else 0
+def _place(x: torch.Tensor):
+    """(address, row stride, head stride) of a [.., rows, heads, head_dim] tensor, None if the library cannot read it in place.  A dimension of
+    one entry has no stride to speak of."""
+    p, st, shape = x.data_ptr(), x.stride(), x.shape
+    if shape[-3] == 0:
+        return 0, 0, 0
+    row, head = st[-3] if shape[-3] > 1 else 0, st[-2] if shape[-2] > 1 else 0
+    mask = 3 if x.dtype is torch.float32 else 7                     # 16 bytes in elements
+    if p & 15 or st[-1] != 1 or row < 0 or head < 0 or (row | head) & mask or row >= _MAX_ROW_BYTES // x.element_size():
+        return None
+    return p, row, head
 
 
-def check_device(device: torch.device, **tensors):
-    for name, t in tensors.items():
+def check_device(device: torch.device, *tensors):
+    first = tensors[0].device
+    for t in tensors:
         d = t.device
-        if d.type != 'cuda' or (device.index is not None and d.index != device.index):
-            raise ValueError(f'{name} is on {d}, the operators run on {device}')
-    ds = {t.device for t in tensors.values()}
-    if len(ds) > 1:
-        raise ValueError(f'tensors on several devices: {sorted(map(str, ds))}')
+        if d.type != 'cuda' or d.index != first.index or (device.index is not None and d.index != device.index):
+            raise ValueError(f'a tensor is on {d}: the operators run on {device}, all tensors of a call on one device')
+
+
+_get_device, _raw_stream = torch._C._cuda_getDevice if hasattr(torch._C, '_cuda_getDevice') else torch.cuda.current_device, getattr(torch._C, '_cuda_getCurrentRawStream', None)
+
+
+def stream_of(t: torch.Tensor) -> int:
+    """Address of the current stream of the tensor's device (torch.cuda.current_stream builds an object per call: 3 us of a 10 us call)."""
+    return _raw_stream(t.device.index) if _raw_stream is not None else torch.cuda.current_stream(t.device).cuda_stream
 
 
 class on_device:
     """Makes the tensors' device current around a launch (a stream belongs to its device)."""
+    __slots__ = ('want', 'prev')
 
     def __init__(self, t: torch.Tensor):
-        self.want, self.prev = t.device.index, torch.cuda.current_device()
+        self.want, self.prev = t.device.index, _get_device()
 
     def __enter__(self):
         if self.want != self.prev:
@@ -105,37 +117,39 @@ def check_norm_rope(device, q, k, gamma_q, gamma_k, positions):
             raise ValueError(f'{name} must be float32 [{D}]')
     if positions.dtype not in (torch.int32, torch.int64) or positions.shape != (q.shape[0],):
         raise ValueError(f'positions must be int32 or int64 [{q.shape[0]}], got {positions.dtype} {tuple(positions.shape)}')
-    check_device(device, q=q, k=k, gamma_q=gamma_q, gamma_k=gamma_k, positions=positions)
+    check_device(device, q, k, gamma_q, gamma_k, positions)
     return q, k
 
 
-def aligned(x: torch.Tensor) -> torch.Tensor:
-    x = x.contiguous()
-    return x.clone() if x.data_ptr() & 15 else x
+def _gain(g: torch.Tensor) -> torch.Tensor:
+    return g if g.is_contiguous() and not g.data_ptr() & 15 else aligned(g)
 
 
 def norm_rope_forward(lib, h, stream, q, k, gamma_q, gamma_k, positions, theta, eps):
     """Launch on checked [rows, heads, head_dim] views -> two new contiguous tensors."""
-    q, k, gamma_q, gamma_k, positions = readable(q), readable(k), aligned(gamma_q), aligned(gamma_k), positions.contiguous()
-    D = q.shape[2]
-    yq, yk = q.new_empty(q.shape), k.new_empty(k.shape)
-    _lib.check(h, lib.some_op_qk_norm_rope(h, DTYPES[q.dtype], D, *_rows(q), q.shape[1], *_rows(k), k.shape[1], q.shape[0], gamma_q.data_ptr(),
-                                           gamma_k.data_ptr(), positions.data_ptr(), positions.dtype == torch.int64, float(theta), float(eps), *_rows(yq),
-                                           *_rows(yk), stream))
+    q, k, gamma_q, gamma_k, positions = readable(q), readable(k), _gain(gamma_q), _gain(gamma_k), positions.contiguous()
+    (M, H, D), G = q.shape, k.shape[1]
+    yq, yk = q.new_empty((M, H, D)), k.new_empty((M, G, D))
+    rc = lib.some_op_qk_norm_rope(h, DTYPES[q.dtype], D, *_place(q), H, *_place(k), G, M, gamma_q.data_ptr(), gamma_k.data_ptr(), positions.data_ptr(),
+                                  positions.dtype is torch.int64, theta, eps, yq.data_ptr(), H * D, D, yk.data_ptr(), G * D, D, stream)
+    if rc:
+        _lib.check(h, rc)
     return yq, yk
 
 
 def norm_rope_backward(lib, h, stream, q, k, gamma_q, gamma_k, positions, theta, eps, dyq, dyk, dgq, dgk, accumulate):
     """-> (dq, dk); the gain gradients go into ``dgq`` / ``dgk``."""
-    q, k, gamma_q, gamma_k, positions = readable(q), readable(k), aligned(gamma_q), aligned(gamma_k), positions.contiguous()
+    q, k, gamma_q, gamma_k, positions = readable(q), readable(k), _gain(gamma_q), _gain(gamma_k), positions.contiguous()
     dyq, dyk = readable(dyq), readable(dyk)
-    D = q.shape[2]
-    dq, dk = q.new_empty(q.shape), k.new_empty(k.shape)
-    work = torch.empty(lib.some_train_qk_norm_rope_bytes(h, q.shape[0], q.shape[1], k.shape[1], D), dtype=torch.uint8, device=q.device)
-    _lib.check(h, lib.some_train_qk_norm_rope_bwd(h, DTYPES[q.dtype], D, *_rows(q), q.shape[1], *_rows(k), k.shape[1], q.shape[0], gamma_q.data_ptr(),
-                                                  gamma_k.data_ptr(), positions.data_ptr(), positions.dtype == torch.int64, float(theta), float(eps),
-                                                  *_rows(dyq), *_rows(dyk), *_rows(dq), *_rows(dk), dgq.data_ptr(), dgk.data_ptr(), int(accumulate),
-                                                  work.data_ptr(), work.numel(), stream))
+    (M, H, D), G = q.shape, k.shape[1]
+    dq, dk = q.new_empty((M, H, D)), k.new_empty((M, G, D))
+    n = lib.some_train_qk_norm_rope_bytes(h, M, H, G, D)
+    work = gamma_q.new_empty((n + 3) // 4)
+    rc = lib.some_train_qk_norm_rope_bwd(h, DTYPES[q.dtype], D, *_place(q), H, *_place(k), G, M, gamma_q.data_ptr(), gamma_k.data_ptr(), positions.data_ptr(),
+                                         positions.dtype is torch.int64, theta, eps, *_place(dyq), *_place(dyk), dq.data_ptr(), H * D, D, dk.data_ptr(),
+                                         G * D, D, dgq.data_ptr(), dgk.data_ptr(), accumulate, work.data_ptr(), n, stream)
+    if rc:
+        _lib.check(h, rc)
     return dq, dk
 
 
@@ -162,34 +176,42 @@ def check_attention(device, q, k, v, batch, kv_batch, head_dim):
         raise ValueError(f'{batch.B} clips of queries, {kv.B} of keys')
     if q.shape[0] != batch.total_frames or k.shape[0] != kv.total_frames:
         raise ValueError(f'q has {q.shape[0]} rows (the batch {batch.total_frames}), k and v {k.shape[0]} (the batch {kv.total_frames})')
-    check_device(device, q=q, k=k, v=v, frame_offsets=batch.frame_offsets_dev, kv_frame_offsets=kv.frame_offsets_dev)
+    check_device(device, q, k, v, batch.frame_offsets_dev, kv.frame_offsets_dev)
     return q, k, v, kv
 
 
 def attention_forward(lib, h, stream, q, k, v, batch, kv, causal, scale, want_lse):
     """Launch on checked, readable views -> (out, lse or None)."""
-    out = q.new_empty(q.shape)
-    lse = torch.empty((q.shape[1], q.shape[0]), dtype=torch.float32, device=q.device) if want_lse else None
-    n = lib.some_op_causal_attention_bytes(h, q.shape[1], k.shape[1], q.shape[2], batch.B, q.shape[0], k.shape[0])
+    (M, H, D), (N, G, _) = q.shape, k.shape
+    out = q.new_empty((M, H, D))
+    lse = torch.empty((H, M), dtype=torch.float32, device=q.device) if want_lse else None
+    n = lib.some_op_causal_attention_bytes(h, H, G, D, batch.B, M, N)
     work = torch.empty(n, dtype=torch.uint8, device=q.device) if n else None
-    _lib.check(h, lib.some_op_causal_attention(h, DTYPES[q.dtype], q.shape[2], *_rows(q), q.shape[1], *_rows(k), *_rows(v), k.shape[1],
-                                               batch.frame_offsets_dev.data_ptr(), kv.frame_offsets_dev.data_ptr(), batch.B, q.shape[0], k.shape[0],
-                                               int(causal), scale, *_rows(out), lse.data_ptr() if want_lse else None, work.data_ptr() if n else None, n, stream))
+    rc = lib.some_op_causal_attention(h, DTYPES[q.dtype], D, *_place(q), H, *_place(k), *_place(v), G, batch.frame_offsets_dev.data_ptr(),
+                                      kv.frame_offsets_dev.data_ptr(), batch.B, M, N, causal, scale, out.data_ptr(), H * D, D,
+                                      lse.data_ptr() if want_lse else None, work.data_ptr() if n else None, n, stream)
+    if rc:
+        _lib.check(h, rc)
     return out, lse
 
 
 def attention_backward(lib, h, stream, q, k, v, batch, kv, causal, scale, out, lse, dout):
     dout = readable(dout)
-    dq, dk, dv = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
-    work = torch.empty(lib.some_train_causal_attention_bytes(h, q.shape[1], k.shape[1], q.shape[2], batch.B, q.shape[0], k.shape[0]), dtype=torch.uint8, device=q.device)
-    _lib.check(h, lib.some_train_causal_attention_bwd(h, DTYPES[q.dtype], q.shape[2], *_rows(q), q.shape[1], *_rows(k), *_rows(v), k.shape[1],
-                                                      batch.frame_offsets_dev.data_ptr(), kv.frame_offsets_dev.data_ptr(), batch.B, q.shape[0], k.shape[0],
-                                                      int(causal), scale, *_rows(out), lse.data_ptr(), *_rows(dout), *_rows(dq), *_rows(dk), *_rows(dv),
-                                                      work.data_ptr(), work.numel(), stream))
+    (M, H, D), (N, G, _) = q.shape, k.shape
+    dq, dk, dv = q.new_empty((M, H, D)), k.new_empty((N, G, D)), v.new_empty((N, G, D))
+    n = lib.some_train_causal_attention_bytes(h, H, G, D, batch.B, M, N)
+    work = torch.empty(n, dtype=torch.uint8, device=q.device)
+    rc = lib.some_train_causal_attention_bwd(h, DTYPES[q.dtype], D, *_place(q), H, *_place(k), *_place(v), G, batch.frame_offsets_dev.data_ptr(),
+                                             kv.frame_offsets_dev.data_ptr(), batch.B, M, N, causal, scale, out.data_ptr(), H * D, D, lse.data_ptr(),
+                                             *_place(dout), dq.data_ptr(), H * D, D, dk.data_ptr(), G * D, D, dv.data_ptr(), G * D, D, work.data_ptr(), n,
+                                             stream)
+    if rc:
+        _lib.check(h, rc)
     return dq, dk, dv
 
 
-def attention_step(lib, h, stream, device, q, k_cache, v_cache, lengths, max_length, scale):
+def check_step(device, q, k_cache, v_cache, lengths, max_length):
+    """-> (q, the caches' places, max_length), checked."""
     q = heads_view(q, 'q', 0)
     B, H, D = q.shape
     for name, c in (('k_cache', k_cache), ('v_cache', v_cache)):
@@ -197,32 +219,42 @@ def attention_step(lib, h, stream, device, q, k_cache, v_cache, lengths, max_len
             raise ValueError(f'{name} must be [{B}, capacity, kv_heads, {D}], k and v alike')
         if c.dtype != q.dtype:
             raise TypeError(f'q and {name} must have one type, got {q.dtype} and {c.dtype}')
-    if H % k_cache.shape[2]:
-        raise ValueError(f'{H} query heads are not a multiple of {k_cache.shape[2]} key / value heads')
+    capacity, G = k_cache.shape[1:3]
+    if H % G:
+        raise ValueError(f'{H} query heads are not a multiple of {G} key / value heads')
     if not isinstance(lengths, torch.Tensor) or lengths.dtype != torch.int32 or lengths.shape != (B,):
         raise ValueError(f'lengths must be int32 [{B}]')
-    capacity = k_cache.shape[1]
     max_length = capacity if max_length is None else int(max_length)
     if not 0 <= max_length <= capacity:
         raise ValueError(f'max_length {max_length} outside the cache of {capacity} frames')
-    check_device(device, q=q, k_cache=k_cache, v_cache=v_cache, lengths=lengths)
+    check_device(device, q, k_cache, v_cache, lengths)
+    places = []
     for name, c in (('k_cache', k_cache), ('v_cache', v_cache)):
-        if readable(c) is not c or (B > 1 and (c.stride(0) < 0 or c.stride(0) * c.element_size() & 15)):
+        p, stride = _place(c), c.stride(0) if B > 1 else 0
+        if p is None or stride < 0 or stride & (3 if c.dtype is torch.float32 else 7):
             raise ValueError(f'{name}: unsupported layout (head_dim contiguous, 16-byte aligned rows, heads and streams; a copy per frame is refused)')
-    scale = default_scale(scale, D)
+        places += [p[0], stride, p[1], p[2]]
+    return q, places, max_length
+
+
+def attention_step(lib, h, stream, q, places, G, lengths, max_length, scale):
     q, lengths = readable(q), lengths.contiguous()
-    out = q.new_empty(q.shape)
-    G = k_cache.shape[2]
-    with on_device(q):
-        n = lib.some_op_attention_step_bytes(h, B, H, G, D, max_length)
-        work = torch.empty(n, dtype=torch.uint8, device=q.device)
-        (ka, kr, kh), (va, vr, vh) = _rows(k_cache), _rows(v_cache)
-        kb, vb = (k_cache.stride(0), v_cache.stride(0)) if B > 1 else (0, 0)
-        _lib.check(h, lib.some_op_attention_step(h, DTYPES[q.dtype], D, *_rows(q), H, ka, kb, kr, kh, va, vb, vr, vh, G, lengths.data_ptr(), B, max_length,
-                                                 scale, *_rows(out), work.data_ptr(), n, stream()))
+    B, H, D = q.shape
+    out = q.new_empty((B, H, D))
+    n = lib.some_op_attention_step_bytes(h, B, H, G, D, max_length)
+    work = torch.empty(n, dtype=torch.uint8, device=q.device)
+    rc = lib.some_op_attention_step(h, DTYPES[q.dtype], D, *_place(q), H, *places, G, lengths.data_ptr(), B, max_length, scale, out.data_ptr(), H * D, D,
+                                    work.data_ptr(), n, stream)
+    if rc:
+        _lib.check(h, rc)
     return out
 
 
 def no_gradient_lost(what: str, *tensors):
-    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t.requires_grad:
+                break
+        else:
+            return
         raise RuntimeError(f'{what} is not differentiable: use the operator of the same name in TrainOps, or torch.no_grad()')

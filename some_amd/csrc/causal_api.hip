@@ -1,5 +1,6 @@
 // C ABI of the causal attention operators (include/some_amd.h, "causal attention over packed clips"): argument checks + launches.
 #include <cmath>
+#include <cstring>
 #include <string>
 
 #include "internal.h"
@@ -39,7 +40,15 @@ size_t dsum_bytes(int heads, int64_t q_rows) { return ((size_t)heads * q_rows * 
 
 bool fill_turns(NormRopeArgs& a, double theta, int head_dim) {
     if (!(theta > 0.0) || !std::isfinite(theta)) return false;
-    for (int i = 0; i < head_dim / 2; ++i) a.turns[i] = std::pow(theta, -2.0 * i / head_dim) / 6.283185307179586476925286766559;
+    // the last table of this thread (a function of these two values alone): 32 powers are 2 us of a 10 us call
+    thread_local double last_theta = 0.0, table[64];
+    thread_local int last_dim = 0;
+    if (theta != last_theta || head_dim != last_dim) {
+        for (int i = 0; i < head_dim / 2; ++i) table[i] = std::pow(theta, -2.0 * i / head_dim) / 6.283185307179586476925286766559;
+        last_theta = theta;
+        last_dim = head_dim;
+    }
+    std::memcpy(a.turns, table, sizeof(table));
     return true;
 }
 

@@ -181,14 +181,15 @@ __global__ __launch_bounds__(256, (D == 128 && sizeof(T) == 4 ? 1 : 2)) void cau
 // ---- dK, dV --------------------------------------------------------------------------------------------------------------------------------
 constexpr int KB = 128;                          // keys per workgroup
 template <typename T, int D> struct DkvShape {
-    static constexpr int QT = sizeof(T) == 4 ? 32 : 64;                    // queries per tile
+    static constexpr bool V_LDS = D == 128;                                // V fragments from LDS, not registers: lets two waves share a SIMD (f32: no spills)
+    static constexpr int QT = sizeof(T) == 4 || V_LDS ? 32 : 64;           // queries per tile
     static constexpr int TILE_B = QT * D * (int)sizeof(T);
     static constexpr int STAGE_B = 2 * TILE_B + 2 * 64 * 4;                // Q, dO, lse, D
-    static constexpr int LDS_B = 2 * STAGE_B;
+    static constexpr int LDS_B = 2 * STAGE_B + (V_LDS ? KB * D * (int)sizeof(T) : 0);
 };
 
 template <typename T, int D>
-__global__ __launch_bounds__(256, (D == 128 ? 1 : 2)) void causal_dkv_kernel(CausalBwdArgs b, int nsub, int slots) {
+__global__ __launch_bounds__(256, (D == 128 && sizeof(T) == 4 ? 1 : 2)) void causal_dkv_kernel(CausalBwdArgs b, int nsub, int slots) {
     constexpr int QT = DkvShape<T, D>::QT, NB = QT / 32, KS = D / 16, DB = D / 32, TILE_B = DkvShape<T, D>::TILE_B, STAGE_B = DkvShape<T, D>::STAGE_B;
     constexpr bool F16 = __is_same(T, f16_t);
     typedef Tile<T, D> TL;
@@ -211,17 +212,28 @@ __global__ __launch_bounds__(256, (D == 128 ? 1 : 2)) void causal_dkv_kernel(Cau
     const int64_t kr = kf + min(key, Tk - 1);
     const T* krow = static_cast<const T*>(a.k.p) + kr * a.k.row + (int64_t)w.kvh * a.k.head + 8 * hi;
     const T* vrow = static_cast<const T*>(a.v.p) + kr * a.v.row + (int64_t)w.kvh * a.v.head + 8 * hi;
-    frag kfr[KS], vfr[KS];
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks) {
-        kfr[ks] = load8<T>(krow + 16 * ks);
-        vfr[ks] = load8<T>(vrow + 16 * ks);
-    }
-
     // the first query that sees key k0 is k0 - shift
     const int t0 = max(0, k0 - shift) / QT, nt = max(0, (Tq + QT - 1) / QT - t0);
     const int total = nt * a.group;                          // (head, tile) pairs; this part's share of them:
     const int it0 = (int)((int64_t)total * w.g / b.parts), it1 = (int)((int64_t)total * (w.g + 1) / b.parts);
+    constexpr bool V_LDS = DkvShape<T, D>::V_LDS;
+    frag kfr[KS], vreg[V_LDS ? 1 : KS];
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+        kfr[ks] = load8<T>(krow + 16 * ks);
+        if constexpr (!V_LDS) vreg[ks] = load8<T>(vrow + 16 * ks);
+    }
+    const char* vtile = lds + 2 * STAGE_B;
+    if (V_LDS && it0 < it1) {                                // (its first iteration waits for the copy)
+        Copier<T, D, KB, 256> cv;
+        cv.init(a.v.row * (int64_t)sizeof(T), tid);
+        cv.run(lds + 2 * STAGE_B, reinterpret_cast<const char*>(static_cast<const T*>(a.v.p) + (int64_t)(kf + k0) * a.v.row + (int64_t)w.kvh * a.v.head), Tk - k0, tid);
+    }
+    const auto vfr = [&](int ks) {
+        if constexpr (V_LDS) return TL::row_frag(vtile, wave * 32 + l31, ks, hi);
+        else return vreg[ks];
+    };
+
     const int64_t qbytes = a.q.row * (int64_t)sizeof(T), gbytes = b.dout.row * (int64_t)sizeof(T);
     const char* qbase = reinterpret_cast<const char*>(static_cast<const T*>(a.q.p) + (int64_t)qf * a.q.row + (int64_t)w.kvh * a.group * a.q.head);
     const char* gbase = reinterpret_cast<const char*>(static_cast<const T*>(b.dout.p) + (int64_t)qf * b.dout.row + (int64_t)w.kvh * a.group * b.dout.head);
@@ -269,7 +281,7 @@ __global__ __launch_bounds__(256, (D == 128 ? 1 : 2)) void causal_dkv_kernel(Cau
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
                 s = mma<T>(TL::row_frag(qt, nb * 32 + l31, ks, hi), kfr[ks], s);
-                dp = mma<T>(TL::row_frag(gt, nb * 32 + l31, ks, hi), vfr[ks], dp);
+                dp = mma<T>(TL::row_frag(gt, nb * 32 + l31, ks, hi), vfr(ks), dp);
             }
             const bool edge = qb0 + shift < kw + 31 || qb0 + 32 > Tq || kw + 32 > Tk;
 #pragma unroll

@@ -314,9 +314,6 @@ class Engine:
         return out
 
     # ---- causal attention over packed clips (some_amd/causal.py; the differentiable forms are TrainOps') ----------------------------
-    def _raw_stream(self):
-        return torch.cuda.current_stream(self.device).cuda_stream
-
     def _serve(self):
         if self.host_only:
             raise RuntimeError('a host-only engine runs no device operators')
@@ -331,8 +328,8 @@ class Engine:
         q3, k3 = causal.check_norm_rope(self.device, q, k, gamma_q, gamma_k, positions)
         causal.no_gradient_lost('Engine.qk_norm_rope', q, k, gamma_q, gamma_k)
         with causal.on_device(q3):
-            yq, yk = causal.norm_rope_forward(lib, h, self._raw_stream(), q3, k3, gamma_q, gamma_k, positions, theta, eps)
-        return yq.view(q.shape), yk.view(k.shape)
+            yq, yk = causal.norm_rope_forward(lib, h, causal.stream_of(q3), q3, k3, gamma_q, gamma_k, positions, float(theta), float(eps))
+        return yq if q3 is q else yq.view(q.shape), yk if k3 is k else yk.view(k.shape)
 
     def causal_attention(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, batch: ClipBatch, kv_batch: Optional[ClipBatch] = None,
                          causal_mask: bool = True, scale: Optional[float] = None, head_dim: int = 0) -> torch.Tensor:
@@ -345,9 +342,9 @@ class Engine:
         causal.no_gradient_lost('Engine.causal_attention', q, k, v)
         scale = causal.default_scale(scale, q3.shape[2])
         with causal.on_device(q3):
-            out, _ = causal.attention_forward(lib, h, self._raw_stream(), causal.readable(q3), causal.readable(k3), causal.readable(v3), batch, kv,
-                                              causal_mask, scale, False)
-        return out.view(q.shape)
+            out, _ = causal.attention_forward(lib, h, causal.stream_of(q3), causal.readable(q3), causal.readable(k3), causal.readable(v3), batch, kv,
+                                              bool(causal_mask), scale, False)
+        return out if q3 is q else out.view(q.shape)
 
     def attention_step(self, q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, lengths: torch.Tensor,
                        max_length: Optional[int] = None, scale: Optional[float] = None) -> torch.Tensor:
@@ -356,7 +353,10 @@ class Engine:
         knows one below the capacity (lengths beyond it are cut).  Returns [B, heads, D]; a stream of length 0 gets 0."""
         lib, h = self._serve()
         causal.no_gradient_lost('Engine.attention_step', q, k_cache, v_cache)
-        return causal.attention_step(lib, h, self._raw_stream, self.device, q, k_cache, v_cache, lengths, max_length, scale)
+        q3, places, max_length = causal.check_step(self.device, q, k_cache, v_cache, lengths, max_length)
+        scale = causal.default_scale(scale, q3.shape[2])
+        with causal.on_device(q3):
+            return causal.attention_step(lib, h, causal.stream_of(q3), q3, places, k_cache.shape[2], lengths, max_length, scale)
 
     # ---- graph replay of a whole step ------------------------------------------------------------
     def graph_runner(self, audio: torch.Tensor, batch: ClipBatch, head_mode: int = _lib.HEAD_LOGITS, quantized: bool = False,

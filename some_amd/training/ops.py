@@ -1250,37 +1250,43 @@ def _attention_bwd16(ctx, dout):
     return dqkv16
 
 
+def _stream_for(ops: TrainOps, t: torch.Tensor) -> int:
+    return ops._lane_ptrs[ops._lane] if ops._pinned_stream is not None else causal.stream_of(t)
+
+
 class _QkNormRope(torch.autograd.Function):
     @staticmethod
     def forward(ctx, ops, q, k, gamma_q, gamma_k, positions, theta, eps):
         D = gamma_q.shape[0]
         q3, k3 = causal.heads_view(q, 'q', D), causal.heads_view(k, 'k', D)
         with causal.on_device(q3):
-            yq, yk = causal.norm_rope_forward(ops.lib, ops.h, ops.stream(), q3, k3, gamma_q, gamma_k, positions, theta, eps)
+            yq, yk = causal.norm_rope_forward(ops.lib, ops.h, _stream_for(ops, q3), q3, k3, gamma_q, gamma_k, positions, theta, eps)
         ctx.ops, ctx.theta, ctx.eps = ops, theta, eps
         ctx.gparams = gamma_q, gamma_k                            # identities only: looked up among the gradient sinks in backward
         ctx.shapes = q.shape, k.shape
         ctx.save_for_backward(q3, k3, gamma_q, gamma_k, positions)
-        return yq.view(q.shape), yk.view(k.shape)
+        return yq if q3 is q else yq.view(q.shape), yk if k3 is k else yk.view(k.shape)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dyq, dyk):
         ops: TrainOps = ctx.ops
         q, k, gamma_q, gamma_k, positions = ctx.saved_tensors
-        dyq = torch.zeros_like(q, memory_format=torch.contiguous_format) if dyq is None else dyq.reshape(q.shape)
-        dyk = torch.zeros_like(k, memory_format=torch.contiguous_format) if dyk is None else dyk.reshape(k.shape)
+        dyq = torch.zeros_like(q, memory_format=torch.contiguous_format) if dyq is None else dyq if dyq.dim() == 3 else dyq.reshape(q.shape)
+        dyk = torch.zeros_like(k, memory_format=torch.contiguous_format) if dyk is None else dyk if dyk.dim() == 3 else dyk.reshape(k.shape)
         pq, pk = ctx.gparams
         sq, sk = ops.sink(pq), ops.sink(pk)
         sunk = sq is not None and sk is not None and sq is not sk and ctx.needs_input_grad[3] and ctx.needs_input_grad[4]
         dgq, dgk = (sq, sk) if sunk else (torch.empty_like(gamma_q), torch.empty_like(gamma_k))
         with causal.on_device(q):
-            dq, dk = causal.norm_rope_backward(ops.lib, ops.h, ops.stream(), q, k, gamma_q, gamma_k, positions, ctx.theta, ctx.eps, dyq, dyk, dgq, dgk, sunk)
+            dq, dk = causal.norm_rope_backward(ops.lib, ops.h, _stream_for(ops, q), q, k, gamma_q, gamma_k, positions, ctx.theta, ctx.eps, dyq, dyk, dgq, dgk,
+                                               sunk)
         if sunk:
             ops.deposited(pq)
             ops.deposited(pk)
             dgq = dgk = None
-        return None, dq.view(ctx.shapes[0]), dk.view(ctx.shapes[1]), dgq, dgk, None, None, None
+        sq, sk = ctx.shapes
+        return None, dq if len(sq) == 3 else dq.view(sq), dk if len(sk) == 3 else dk.view(sk), dgq, dgk, None, None, None
 
 
 class _CausalAttention(torch.autograd.Function):
@@ -1288,13 +1294,15 @@ class _CausalAttention(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, ops, q, k, v, batch, kv, causal_mask, scale, head_dim):
-        q3, k3, v3 = (causal.readable(causal.heads_view(t, n, head_dim)) for t, n in ((q, 'q'), (k, 'k'), (v, 'v')))
+        q3, k3, v3 = causal.heads_view(q, 'q', head_dim), causal.heads_view(k, 'k', head_dim), causal.heads_view(v, 'v', head_dim)
+        flat = q3 is not q
+        q3, k3, v3 = causal.readable(q3), causal.readable(k3), causal.readable(v3)
         with causal.on_device(q3):
-            out, lse = causal.attention_forward(ops.lib, ops.h, ops.stream(), q3, k3, v3, batch, kv, causal_mask, scale, True)
+            out, lse = causal.attention_forward(ops.lib, ops.h, _stream_for(ops, q3), q3, k3, v3, batch, kv, causal_mask, scale, True)
         ctx.ops, ctx.batch, ctx.kv, ctx.causal_mask, ctx.scale = ops, batch, kv, causal_mask, scale
         ctx.shapes = q.shape, k.shape, v.shape
         ctx.save_for_backward(q3, k3, v3, out, lse)
-        return out.view(q.shape)
+        return out.view(q.shape) if flat else out
 
     @staticmethod
     @once_differentiable
@@ -1302,9 +1310,10 @@ class _CausalAttention(torch.autograd.Function):
         ops: TrainOps = ctx.ops
         q, k, v, out, lse = ctx.saved_tensors
         with causal.on_device(q):
-            dq, dk, dv = causal.attention_backward(ops.lib, ops.h, ops.stream(), q, k, v, ctx.batch, ctx.kv, ctx.causal_mask, ctx.scale, out, lse,
-                                                   dout.reshape(q.shape))
-        return (None, dq.view(ctx.shapes[0]), dk.view(ctx.shapes[1]), dv.view(ctx.shapes[2])) + (None,) * 5
+            grads = causal.attention_backward(ops.lib, ops.h, _stream_for(ops, q), q, k, v, ctx.batch, ctx.kv, ctx.causal_mask, ctx.scale, out.view(q.shape), lse,
+                                              dout if dout.dim() == 3 else dout.reshape(q.shape))
+        dq, dk, dv = (g if len(s) == 3 else g.view(s) for g, s in zip(grads, ctx.shapes))
+        return None, dq, dk, dv, None, None, None, None, None
 
 
 class _Bce(torch.autograd.Function):

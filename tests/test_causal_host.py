@@ -53,7 +53,7 @@ def test_norm_rope_refuses(kw, msg):
 
 def test_step_refuses():
     def call(q=(2, 4, 64), k=(2, 9, 2, 64), v=None, n=torch.zeros(2, dtype=torch.int32), m=None, t=torch.float32):
-        return causal.attention_step(None, None, None, CUDA, torch.zeros(q), torch.zeros(k, dtype=t), torch.zeros(v or k, dtype=t), n, m, None)
+        return causal.check_step(CUDA, torch.zeros(q), torch.zeros(k, dtype=t), torch.zeros(v or k, dtype=t), n, m)
     for kw, msg in [(dict(k=(3, 9, 2, 64)), 'k_cache'), (dict(v=(2, 8, 2, 64)), 'v_cache'), (dict(k=(2, 9, 3, 64)), 'multiple of 3'),
                     (dict(n=torch.zeros(2, dtype=torch.int64)), 'int32'), (dict(n=torch.zeros(3, dtype=torch.int32)), 'lengths'),
                     (dict(m=10), 'max_length'), (dict(m=-1), 'max_length'), (dict(k=(2, 9, 2, 128)), 'k_cache'), (dict(), 'on cpu')]:
