@@ -1,30 +1,34 @@
 // Attention of ONE new frame per stream over its cache: out[b, h] = sum_j softmax_j(scale q_bh . k_j) v_j over the first lengths[b] rows of the cache of kv
 // head h / group.  Bound by reading the live rows of K and V once, so the keys are cut into chunks that fill the machine whatever the batch is:
-//   step_kernel     block = (stream, kv head, chunk).  A wave takes every NW-th 32 keys of the chunk through its own double-buffered LDS tiles (DMA, no
-//                   barrier in the loop); the heads of a group are the columns of its products, so a key is read once for all of them.  Running maximum
-//                   and sum per wave, the waves of a block joined through LDS; one chunk in all: the output, otherwise a partial (O, m, l).
+//   step_kernel     block = (stream, kv head, chunk).  A wave takes every 4th 32 keys of the chunk, K straight into registers (a key is a row of the A
+//                   operand), V through its own double-buffered LDS tile (DMA, no barrier in the loop), the next tile always in flight.  The heads of a
+//                   group are the columns of its products, so a key is read once for all of them.  Running maximum and sum per wave, the waves of a
+//                   block joined through LDS; one chunk in all: the output, otherwise a partial (O, m, l).
 //   join_kernel     joins a stream's chunks in chunk order (the result does not depend on which block finished first).
 #include "causal_core.h"
 
 namespace {
 using namespace causal;
 
+constexpr int NW = 4;                            // waves of a block
+constexpr float kSlack = 8.f;                    // the running maximum moves when a score passes it by 2^8 (causal_fwd.hip)
 template <typename T, int D> struct StepShape {
-    static constexpr int NW = (sizeof(T) == 4 && D == 128) ? 2 : 4;       // waves
     static constexpr int TILE_B = 32 * D * (int)sizeof(T);
-    static constexpr int WAVE_B = 4 * TILE_B;                              // two stages of K | V
-    static constexpr int LDS_B = NW * WAVE_B;                              // >= NW * 32 * (D + 2) * 4, what the join inside a block needs
-    static_assert(LDS_B >= NW * 32 * (D + 2) * 4, "join space");
+    static constexpr int WAVE_B = 2 * TILE_B;                              // two V tiles
+    static constexpr int JOIN_B = NW * 32 * (D + 2) * 4;                   // what the join inside a block needs
+    static constexpr int LDS_B = NW * WAVE_B > JOIN_B ? NW * WAVE_B : JOIN_B;
 };
 
 template <typename T, int D>
-__global__ __launch_bounds__((StepShape<T, D>::NW * 64)) void step_kernel(StepArgs a) {
-    constexpr int NW = StepShape<T, D>::NW, TILE_B = StepShape<T, D>::TILE_B, KS = D / 16, DB = D / 32;
+__global__ __launch_bounds__(NW * 64, (sizeof(T) == 4 && D == 128 ? 1 : 2)) void step_kernel(StepArgs a) {
+    constexpr int TILE_B = StepShape<T, D>::TILE_B, KS = D / 16, DB = D / 32;
     typedef Tile<T, D> TL;
     typedef typename Frag<T>::type frag;
     extern __shared__ __attribute__((aligned(16))) char lds[];
     const int hgs = (a.group + 31) / 32;                                   // blocks of 32 heads of a group
-    const int chunk = blockIdx.x, kvh = blockIdx.y / hgs, hg = blockIdx.y % hgs, b = blockIdx.z;
+    // chunk outermost: workgroups go round the 8 XCDs in order, and whether a stream still has its n-th chunk depends on n
+    const int per = a.kv_heads * hgs, unit = blockIdx.x % per, rest = blockIdx.x / per;
+    const int kvh = unit / hgs, hg = unit % hgs, b = rest % a.B, chunk = rest / a.B;
     const int len = min(max(a.lengths[b], 0), a.capacity);
     const int lo = chunk * a.chunk, hi_key = min(len, lo + a.chunk);
     if (chunk > 0 && lo >= len) return;                                    // (chunk 0 of an empty stream writes its zeros)
@@ -39,41 +43,38 @@ __global__ __launch_bounds__((StepShape<T, D>::NW * 64)) void step_kernel(StepAr
     const int64_t kbytes = a.k.row * (int64_t)sizeof(T), vbytes = a.v.row * (int64_t)sizeof(T);
     const char* kbase = reinterpret_cast<const char*>(static_cast<const T*>(a.k.p) + (int64_t)b * a.k_batch + (int64_t)kvh * a.k.head);
     const char* vbase = reinterpret_cast<const char*>(static_cast<const T*>(a.v.p) + (int64_t)b * a.v_batch + (int64_t)kvh * a.v.head);
-    Copier<T, D, 32, 64> ck, cv;
-    ck.init(kbytes, lane);
+    Copier<T, D, 32, 64> cv;
     cv.init(vbytes, lane);
     char* own = lds + wave * StepShape<T, D>::WAVE_B;
     const int ntiles = (max(0, hi_key - lo) + 31) / 32;
-    auto fetch = [&](int t, int stage) {
-        char* st = own + stage * 2 * TILE_B;
+    frag kfr[KS], knext[KS];
+    auto fetch = [&](int t, int stage) {                                   // (rows past the chunk: copies of its last one)
         const int key0 = lo + t * 32;
-        ck.run(st, kbase + (int64_t)key0 * kbytes, hi_key - key0, lane);
-        cv.run(st + TILE_B, vbase + (int64_t)key0 * vbytes, hi_key - key0, lane);
+        const T* krow = reinterpret_cast<const T*>(kbase + (int64_t)min(key0 + l31, hi_key - 1) * kbytes) + 8 * hi;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) knext[ks] = load8<T>(krow + 16 * ks);
+        cv.run(own + stage * TILE_B, vbase + (int64_t)key0 * vbytes, hi_key - key0, lane);
     };
-    constexpr int PER_TILE = 2 * Copier<T, D, 32, 64>::PASSES;
 
     f32x16 o[DB];
 #pragma unroll
     for (int d = 0; d < DB; ++d) o[d] = zero16();
     float m = -INFINITY, l = 0.f;
-    const float c2 = a.scale * 1.4426950408889634f;
+    const float c2 = a.scale * 1.4426950408889634f, slack = kSlack / c2;
 
     if (wave < ntiles) fetch(wave, 0);
     int stage = 0;
     for (int t = wave; t < ntiles; t += NW, stage ^= 1) {
-        // the tile being read next was last touched one iteration ago, by this wave alone: its reads must have returned before the copy starts
+        // tile t has landed; the other V tile was read an iteration ago, by this wave alone, and those reads have returned
+        wait_vm<0>();
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        if (t + NW < ntiles) {
-            fetch(t + NW, stage ^ 1);
-            wait_vm<PER_TILE>();
-        } else {
-            wait_vm<0>();
-        }
-        const char* kt = own + stage * 2 * TILE_B;
-        const char* vt = kt + TILE_B;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) kfr[ks] = knext[ks];
+        if (t + NW < ntiles) fetch(t + NW, stage ^ 1);
+        const char* vt = own + stage * TILE_B;
         f32x16 s = zero16();
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) s = mma<T>(TL::row_frag(kt, l31, ks, hi), qfr[ks], s);
+        for (int ks = 0; ks < KS; ++ks) s = mma<T>(kfr[ks], qfr[ks], s);
         const int key0 = lo + t * 32;
         if (key0 + 32 > hi_key) {
 #pragma unroll
@@ -83,8 +84,8 @@ __global__ __launch_bounds__((StepShape<T, D>::NW * 64)) void step_kernel(StepAr
 #pragma unroll
         for (int r = 1; r < 16; ++r) mx = fmaxf(mx, s[r]);
         mx = halves_max(mx);
-        if (__any(mx > m)) {
-            const float mn = fmaxf(m, mx);
+        if (__any(mx > m + slack)) {
+            const float mn = mx > m + slack ? mx : m;
             const float f = m == -INFINITY ? 0.f : exp2_((m - mn) * c2);
             m = mn;
             l *= f;
@@ -174,7 +175,7 @@ template <typename T, int D> hipError_t run(const StepArgs& a, hipStream_t s) {
         once.mark();
     }
     const unsigned hgs = (unsigned)((a.group + 31) / 32);
-    hipLaunchKernelGGL((step_kernel<T, D>), dim3((unsigned)a.chunks, (unsigned)a.kv_heads * hgs, (unsigned)a.B), dim3(StepShape<T, D>::NW * 64), lds, s, a);
+    hipLaunchKernelGGL((step_kernel<T, D>), dim3((unsigned)a.chunks * (unsigned)a.kv_heads * hgs * (unsigned)a.B), dim3(NW * 64), lds, s, a);
     if (a.chunks > 1) hipLaunchKernelGGL((join_kernel<T, D>), dim3((unsigned)(a.kv_heads * a.group), (unsigned)a.B), dim3(D), 0, s, a);
     return hipGetLastError();
 }

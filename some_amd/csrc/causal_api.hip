@@ -235,6 +235,7 @@ int some_op_attention_step(SomeHandle* h, int32_t dtype, int32_t head_dim, const
     a.k_batch = k_batch; a.v_batch = v_batch; a.lengths = lengths_dev; a.B = B; a.capacity = max_length;
     a.kv_heads = kv_heads; a.group = heads / kv_heads; a.scale = scale;
     a.chunks = step_chunks(B, kv_heads, a.group, max_length, &a.chunk);
+    C_CHECK((int64_t)a.chunks * B * kv_heads * ((a.group + 31) / 32) < 0x7fffffffll && (int64_t)heads * B < 0x7fffffffll, "too many streams and heads for one launch");
     if (a.chunks > 1) {
         if (!workspace_dev || workspace_bytes < some_op_attention_step_bytes(h, B, heads, kv_heads, head_dim, max_length))
             return cfail(h, SOME_ENOMEM, __func__, "workspace too small (some_op_attention_step_bytes)");
