@@ -34,7 +34,7 @@ constexpr float kFitStart = 0x1p100f;
 template <typename T> constexpr float kProbLog2 = __is_same(T, f16_t) ? 10.f : 0.f;
 
 // ---- dQ (and D) ----------------------------------------------------------------------------------------------------------------------------
-constexpr int QB = 128;
+constexpr int QB = TR;
 template <typename T, int D> struct DqShape {
     static constexpr int KT = (sizeof(T) == 4 && D == 128) ? 32 : 64;
     static constexpr int TILE_B = KT * D * (int)sizeof(T);
@@ -42,7 +42,7 @@ template <typename T, int D> struct DqShape {
 };
 
 template <typename T, int D>
-__global__ __launch_bounds__(256, (D == 128 && sizeof(T) == 4 ? 1 : 2)) void causal_dq_kernel(CausalBwdArgs b, int nsub, int slots) {
+__global__ __launch_bounds__(256, (D == 128 && sizeof(T) == 4 ? 1 : 2)) void causal_dq_kernel(CausalBwdArgs b, int nsub, int positions) {
     constexpr int KT = DqShape<T, D>::KT, NB = KT / 32, KS = D / 16, DB = D / 32, TILE_B = DqShape<T, D>::TILE_B;
     constexpr bool F16 = __is_same(T, f16_t);
     typedef Tile<T, D> TL;
@@ -50,13 +50,11 @@ __global__ __launch_bounds__(256, (D == 128 && sizeof(T) == 4 ? 1 : 2)) void cau
     extern __shared__ __attribute__((aligned(16))) char lds[];
     const CausalArgs& a = b.f;
 
-    const Work w = find_work(a.kv_heads, nsub, a.group, slots);
-    if (w.slot < 0) return;
-    const Place pl = find_clip<QB>(a.q_offsets, a.B, w.slot);
-    const int qf = a.q_offsets[pl.b], Tq = a.q_offsets[pl.b + 1] - qf;
-    const int kf = a.k_offsets[pl.b], Tk = a.k_offsets[pl.b + 1] - kf;
-    const int q0 = pl.tile * QB;
-    if (q0 >= Tq) return;
+    const Work w = find_work(a.kv_heads, nsub, a.group);
+    if (w.pos >= positions) return;
+    const Clip clip = find_clip<false>(a.q_offsets, a.k_offsets, a.B, a.causal, w.pos);
+    if (clip.b < 0) return;
+    const int qf = clip.qf, Tq = clip.Tq, kf = clip.kf, Tk = clip.Tk, q0 = clip.tile * QB;
     const int shift = a.causal ? Tk - Tq : 0x3fffffff;
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -179,7 +177,7 @@ __global__ __launch_bounds__(256, (D == 128 && sizeof(T) == 4 ? 1 : 2)) void cau
 }
 
 // ---- dK, dV --------------------------------------------------------------------------------------------------------------------------------
-constexpr int KB = 128;                          // keys per workgroup
+constexpr int KB = TR;                           // keys per workgroup
 template <typename T, int D> struct DkvShape {
     static constexpr bool V_LDS = D == 128;                                // V fragments from LDS, not registers: lets two waves share a SIMD (f32: no spills)
     static constexpr int QT = sizeof(T) == 4 || V_LDS ? 32 : 64;           // queries per tile
@@ -189,7 +187,7 @@ template <typename T, int D> struct DkvShape {
 };
 
 template <typename T, int D>
-__global__ __launch_bounds__(256, (D == 128 && sizeof(T) == 4 ? 1 : 2)) void causal_dkv_kernel(CausalBwdArgs b, int nsub, int slots) {
+__global__ __launch_bounds__(256, (D == 128 && sizeof(T) == 4 ? 1 : 2)) void causal_dkv_kernel(CausalBwdArgs b, int nsub, int positions) {
     constexpr int QT = DkvShape<T, D>::QT, NB = QT / 32, KS = D / 16, DB = D / 32, TILE_B = DkvShape<T, D>::TILE_B, STAGE_B = DkvShape<T, D>::STAGE_B;
     constexpr bool F16 = __is_same(T, f16_t);
     typedef Tile<T, D> TL;
@@ -197,13 +195,11 @@ __global__ __launch_bounds__(256, (D == 128 && sizeof(T) == 4 ? 1 : 2)) void cau
     extern __shared__ __attribute__((aligned(16))) char lds[];
     const CausalArgs& a = b.f;
 
-    const Work w = find_work(a.kv_heads, nsub, b.parts, slots);
-    if (w.slot < 0) return;
-    const Place pl = find_clip<KB>(a.k_offsets, a.B, slots - 1 - w.slot);        // the first keys of a clip are seen by most queries: first slots first
-    const int qf = a.q_offsets[pl.b], Tq = a.q_offsets[pl.b + 1] - qf;
-    const int kf = a.k_offsets[pl.b], Tk = a.k_offsets[pl.b + 1] - kf;
-    const int k0 = pl.tile * KB;
-    if (k0 >= Tk) return;
+    const Work w = find_work(a.kv_heads, nsub, b.parts);
+    if (w.pos >= positions) return;
+    const Clip clip = find_clip<true>(a.q_offsets, a.k_offsets, a.B, a.causal, w.pos);
+    if (clip.b < 0) return;
+    const int qf = clip.qf, Tq = clip.Tq, kf = clip.kf, Tk = clip.Tk, k0 = clip.tile * KB;
     const int shift = a.causal ? Tk - Tq : 0x3fffffff;
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -409,13 +405,13 @@ template <typename T, int D> hipError_t run(const CausalBwdArgs& b, hipStream_t 
     }
     const int nsub = work_subs(a.kv_heads);
     if (a.q_rows > 0) {
-        const int slots = (int)(a.q_rows / QB) + a.B;
-        hipLaunchKernelGGL((causal_dq_kernel<T, D>), dim3((unsigned)work_blocks(a.kv_heads, a.group, slots)), dim3(256), (DqShape<T, D>::LDS_B), s, b, nsub, slots);
+        const int positions = (int)(a.q_rows / QB) + a.B;
+        hipLaunchKernelGGL((causal_dq_kernel<T, D>), dim3((unsigned)work_blocks(a.kv_heads, a.group, positions)), dim3(256), (DqShape<T, D>::LDS_B), s, b, nsub, positions);
     }
     if (b.k_rows > 0) {
-        const int slots = (int)(b.k_rows / KB) + a.B;
-        hipLaunchKernelGGL((causal_dkv_kernel<T, D>), dim3((unsigned)work_blocks(a.kv_heads, b.parts, slots)), dim3(256), (DkvShape<T, D>::LDS_B), s, b, nsub,
-                           slots);
+        const int positions = (int)(b.k_rows / KB) + a.B;
+        hipLaunchKernelGGL((causal_dkv_kernel<T, D>), dim3((unsigned)work_blocks(a.kv_heads, b.parts, positions)), dim3(256), (DkvShape<T, D>::LDS_B), s, b, nsub,
+                           positions);
         if (b.parts > 1)
             hipLaunchKernelGGL((causal_sum_kernel<T, D>), dim3((unsigned)((b.k_rows * a.kv_heads * (D / 4) + 255) / 256), 2), dim3(256), 0, s, b);
     }

@@ -120,7 +120,7 @@ template <typename T, int D> struct Tile {
 
     static __device__ __forceinline__ int swz(int r) {
         if constexpr (sizeof(T) == 4) return ((r & 4) << 1) | ((r & 3) << 1) | ((r >> 3) & 1);
-        else if constexpr (CHUNKS == 8) return r & 7;
+        else if constexpr (CHUNKS == 8) return ((r & 2) << 1) | ((r >> 1) & 2) | ((r >> 3) & 1);
         else return ((r & 3) << 2) | ((r >> 2) & 3);
     }
     // fragment of row `row` (any row = 32 n + l31): values 16 ks + 8 hi .. + 7
@@ -229,24 +229,88 @@ __device__ __forceinline__ void solo_column(float (&acc)[(D + 63) / 64], int r0,
 }
 
 // ---- block map ------------------------------------------------------------------------------------------------------------------------
-// Rows are packed: clip b owns rows [off[b], off[b + 1]).  Tiles of TR rows: clip b's first tile sits in slot off[b] / TR + b, so `rows / TR + B` slots
-// hold every clip's tiles without a table, and a block finds its clip by counting the clips that begin at or before its slot (64 per step).
-struct Place { int b, tile; };
-template <int TR> __device__ __forceinline__ Place find_clip(const int32_t* __restrict__ off, int B, int slot) {
+// Rows are packed: clip b owns rows [off[b], off[b + 1]) of the queries and of the keys.  A launch has a position for every tile of TR rows the clips can
+// have (`rows / TR + B` of them cover any lengths); a block finds its clip and tile from its position and the offsets alone, without a table.
+constexpr int TR = 128;
+struct Clip { int b, tile, qf, Tq, kf, Tk; };             // b < 0: no such tile
+
+// sum over the wave of the lanes up to this one (lane 63: of all)
+__device__ __forceinline__ int wave_scan(int x) {
+    x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);      // row_shr 1, 2, 4, 8: within 16 lanes
+    x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);      // row_bcast 15 into rows 1 and 3
+    x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);      // row_bcast 31 into rows 2 and 3
+    return x;
+}
+__device__ __forceinline__ int wave_total(int x) { return __builtin_amdgcn_readlane(wave_scan(x), 63); }
+
+// Up to 64 clips: positions run through the tiles of all clips by falling work - the keys a query tile sees, or (KEYS) the queries that see a key tile -
+// so the longest blocks start first whichever clip they belong to and the launch ends evenly.  A lane holds a clip; a clip's tiles in falling order of
+// work are its last query tile first (its first key tile first), `at_least(x)` of them with a work of x units of 128 or more; a bisection finds the
+// level position p falls into.  More clips: clip after clip (each is then a small part of the launch), found by counting the clips that begin before.
+template <bool KEYS> __device__ __forceinline__ Clip find_clip(const int32_t* __restrict__ q_off, const int32_t* __restrict__ k_off, int B, bool causal, int p) {
     const int lane = threadIdx.x & 63;
+    Clip c;
+    if (B <= 64) {
+        const int b0 = min(lane, B - 1);
+        const int qf = q_off[b0], Tq = q_off[b0 + 1] - qf, kf = k_off[b0], Tk = k_off[b0 + 1] - kf;
+        const int nq = (Tq + TR - 1) / TR, nk = (Tk + TR - 1) / TR;
+        const int n = lane < B ? (KEYS ? nk : nq) : 0;
+        const int past = max(0, nk - nq);                                // key tiles every query tile sees (and query levels below nought are all alike)
+        const int top = KEYS ? nq : nk;
+        const auto at_least = [&](int x) {
+            if (!causal) return top >= x ? n : 0;
+            return top >= x ? min(n, top - x + 1 + (KEYS ? past : 0)) : 0;
+        };
+        if (p >= wave_total(n)) return {-1, 0, 0, 0, 0, 0};
+        int lo = -(1 << 22), hi = 1 << 22;                               // at_least(lo) counts everything, at_least(hi) nothing
+        {
+            int mx = lane < B ? top : 0;                                 // tighten: levels lie in (top - n, top]
+            int mn = lane < B ? top - n - 1 : 0;
+#pragma unroll
+            for (int o = 1; o < 64; o *= 2) {
+                mx = max(mx, __shfl_xor(mx, o, 64));
+                mn = min(mn, __shfl_xor(mn, o, 64));
+            }
+            hi = __builtin_amdgcn_readfirstlane(mx) + 1;
+            lo = __builtin_amdgcn_readfirstlane(mn);
+        }
+        while (hi - lo > 1) {                                            // the largest level with more than p tiles at or above it
+            const int mid = (lo + hi) >> 1;
+            if (wave_total(at_least(mid)) > p) lo = mid;
+            else hi = mid;
+        }
+        const int above = at_least(lo + 1), here = at_least(lo) - above, upto = wave_scan(here);
+        const int r = p - wave_total(above);                             // the r-th tile of this level
+        const int b = __ffsll((unsigned long long)__ballot(upto > r)) - 1;
+        const int k = __builtin_amdgcn_readlane(above, b) + r - (__builtin_amdgcn_readlane(upto, b) - __builtin_amdgcn_readlane(here, b));
+        c.b = b;
+        c.tile = KEYS ? k : __builtin_amdgcn_readlane(nq, b) - 1 - k;
+        c.qf = __builtin_amdgcn_readlane(qf, b);
+        c.Tq = __builtin_amdgcn_readlane(Tq, b);
+        c.kf = __builtin_amdgcn_readlane(kf, b);
+        c.Tk = __builtin_amdgcn_readlane(Tk, b);
+        return c;
+    }
+    const int32_t* off = KEYS ? k_off : q_off;
     int n = 0;
     for (int base = 0; base < B; base += 64) {
         const int b = base + lane;
-        const bool below = b < B && off[b] / TR + b <= slot;
-        const int c = __popcll(__ballot(below));
-        n += c;
-        if (c < 64) break;
+        const int m = __popcll(__ballot(b < B && off[b] / TR + b <= p));
+        n += m;
+        if (m < 64) break;
     }
-    const int b = n > 0 ? n - 1 : 0;
-    return {__builtin_amdgcn_readfirstlane(b), __builtin_amdgcn_readfirstlane(slot - (off[b] / TR + b))};
+    c.b = __builtin_amdgcn_readfirstlane(n > 0 ? n - 1 : 0);
+    c.qf = q_off[c.b]; c.Tq = q_off[c.b + 1] - c.qf;
+    c.kf = k_off[c.b]; c.Tk = k_off[c.b + 1] - c.kf;
+    c.tile = __builtin_amdgcn_readfirstlane(p - (off[c.b] / TR + c.b));
+    if (c.tile * TR >= (KEYS ? c.Tk : c.Tq)) c.b = -1;
+    return c;
 }
 // the clip of a packed row (off[0] <= row < off[B])
-__device__ __forceinline__ Place find_row(const int32_t* __restrict__ off, int B, int row) {
+__device__ __forceinline__ int find_row(const int32_t* __restrict__ off, int B, int row) {
     const int lane = threadIdx.x & 63;
     int n = 0;
     for (int base = 0; base < B; base += 64) {
@@ -255,24 +319,22 @@ __device__ __forceinline__ Place find_row(const int32_t* __restrict__ off, int B
         n += c;
         if (c < 64) break;
     }
-    const int b = __builtin_amdgcn_readfirstlane(n - 1);
-    return {b, row - off[b]};
+    return __builtin_amdgcn_readfirstlane(n - 1);
 }
-// blockIdx -> (kv head, slot, head of the group): the blocks of one kv head run on as few of the 8 XCDs as balance allows (they read the same K
-// and V through that XCD's L2), neighbouring slots at the same time, the last slot of the packed rows first (a clip's last tile sees most keys).
-struct Work { int kvh, slot, g; };
+// blockIdx -> (kv head, position, head of the group and part): the blocks of one kv head run on as few of the 8 XCDs as balance allows (they read the same
+// K and V through that XCD's L2), neighbouring positions at the same time.
+struct Work { int kvh, pos, g; };
 inline int work_subs(int kv_heads) { return (kv_heads & 1) ? 8 : (kv_heads & 2) ? 4 : (kv_heads & 4) ? 2 : 1; }
-inline int64_t work_blocks(int kv_heads, int per_slot, int slots) {
+inline int64_t work_blocks(int kv_heads, int per_pos, int positions) {
     const int nsub = work_subs(kv_heads);
-    return 8ll * (kv_heads * nsub / 8) * per_slot * ((slots + nsub - 1) / nsub);
+    return 8ll * (kv_heads * nsub / 8) * per_pos * ((positions + nsub - 1) / nsub);
 }
-__device__ __forceinline__ Work find_work(int kv_heads, int nsub, int per_slot, int slots) {
+__device__ __forceinline__ Work find_work(int kv_heads, int nsub, int per_pos) {
     const int xcd = blockIdx.x & 7, j = blockIdx.x >> 3;
     const int upx = kv_heads * nsub / 8;
-    const int g = j % per_slot, t = j / per_slot;
+    const int g = j % per_pos, t = j / per_pos;
     const int u = (t % upx) * 8 + xcd;
-    const int s = (t / upx) * nsub + u % nsub;
-    return {u / nsub, slots - 1 - s, g};
+    return {u / nsub, (t / upx) * nsub + u % nsub, g};
 }
 
 }  // namespace causal

@@ -20,6 +20,7 @@ template <typename T, int D, int QN> struct Shape {
     static constexpr int STAGES = 2;
     static constexpr int LDS_B = STAGES * 2 * TILE_B;
     static constexpr int QB = 128 * QN;                                    // queries per workgroup
+    static_assert(QB == TR, "one position, one workgroup");
 };
 
 // one query, all its visible keys in [j0, j1) (causal_core.h, "not-a-number and infinities"): unnormalised sums, maximum and sum
@@ -47,20 +48,18 @@ __device__ __forceinline__ void solo_query(const CausalArgs& a, const T* q, cons
 }
 
 template <typename T, int D, int QN>
-__global__ __launch_bounds__(256, 2) void causal_fwd_kernel(CausalArgs a, int nsub, int slots) {
+__global__ __launch_bounds__(256, 2) void causal_fwd_kernel(CausalArgs a, int nsub, int positions) {
     typedef Shape<T, D, QN> SH;
     constexpr int KT = SH::KT, NB = KT / 32, KS = D / 16, DB = D / 32, TILE_B = SH::TILE_B, STAGES = SH::STAGES, QB = SH::QB;
     typedef Tile<T, D> TL;
     typedef typename Frag<T>::type frag;
     extern __shared__ __attribute__((aligned(16))) char lds[];
 
-    const Work w = find_work(a.kv_heads, nsub, a.group * a.parts, slots);
-    if (w.slot < 0) return;
-    const Place pl = find_clip<QB>(a.q_offsets, a.B, w.slot);
-    const int qf = a.q_offsets[pl.b], Tq = a.q_offsets[pl.b + 1] - qf;
-    const int kf = a.k_offsets[pl.b], Tk = a.k_offsets[pl.b + 1] - kf;
-    const int q0 = pl.tile * QB;
-    if (q0 >= Tq) return;
+    const Work w = find_work(a.kv_heads, nsub, a.group * a.parts);
+    if (w.pos >= positions) return;
+    const Clip clip = find_clip<false>(a.q_offsets, a.k_offsets, a.B, a.causal, w.pos);
+    if (clip.b < 0) return;
+    const int qf = clip.qf, Tq = clip.Tq, kf = clip.kf, Tk = clip.Tk, q0 = clip.tile * QB;
     const int shift = a.causal ? Tk - Tq : 0x3fffffff;       // query i sees keys j <= i + shift
     const int head = w.kvh * a.group + w.g % a.group, part = w.g / a.group;
 
@@ -238,8 +237,8 @@ template <typename T, int D> __global__ __launch_bounds__(256) void causal_join_
     const int heads = a.kv_heads * a.group;
     const int64_t row = blockIdx.x;
     if (row < a.q_offsets[0] || row >= a.q_offsets[a.B]) return;
-    const Place pl = find_row(a.q_offsets, a.B, (int)row);
-    const int i = (int)row - a.q_offsets[pl.b], Tq = a.q_offsets[pl.b + 1] - a.q_offsets[pl.b], Tk = a.k_offsets[pl.b + 1] - a.k_offsets[pl.b];
+    const int b = find_row(a.q_offsets, a.B, (int)row);
+    const int i = (int)row - a.q_offsets[b], Tq = a.q_offsets[b + 1] - a.q_offsets[b], Tk = a.k_offsets[b + 1] - a.k_offsets[b];
     const bool any = Tk > 0 && (!a.causal || i + Tk - Tq >= 0);
     const int64_t step = a.q_rows * heads;
     for (int c = threadIdx.x; c < heads * (D / 4); c += 256) {
@@ -271,9 +270,9 @@ template <typename T, int D, int QN> hipError_t run(const CausalArgs& a, hipStre
         if (e != hipSuccess) return e;
         once.mark();
     }
-    const int slots = (int)(a.q_rows / SH::QB) + a.B;
-    hipLaunchKernelGGL((causal_fwd_kernel<T, D, QN>), dim3((unsigned)work_blocks(a.kv_heads, a.group * a.parts, slots)), dim3(256), SH::LDS_B, s, a,
-                       work_subs(a.kv_heads), slots);
+    const int positions = (int)(a.q_rows / TR) + a.B;
+    hipLaunchKernelGGL((causal_fwd_kernel<T, D, QN>), dim3((unsigned)work_blocks(a.kv_heads, a.group * a.parts, positions)), dim3(256), SH::LDS_B, s, a,
+                       work_subs(a.kv_heads), positions);
     if (a.parts > 1) hipLaunchKernelGGL((causal_join_kernel<T, D>), dim3((unsigned)a.q_rows), dim3(256), 0, s, a);
     return hipGetLastError();
 }
@@ -282,7 +281,7 @@ template <typename T, int D> hipError_t pick(const CausalArgs& a, hipStream_t s)
 
 }  // namespace
 
-int64_t causal_fwd_blocks(const CausalArgs& a) { return causal::work_blocks(a.kv_heads, a.group * a.parts, (int)(a.q_rows / 128) + a.B); }
+int64_t causal_fwd_blocks(const CausalArgs& a) { return causal::work_blocks(a.kv_heads, a.group * a.parts, (int)(a.q_rows / causal::TR) + a.B); }
 
 // Parts the keys are cut into: 1 unless the queries alone give too few workgroups (below 3 per CU) AND the keys are long (256 of them per part at
 // least).  Lengths are on the device, so the averages over the batch decide.

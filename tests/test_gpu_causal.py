@@ -132,6 +132,24 @@ def test_attention(ops, eng, dtype, H, G, D, ql, kl, causal):
     assert all(torch.equal(a, b) for a, b in zip(grads, again))
 
 
+@pytest.mark.parametrize('B', [2, 63, 64, 65, 150])
+@pytest.mark.parametrize('past', [False, True])
+def test_attention_of_many_clips(ops, B, past):
+    """Every tile of every clip is worked on once, whatever the number of clips and their lengths."""
+    rng = np.random.default_rng(B)
+    ql = [int(n) for n in rng.choice([0, 1, 5, 127, 128, 129, 200, 260], B)]
+    kl = [n + int(rng.choice([0, 3, 128, 140])) for n in ql] if past else ql
+    H, G, D = 3, 1, 64
+    q, k, v = _qkv(37, sum(ql), sum(kl), H, G, D, torch.bfloat16)
+    dout = _normal(39, sum(ql), H, D, dtype=torch.bfloat16)
+    leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+    out = ops.causal_attention(*leaves, _batch(ql), kv_batch=_batch(kl))
+    grads = torch.autograd.grad(out, leaves, dout)
+    w = oracle.attention(q, k, v, ql, kl, dout=dout)
+    for i, (name, got) in enumerate(zip(('out', 'dq', 'dk', 'dv'), (out.detach(), *grads))):
+        oracle.check(got, w[2 * i], w[2 * i + 1], name)
+
+
 @pytest.mark.parametrize('dtype', TYPES)
 def test_attention_of_slices_and_scale(ops, eng, dtype):
     lens, H, G, D = [70, 1, 150], 4, 2, 64
