@@ -123,7 +123,7 @@ int some_train_qk_norm_rope_bwd(SomeHandle* h, int32_t dtype, int32_t head_dim, 
 size_t some_op_causal_attention_bytes(const SomeHandle* h, int32_t heads, int32_t kv_heads, int32_t head_dim, int32_t B, int64_t q_rows, int64_t k_rows) {
     (void)h;
     if (!heads_ok(heads, kv_heads) || head_dim <= 0 || B <= 0 || q_rows <= 0 || k_rows <= 0 || q_rows >= kMaxRows || k_rows >= kMaxRows) return 0;
-    const int parts = causal_fwd_parts(q_rows, k_rows, B, heads);
+    const int parts = causal_fwd_parts(q_rows, k_rows, B, heads, kv_heads);
     return parts > 1 ? (size_t)parts * q_rows * heads * (head_dim + 2) * sizeof(float) : 0;
 }
 
@@ -151,7 +151,7 @@ int some_op_causal_attention(SomeHandle* h, int32_t dtype, int32_t head_dim, con
     C_CHECK(laid_out(dtype, a.q) && laid_out(dtype, a.k) && laid_out(dtype, a.v) && laid_out(dtype, a.out), kLayout);
     a.lse = lse_dev; a.q_offsets = q_offsets_dev; a.k_offsets = k_offsets_dev; a.q_rows = q_rows;
     a.B = B; a.kv_heads = kv_heads; a.group = heads / kv_heads; a.causal = causal; a.scale = scale;
-    a.parts = k_rows > 0 ? causal_fwd_parts(q_rows, k_rows, B, heads) : 1;
+    a.parts = k_rows > 0 ? causal_fwd_parts(q_rows, k_rows, B, heads, kv_heads) : 1;
     if (a.parts > 1) {
         if (!workspace_dev || workspace_bytes < some_op_causal_attention_bytes(h, heads, kv_heads, head_dim, B, q_rows, k_rows))
             return cfail(h, SOME_ENOMEM, __func__, "workspace too small (some_op_causal_attention_bytes)");
@@ -159,7 +159,7 @@ int some_op_causal_attention(SomeHandle* h, int32_t dtype, int32_t head_dim, con
         a.part_o = static_cast<float*>(workspace_dev);
         a.part_ml = a.part_o + (int64_t)a.parts * q_rows * heads * head_dim;
     }
-    C_CHECK(causal_fwd_blocks(a) < 0x7fffffffll, "too many rows, clips and heads for one launch");
+    C_CHECK(q_rows * a.group < 0x7fffffffll && causal_fwd_blocks(a) < 0x7fffffffll, "too many rows, clips and heads for one launch");
     C_TRY(launch_causal_fwd(dtype, head_dim, a, static_cast<hipStream_t>(stream)));
     return SOME_OK;
 }
@@ -196,7 +196,7 @@ int some_train_causal_attention_bwd(SomeHandle* h, int32_t dtype, int32_t head_d
     b.dsum = static_cast<float*>(workspace_dev);
     b.part_k = reinterpret_cast<float*>(static_cast<char*>(workspace_dev) + dsum_bytes(heads, q_rows));
     b.part_v = b.part_k + (int64_t)b.parts * k_rows * kv_heads * head_dim;
-    C_CHECK(causal_fwd_blocks(a) < 0x7fffffffll && causal_bwd_blocks(b) < 0x7fffffffll && k_rows * kv_heads * (head_dim / 4) / 256 < 0x7ffffff0ll, "too many rows, clips and heads for one launch");
+    C_CHECK(q_rows * a.group < 0x7fffffffll && causal_fwd_blocks(a) < 0x7fffffffll && causal_bwd_blocks(b) < 0x7fffffffll && k_rows * kv_heads * (head_dim / 4) / 256 < 0x7ffffff0ll, "too many rows, clips and heads for one launch");
     C_TRY(launch_causal_bwd(dtype, head_dim, b, static_cast<hipStream_t>(stream)));
     return SOME_OK;
 }

@@ -50,18 +50,20 @@ __global__ __launch_bounds__(256, (D == 128 && sizeof(T) == 4 ? 1 : 2)) void cau
     extern __shared__ __attribute__((aligned(16))) char lds[];
     const CausalArgs& a = b.f;
 
-    const Work w = find_work(a.kv_heads, nsub, a.group);
+    const Work w = find_work(a.kv_heads, nsub, 1);
     if (w.pos >= positions) return;
-    const Clip clip = find_clip<false>(a.q_offsets, a.k_offsets, a.B, a.causal, w.pos);
+    const Clip clip = find_clip<false>(a.q_offsets, a.k_offsets, a.B, a.causal, a.group, w.pos);
     if (clip.b < 0) return;
     const int qf = clip.qf, Tq = clip.Tq, kf = clip.kf, Tk = clip.Tk, q0 = clip.tile * QB;
     const int shift = a.causal ? Tk - Tq : 0x3fffffff;
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int l31 = lane & 31, hi = lane >> 5;
-    const int head = w.kvh * a.group + w.g;
-    const int qw = q0 + wave * 32, q = qw + l31;
-    const int64_t qr = qf + min(q, Tq - 1);
+    const int G = a.group, N = Tq * G, qw = q0 + wave * 32;  // queries: frame n / G, head n % G
+    const unsigned n_lane = (unsigned)min(qw + l31, N - 1);
+    const int q = (int)(n_lane / (unsigned)G), head = w.kvh * G + (int)(n_lane % (unsigned)G);
+    const bool mine = qw + l31 < N;
+    const int64_t qr = qf + q;
     const T* qrow = static_cast<const T*>(a.q.p) + qr * a.q.row + (int64_t)head * a.q.head + 8 * hi;
     const T* grow = static_cast<const T*>(b.dout.p) + qr * b.dout.row + (int64_t)head * b.dout.head + 8 * hi;
     const T* orow = static_cast<const T*>(a.out.p) + qr * a.out.row + (int64_t)head * a.out.head + 8 * hi;
@@ -80,14 +82,14 @@ __global__ __launch_bounds__(256, (D == 128 && sizeof(T) == 4 ? 1 : 2)) void cau
     }
     dsum = halves_sum(dsum);
     const float lse = a.lse[(int64_t)head * a.q_rows + qr];
-    if (q < Tq && hi == 0) b.dsum[(int64_t)head * a.q_rows + qf + q] = dsum;
+    if (mine && hi == 0) b.dsum[(int64_t)head * a.q_rows + qr] = dsum;
 
-    const int last_q = min(q0 + QB, Tq) - 1;
+    const int last_q = (int)((unsigned)(min(q0 + QB, N) - 1) / (unsigned)G);
     const int nkeys = min(Tk, max(0, last_q + shift + 1));
     const int ntiles = (nkeys + KT - 1) / KT;
-    const int seen_w = min(Tk, max(0, min(qw + 31, Tq - 1) + shift + 1));
+    const int seen_w = min(Tk, max(0, (int)((unsigned)min(qw + 31, N - 1) / (unsigned)G) + shift + 1));
     const int limit = min(q + shift, Tk - 1);
-    const int full_w = min(Tk, max(0, qw + shift + 1));
+    const int full_w = min(Tk, max(0, (int)((unsigned)qw / (unsigned)G) + shift + 1));
 
     const char* kbase = reinterpret_cast<const char*>(static_cast<const T*>(a.k.p) + (int64_t)kf * a.k.row + (int64_t)w.kvh * a.k.head);
     const char* vbase = reinterpret_cast<const char*>(static_cast<const T*>(a.v.p) + (int64_t)kf * a.v.row + (int64_t)w.kvh * a.v.head);
@@ -151,24 +153,25 @@ __global__ __launch_bounds__(256, (D == 128 && sizeof(T) == 4 ? 1 : 2)) void cau
     if (bad) {                                               // (wave-uniform; causal_core.h, "not-a-number and infinities")
         const T* kp = reinterpret_cast<const T*>(kbase);
         const T* vp = reinterpret_cast<const T*>(vbase);
-        for (int n = 0; n < 32 && qw + n < Tq; ++n) {
-            const int64_t row = qf + qw + n;
-            const T* qp = static_cast<const T*>(a.q.p) + row * a.q.row + (int64_t)head * a.q.head;
-            const T* gp = static_cast<const T*>(b.dout.p) + row * b.dout.row + (int64_t)head * b.dout.head;
+        for (int n = 0; n < 32 && qw + n < N; ++n) {
+            const int qn = (qw + n) / G, hd = w.kvh * G + (qw + n) % G;
+            const int64_t row = qf + qn;
+            const T* qp = static_cast<const T*>(a.q.p) + row * a.q.row + (int64_t)hd * a.q.head;
+            const T* gp = static_cast<const T*>(b.dout.p) + row * b.dout.row + (int64_t)hd * b.dout.head;
             const float lse_n = __shfl(lse, n, 64), dsum_n = __shfl(dsum, n, 64);
             float x[(D + 63) / 64] = {};
-            solo_column<T, D>(x, 0, min(qw + n + shift, Tk - 1) + 1, kp, a.k.row, [&](int j) {
+            solo_column<T, D>(x, 0, min(qn + shift, Tk - 1) + 1, kp, a.k.row, [&](int j) {
                 return exp2_(fmaf(dot_rows<T, D>(qp, kp + (int64_t)j * a.k.row), c2, -lse_n)) * (dot_rows<T, D>(gp, vp + (int64_t)j * a.v.row) - dsum_n);
             });
-            T* dst = static_cast<T*>(b.dq.p) + row * b.dq.row + (int64_t)head * b.dq.head;
+            T* dst = static_cast<T*>(b.dq.p) + row * b.dq.row + (int64_t)hd * b.dq.head;
 #pragma unroll
             for (int e = 0; e < (D + 63) / 64; ++e) dst[lane + 64 * e] = (T)(x[e] * a.scale);
         }
         return;
     }
-    if (q < Tq) {
+    if (mine) {
         const float f = a.scale / F;
-        T* dst = static_cast<T*>(b.dq.p) + (int64_t)(qf + q) * b.dq.row + (int64_t)head * b.dq.head + 4 * hi;
+        T* dst = static_cast<T*>(b.dq.p) + qr * b.dq.row + (int64_t)head * b.dq.head + 4 * hi;
 #pragma unroll
         for (int d = 0; d < DB; ++d)
 #pragma unroll
@@ -197,7 +200,7 @@ __global__ __launch_bounds__(256, (D == 128 && sizeof(T) == 4 ? 1 : 2)) void cau
 
     const Work w = find_work(a.kv_heads, nsub, b.parts);
     if (w.pos >= positions) return;
-    const Clip clip = find_clip<true>(a.q_offsets, a.k_offsets, a.B, a.causal, w.pos);
+    const Clip clip = find_clip<true>(a.q_offsets, a.k_offsets, a.B, a.causal, a.group, w.pos);
     if (clip.b < 0) return;
     const int qf = clip.qf, Tq = clip.Tq, kf = clip.kf, Tk = clip.Tk, k0 = clip.tile * KB;
     const int shift = a.causal ? Tk - Tq : 0x3fffffff;
@@ -405,8 +408,8 @@ template <typename T, int D> hipError_t run(const CausalBwdArgs& b, hipStream_t 
     }
     const int nsub = work_subs(a.kv_heads);
     if (a.q_rows > 0) {
-        const int positions = (int)(a.q_rows / QB) + a.B;
-        hipLaunchKernelGGL((causal_dq_kernel<T, D>), dim3((unsigned)work_blocks(a.kv_heads, a.group, positions)), dim3(256), (DqShape<T, D>::LDS_B), s, b, nsub, positions);
+        const int positions = (int)(a.q_rows * a.group / QB) + a.B;
+        hipLaunchKernelGGL((causal_dq_kernel<T, D>), dim3((unsigned)work_blocks(a.kv_heads, 1, positions)), dim3(256), (DqShape<T, D>::LDS_B), s, b, nsub, positions);
     }
     if (b.k_rows > 0) {
         const int positions = (int)(b.k_rows / KB) + a.B;

@@ -229,8 +229,9 @@ __device__ __forceinline__ void solo_column(float (&acc)[(D + 63) / 64], int r0,
 }
 
 // ---- block map ------------------------------------------------------------------------------------------------------------------------
-// Rows are packed: clip b owns rows [off[b], off[b + 1]) of the queries and of the keys.  A launch has a position for every tile of TR rows the clips can
-// have (`rows / TR + B` of them cover any lengths); a block finds its clip and tile from its position and the offsets alone, without a table.
+// Rows are packed: clip b owns rows [off[b], off[b + 1]) of the queries and of the keys.  The heads of a group share keys, so a query tile holds 128 / group
+// frames with all their heads: query n of a clip is frame n / group, head n % group.  A launch has a position for every tile of TR queries (keys) the clips
+// can have (`rows / TR + B` of them cover any lengths); a block finds its clip and tile from its position and the offsets alone, without a table.
 constexpr int TR = 128;
 struct Clip { int b, tile, qf, Tq, kf, Tk; };             // b < 0: no such tile
 
@@ -250,13 +251,16 @@ __device__ __forceinline__ int wave_total(int x) { return __builtin_amdgcn_readl
 // so the longest blocks start first whichever clip they belong to and the launch ends evenly.  A lane holds a clip; a clip's tiles in falling order of
 // work are its last query tile first (its first key tile first), `at_least(x)` of them with a work of x units of 128 or more; a bisection finds the
 // level position p falls into.  More clips: clip after clip (each is then a small part of the launch), found by counting the clips that begin before.
-template <bool KEYS> __device__ __forceinline__ Clip find_clip(const int32_t* __restrict__ q_off, const int32_t* __restrict__ k_off, int B, bool causal, int p) {
+// (Query tiles count in units of 128 / group keys, so that a clip's next tile sees one unit more.)
+template <bool KEYS>
+__device__ __forceinline__ Clip find_clip(const int32_t* __restrict__ q_off, const int32_t* __restrict__ k_off, int B, bool causal, int group, int p) {
     const int lane = threadIdx.x & 63;
     Clip c;
     if (B <= 64) {
         const int b0 = min(lane, B - 1);
         const int qf = q_off[b0], Tq = q_off[b0 + 1] - qf, kf = k_off[b0], Tk = k_off[b0 + 1] - kf;
-        const int nq = (Tq + TR - 1) / TR, nk = (Tk + TR - 1) / TR;
+        const int mul = KEYS ? 1 : group;
+        const int nq = (int)(((int64_t)Tq * mul + TR - 1) / TR), nk = (int)(((int64_t)Tk * mul + TR - 1) / TR);
         const int n = lane < B ? (KEYS ? nk : nq) : 0;
         const int past = max(0, nk - nq);                                // key tiles every query tile sees (and query levels below nought are all alike)
         const int top = KEYS ? nq : nk;
@@ -295,18 +299,19 @@ template <bool KEYS> __device__ __forceinline__ Clip find_clip(const int32_t* __
         return c;
     }
     const int32_t* off = KEYS ? k_off : q_off;
+    const int64_t mul = KEYS ? 1 : group;
     int n = 0;
     for (int base = 0; base < B; base += 64) {
         const int b = base + lane;
-        const int m = __popcll(__ballot(b < B && off[b] / TR + b <= p));
+        const int m = __popcll(__ballot(b < B && off[b] * mul / TR + b <= p));
         n += m;
         if (m < 64) break;
     }
     c.b = __builtin_amdgcn_readfirstlane(n > 0 ? n - 1 : 0);
     c.qf = q_off[c.b]; c.Tq = q_off[c.b + 1] - c.qf;
     c.kf = k_off[c.b]; c.Tk = k_off[c.b + 1] - c.kf;
-    c.tile = __builtin_amdgcn_readfirstlane(p - (off[c.b] / TR + c.b));
-    if (c.tile * TR >= (KEYS ? c.Tk : c.Tq)) c.b = -1;
+    c.tile = __builtin_amdgcn_readfirstlane(p - (int)(off[c.b] * mul / TR + c.b));
+    if ((int64_t)c.tile * TR >= (KEYS ? c.Tk : c.Tq) * mul) c.b = -1;
     return c;
 }
 // the clip of a packed row (off[0] <= row < off[B])

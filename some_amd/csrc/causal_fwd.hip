@@ -1,8 +1,8 @@
 // Causal attention over packed clips, forward: out[i] = sum_j softmax_j(scale q_i . k_j) v_j over the keys j <= i + Tk - Tq of the clip (rows aligned at
 // the end: the queries are the clip's last Tq frames), heads in groups that share keys and values.  A row that sees no key is 0 (log-sum -inf).
 //
-// One pass over the keys with a running maximum and sum (base 2, the scale folded into the exponent's multiplier).  A workgroup is 128 QN queries of one
-// head, a wave 32 QN of them; S^T = K Q^T puts a query in every lane's column, so its maximum and sum are the lane's own registers plus one exchange
+// One pass over the keys with a running maximum and sum (base 2, the scale folded into the exponent's multiplier).  A workgroup is 128 queries - 128 /
+// group frames with all heads of a group, which read every key tile together -, a wave 32 of them; S^T = K Q^T puts a query in every lane's column, so its maximum and sum are the lane's own registers plus one exchange
 // with the other half, and P^T is already the B operand of O^T += V^T P^T (causal_core.h): no probability touches LDS.  K and V tiles go global ->
 // LDS by DMA into a ring; V is read transposed by ds_read_b64_tr_b16.
 #include "causal_core.h"
@@ -55,31 +55,36 @@ __global__ __launch_bounds__(256, 2) void causal_fwd_kernel(CausalArgs a, int ns
     typedef typename Frag<T>::type frag;
     extern __shared__ __attribute__((aligned(16))) char lds[];
 
-    const Work w = find_work(a.kv_heads, nsub, a.group * a.parts);
+    const Work w = find_work(a.kv_heads, nsub, a.parts);
     if (w.pos >= positions) return;
-    const Clip clip = find_clip<false>(a.q_offsets, a.k_offsets, a.B, a.causal, w.pos);
+    const Clip clip = find_clip<false>(a.q_offsets, a.k_offsets, a.B, a.causal, a.group, w.pos);
     if (clip.b < 0) return;
     const int qf = clip.qf, Tq = clip.Tq, kf = clip.kf, Tk = clip.Tk, q0 = clip.tile * QB;
     const int shift = a.causal ? Tk - Tq : 0x3fffffff;       // query i sees keys j <= i + shift
-    const int head = w.kvh * a.group + w.g % a.group, part = w.g / a.group;
+    const int G = a.group, N = Tq * G, head0 = w.kvh * G, part = w.g;
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int l31 = lane & 31, hi = lane >> 5;
     const int qw = q0 + wave * 32 * QN;                      // the wave's first query; block n holds qw + 32 n ..
-    const T* qhead = static_cast<const T*>(a.q.p) + (int64_t)head * a.q.head;
+    int row[QN], head[QN];                                   // this lane's frames and heads
     frag qfr[QN][KS];
 #pragma unroll
-    for (int n = 0; n < QN; ++n)
+    for (int n = 0; n < QN; ++n) {
+        const unsigned i = (unsigned)min(qw + 32 * n + l31, N - 1);
+        row[n] = (int)(i / (unsigned)G);
+        head[n] = head0 + (int)(i % (unsigned)G);
+        const T* qrow = static_cast<const T*>(a.q.p) + (int64_t)(qf + row[n]) * a.q.row + (int64_t)head[n] * a.q.head + 8 * hi;
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) qfr[n][ks] = load8<T>(qhead + (int64_t)(qf + min(qw + 32 * n + l31, Tq - 1)) * a.q.row + 8 * hi + 16 * ks);
+        for (int ks = 0; ks < KS; ++ks) qfr[n][ks] = load8<T>(qrow + 16 * ks);
+    }
 
-    const int last_q = min(q0 + QB, Tq) - 1;
+    const int last_q = (int)((unsigned)(min(q0 + QB, N) - 1) / (unsigned)G);
     const int nkeys = min(Tk, max(0, last_q + shift + 1));   // keys anybody here sees
     const int ntiles = (nkeys + KT - 1) / KT;
     // this part's tiles
     const int t_begin = (int)((int64_t)ntiles * part / a.parts), t_end = (int)((int64_t)ntiles * (part + 1) / a.parts);
-    const int seen_w = min(Tk, max(0, min(qw + 32 * QN - 1, Tq - 1) + shift + 1));        // keys this wave sees
-    const int full_w = min(Tk, max(0, qw + shift + 1));      // keys every query of the wave sees
+    const int seen_w = min(Tk, max(0, (int)((unsigned)min(qw + 32 * QN - 1, N - 1) / (unsigned)G) + shift + 1));        // keys this wave sees
+    const int full_w = min(Tk, max(0, (int)((unsigned)qw / (unsigned)G) + shift + 1));      // keys every query of the wave sees
 
     const char* kbase = reinterpret_cast<const char*>(static_cast<const T*>(a.k.p) + (int64_t)kf * a.k.row + (int64_t)w.kvh * a.k.head);
     const char* vbase = reinterpret_cast<const char*>(static_cast<const T*>(a.v.p) + (int64_t)kf * a.v.row + (int64_t)w.kvh * a.v.head);
@@ -133,7 +138,7 @@ __global__ __launch_bounds__(256, 2) void causal_fwd_kernel(CausalArgs a, int ns
                 bad |= block_not_finite<T, D>(vt, nb * 32);
 #pragma unroll
                 for (int n = 0; n < QN; ++n) {
-                    const int limit = min(qw + 32 * n + l31 + shift, Tk - 1);
+                    const int limit = min(row[n] + shift, Tk - 1);
 #pragma unroll
                     for (int r = 0; r < 16; ++r) s[n][nb][r] = key0 + nb * 32 + crow(r, hi) <= limit ? s[n][nb][r] : -INFINITY;
                 }
@@ -184,34 +189,33 @@ __global__ __launch_bounds__(256, 2) void causal_fwd_kernel(CausalArgs a, int ns
 
     const int64_t prow = (int64_t)part * a.q_rows * a.kv_heads * a.group;
     if (bad) {                                               // (wave-uniform)
-        for (int n = 0; n < 32 * QN; ++n) {
-            const int q = qw + n, limit = min(q + shift, Tk - 1);
-            if (q >= Tq) break;
+        for (int n = 0; n < 32 * QN && qw + n < N; ++n) {
+            const int q = (qw + n) / G, hd = head0 + (qw + n) % G, limit = min(q + shift, Tk - 1);
             float mm, ll, o0, o1;
-            solo_query<T, D>(a, qhead + (int64_t)(qf + q) * a.q.row, reinterpret_cast<const T*>(kbase), reinterpret_cast<const T*>(vbase), t_begin * KT,
-                             min(t_end * KT, limit + 1), c2, &mm, &ll, &o0, &o1);
+            solo_query<T, D>(a, static_cast<const T*>(a.q.p) + (int64_t)(qf + q) * a.q.row + (int64_t)hd * a.q.head, reinterpret_cast<const T*>(kbase),
+                             reinterpret_cast<const T*>(vbase), t_begin * KT, min(t_end * KT, limit + 1), c2, &mm, &ll, &o0, &o1);
             if (a.parts > 1) {
-                const int64_t i = prow + (int64_t)(qf + q) * a.kv_heads * a.group + head;
+                const int64_t i = prow + (int64_t)(qf + q) * a.kv_heads * G + hd;
                 a.part_o[i * D + lane] = o0;
                 if (D > 64) a.part_o[i * D + 64 + lane] = o1;
                 if (lane == 0) *reinterpret_cast<f32x2*>(a.part_ml + 2 * i) = (f32x2){mm * c2, ll};
             } else {
                 const float inv = limit >= 0 ? 1.f / ll : 0.f;
-                T* orow = static_cast<T*>(a.out.p) + (int64_t)(qf + q) * a.out.row + (int64_t)head * a.out.head;
+                T* orow = static_cast<T*>(a.out.p) + (int64_t)(qf + q) * a.out.row + (int64_t)hd * a.out.head;
                 orow[lane] = (T)(o0 * inv);
                 if (D > 64) orow[64 + lane] = (T)(o1 * inv);
-                if (a.lse && lane == 0) a.lse[(int64_t)head * a.q_rows + qf + q] = limit >= 0 ? mm * c2 + log2_(ll) : -INFINITY;
+                if (a.lse && lane == 0) a.lse[(int64_t)hd * a.q_rows + qf + q] = limit >= 0 ? mm * c2 + log2_(ll) : -INFINITY;
             }
         }
         return;
     }
 #pragma unroll
     for (int n = 0; n < QN; ++n) {
-        const int q = qw + 32 * n + l31;
-        if (q >= Tq) continue;
+        if (qw + 32 * n + l31 >= N) continue;
+        const int q = row[n];
         const float sum = halves_sum(l[n]);
         if (a.parts > 1) {
-            const int64_t i = prow + (int64_t)(qf + q) * a.kv_heads * a.group + head;
+            const int64_t i = prow + (int64_t)(qf + q) * a.kv_heads * G + head[n];
 #pragma unroll
             for (int d = 0; d < DB; ++d)
 #pragma unroll
@@ -221,13 +225,13 @@ __global__ __launch_bounds__(256, 2) void causal_fwd_kernel(CausalArgs a, int ns
         } else {
             const bool any = q + shift >= 0 && Tk > 0;
             const float inv = any ? 1.f / sum : 0.f;         // no visible key: zero
-            T* orow = static_cast<T*>(a.out.p) + (int64_t)(qf + q) * a.out.row + (int64_t)head * a.out.head;
+            T* orow = static_cast<T*>(a.out.p) + (int64_t)(qf + q) * a.out.row + (int64_t)head[n] * a.out.head;
 #pragma unroll
             for (int d = 0; d < DB; ++d)
 #pragma unroll
                 for (int r4 = 0; r4 < 4; ++r4)
                     store4<T>(orow + 32 * d + 8 * r4 + 4 * hi, o[n][d][4 * r4] * inv, o[n][d][4 * r4 + 1] * inv, o[n][d][4 * r4 + 2] * inv, o[n][d][4 * r4 + 3] * inv);
-            if (a.lse && hi == 0) a.lse[(int64_t)head * a.q_rows + qf + q] = any ? m[n] * c2 + log2_(sum) : -INFINITY;
+            if (a.lse && hi == 0) a.lse[(int64_t)head[n] * a.q_rows + qf + q] = any ? m[n] * c2 + log2_(sum) : -INFINITY;
         }
     }
 }
@@ -270,8 +274,8 @@ template <typename T, int D, int QN> hipError_t run(const CausalArgs& a, hipStre
         if (e != hipSuccess) return e;
         once.mark();
     }
-    const int positions = (int)(a.q_rows / TR) + a.B;
-    hipLaunchKernelGGL((causal_fwd_kernel<T, D, QN>), dim3((unsigned)work_blocks(a.kv_heads, a.group * a.parts, positions)), dim3(256), SH::LDS_B, s, a,
+    const int positions = (int)(a.q_rows * a.group / TR) + a.B;
+    hipLaunchKernelGGL((causal_fwd_kernel<T, D, QN>), dim3((unsigned)work_blocks(a.kv_heads, a.parts, positions)), dim3(256), SH::LDS_B, s, a,
                        work_subs(a.kv_heads), positions);
     if (a.parts > 1) hipLaunchKernelGGL((causal_join_kernel<T, D>), dim3((unsigned)a.q_rows), dim3(256), 0, s, a);
     return hipGetLastError();
@@ -281,14 +285,14 @@ template <typename T, int D> hipError_t pick(const CausalArgs& a, hipStream_t s)
 
 }  // namespace
 
-int64_t causal_fwd_blocks(const CausalArgs& a) { return causal::work_blocks(a.kv_heads, a.group * a.parts, (int)(a.q_rows / causal::TR) + a.B); }
+int64_t causal_fwd_blocks(const CausalArgs& a) { return causal::work_blocks(a.kv_heads, a.parts, (int)(a.q_rows * a.group / causal::TR) + a.B); }
 
 // Parts the keys are cut into: 1 unless the queries alone give too few workgroups (below 3 per CU) AND the keys are long (256 of them per part at
 // least).  Lengths are on the device, so the averages over the batch decide.
-int causal_fwd_parts(int64_t q_rows, int64_t k_rows, int B, int heads) {
+int causal_fwd_parts(int64_t q_rows, int64_t k_rows, int B, int heads, int kv_heads) {
     if (B <= 0 || q_rows <= 0) return 1;
-    const int64_t groups = (q_rows + 127) / 128 > B ? (q_rows + 127) / 128 : B;
-    const int64_t want = 768 / (groups * heads), room = k_rows / B / 256;
+    const int64_t queries = q_rows * (heads / kv_heads), tiles = (queries + 127) / 128 > B ? (queries + 127) / 128 : B;
+    const int64_t want = 768 / (tiles * kv_heads), room = k_rows / B / 256;
     const int64_t p = want < room ? want : room;
     return p < 1 ? 1 : p > 32 ? 32 : (int)p;
 }
