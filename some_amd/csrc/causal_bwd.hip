@@ -1,6 +1,6 @@
 // Causal attention over packed clips, backward (causal_fwd.hip's mask, groups and layouts).  With s2 = scale log2(e) q.k, P = exp2(s2 - lse) is recomputed
 // tile by tile:
-//     D_i = sum_d dO O,   dV = P^T dO,   dP = dO V^T,   dS = P (dP - D),   dQ = scale dS K,   dK = scale dS^T Q     (dK, dV summed over a group's heads)
+//     D_i = sum_d dO O (kept negated),   dV = P^T dO,   dP = dO V^T,   dS = P (dP - D),   dQ = scale dS K,   dK = scale dS^T Q     (dK, dV summed over a group's heads)
 // Two kernels, no atomics, so the gradients do not depend on the order blocks run in:
 //   causal_dq_kernel   a wave owns 32 queries (a lane's column is a query), loops over the keys they see; writes D on the way in
 //   causal_dkv_kernel  a wave owns 32 keys of one kv head (a lane's column is a key), loops over the group's heads and the queries that see them
@@ -34,7 +34,7 @@ constexpr float kFitStart = 0x1p100f;
 template <typename T> constexpr float kProbLog2 = __is_same(T, f16_t) ? 10.f : 0.f;
 
 // ---- dQ (and D) ----------------------------------------------------------------------------------------------------------------------------
-constexpr int QB = TR;
+constexpr int QB = 128;                          // queries per workgroup
 template <typename T, int D> struct DqShape {
     static constexpr int KT = (sizeof(T) == 4 && D == 128) ? 32 : 64;
     static constexpr int TILE_B = KT * D * (int)sizeof(T);
@@ -42,7 +42,7 @@ template <typename T, int D> struct DqShape {
 };
 
 template <typename T, int D>
-__global__ __launch_bounds__(256, (D == 128 && sizeof(T) == 4 ? 1 : 2)) void causal_dq_kernel(CausalBwdArgs b, int nsub, int positions) {
+__global__ __launch_bounds__(256, (D == 64 ? (sizeof(T) == 2 ? 4 : 2) : sizeof(T) == 2 ? 2 : 1)) void causal_dq_kernel(CausalBwdArgs b, int nsub, int positions) {
     constexpr int KT = DqShape<T, D>::KT, NB = KT / 32, KS = D / 16, DB = D / 32, TILE_B = DqShape<T, D>::TILE_B;
     constexpr bool F16 = __is_same(T, f16_t);
     typedef Tile<T, D> TL;
@@ -52,7 +52,7 @@ __global__ __launch_bounds__(256, (D == 128 && sizeof(T) == 4 ? 1 : 2)) void cau
 
     const Work w = find_work(a.kv_heads, nsub, 1);
     if (w.pos >= positions) return;
-    const Clip clip = find_clip<false>(a.q_offsets, a.k_offsets, a.B, a.causal, a.group, w.pos);
+    const Clip clip = find_clip<false, QB>(a.q_offsets, a.k_offsets, a.B, a.causal, a.group, w.pos);
     if (clip.b < 0) return;
     const int qf = clip.qf, Tq = clip.Tq, kf = clip.kf, Tk = clip.Tk, q0 = clip.tile * QB;
     const int shift = a.causal ? Tk - Tq : 0x3fffffff;
@@ -82,7 +82,7 @@ __global__ __launch_bounds__(256, (D == 128 && sizeof(T) == 4 ? 1 : 2)) void cau
     }
     dsum = halves_sum(dsum);
     const float lse = a.lse[(int64_t)head * a.q_rows + qr];
-    if (mine && hi == 0) b.dsum[(int64_t)head * a.q_rows + qr] = dsum;
+    if (mine && hi == 0) b.dsum[(int64_t)head * a.q_rows + qr] = -dsum;
 
     const int last_q = (int)((unsigned)(min(q0 + QB, N) - 1) / (unsigned)G);
     const int nkeys = min(Tk, max(0, last_q + shift + 1));
@@ -180,7 +180,7 @@ __global__ __launch_bounds__(256, (D == 128 && sizeof(T) == 4 ? 1 : 2)) void cau
 }
 
 // ---- dK, dV --------------------------------------------------------------------------------------------------------------------------------
-constexpr int KB = TR;                           // keys per workgroup
+constexpr int KB = 128;                         // keys per workgroup
 template <typename T, int D> struct DkvShape {
     static constexpr bool V_LDS = D == 128;                                // V fragments from LDS, not registers: lets two waves share a SIMD (f32: no spills)
     static constexpr int QT = sizeof(T) == 4 || V_LDS ? 32 : 64;           // queries per tile
@@ -190,7 +190,7 @@ template <typename T, int D> struct DkvShape {
 };
 
 template <typename T, int D>
-__global__ __launch_bounds__(256, (D == 128 && sizeof(T) == 4 ? 1 : 2)) void causal_dkv_kernel(CausalBwdArgs b, int nsub, int positions) {
+__global__ __launch_bounds__(256, (D == 64 ? (sizeof(T) == 2 ? 3 : 2) : sizeof(T) == 2 ? 2 : 1)) void causal_dkv_kernel(CausalBwdArgs b, int nsub, int positions) {
     constexpr int QT = DkvShape<T, D>::QT, NB = QT / 32, KS = D / 16, DB = D / 32, TILE_B = DkvShape<T, D>::TILE_B, STAGE_B = DkvShape<T, D>::STAGE_B;
     constexpr bool F16 = __is_same(T, f16_t);
     typedef Tile<T, D> TL;
@@ -200,7 +200,7 @@ __global__ __launch_bounds__(256, (D == 128 && sizeof(T) == 4 ? 1 : 2)) void cau
 
     const Work w = find_work(a.kv_heads, nsub, b.parts);
     if (w.pos >= positions) return;
-    const Clip clip = find_clip<true>(a.q_offsets, a.k_offsets, a.B, a.causal, a.group, w.pos);
+    const Clip clip = find_clip<true, KB>(a.q_offsets, a.k_offsets, a.B, a.causal, a.group, w.pos);
     if (clip.b < 0) return;
     const int qf = clip.qf, Tq = clip.Tq, kf = clip.kf, Tk = clip.Tk, k0 = clip.tile * KB;
     const int shift = a.causal ? Tk - Tq : 0x3fffffff;
@@ -276,7 +276,14 @@ __global__ __launch_bounds__(256, (D == 128 && sizeof(T) == 4 ? 1 : 2)) void cau
         for (int nb = 0; nb < NB; ++nb) {
             const int qb0 = t * QT + nb * 32;
             if (qb0 >= Tq || qb0 + 31 + shift < kw) continue;             // nobody here / nobody sees this wave's first key
+            // 16-bit: the product dP starts from -D, which saves the subtraction (f32, bound by its matrix products: 80 -> 88 us at 8 x 520 frames)
             f32x16 s = zero16(), dp = zero16();
+#pragma unroll
+            for (int r4 = 0; r4 < 4 && sizeof(T) == 2; ++r4) {
+                const f32x4 d4 = *reinterpret_cast<const f32x4*>(lt + 64 + nb * 32 + 8 * r4 + 4 * hi);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) dp[4 * r4 + i] = d4[i];
+            }
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
                 s = mma<T>(TL::row_frag(qt, nb * 32 + l31, ks, hi), kfr[ks], s);
@@ -286,28 +293,30 @@ __global__ __launch_bounds__(256, (D == 128 && sizeof(T) == 4 ? 1 : 2)) void cau
 #pragma unroll
             for (int r4 = 0; r4 < 4; ++r4) {
                 const f32x4 lv = *reinterpret_cast<const f32x4*>(lt + nb * 32 + 8 * r4 + 4 * hi);
-                const f32x4 dv4 = *reinterpret_cast<const f32x4*>(lt + 64 + nb * 32 + 8 * r4 + 4 * hi);
+                f32x4 d4 = {0.f, 0.f, 0.f, 0.f};
+                if constexpr (sizeof(T) == 4) d4 = *reinterpret_cast<const f32x4*>(lt + 64 + nb * 32 + 8 * r4 + 4 * hi);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const int r = 4 * r4 + i;
-                    float p = exp2_(fmaf(s[r], c2, kProbLog2<T> - lv[i]));
-                    float d = p * (dp[r] - dv4[i]);
-                    if (edge) {
-                        const int qi = qb0 + crow(r, hi);
-                        const bool see = qi < Tq && key < Tk && key <= qi + shift;
-                        p = see ? p : 0.f;
-                        d = see ? d : 0.f;
-                    }
-                    s[r] = p;
-                    dp[r] = d;
+                    s[r] = exp2_(kProbLog2<T> == 0.f ? fmaf(s[r], c2, -lv[i]) : fmaf(s[r], c2, kProbLog2<T> - lv[i]));
+                    dp[r] = s[r] * (sizeof(T) == 4 ? dp[r] + d4[i] : dp[r]);
                 }
+            }
+            if (edge) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const int qi = qb0 + crow(r, hi);
+                    const bool see = qi < Tq && key < Tk && key <= qi + shift;
+                    s[r] = see ? s[r] : 0.f;
+                    dp[r] = see ? dp[r] : 0.f;
+                }
+                bad |= block_not_finite<T, D>(qt, nb * 32) || block_not_finite<T, D>(gt, nb * 32);
             }
             if constexpr (F16) {
                 fit_column<DB>(dp, F, dk);
 #pragma unroll
                 for (int r = 0; r < 16; ++r) dp[r] *= F;
             }
-            if (edge) bad |= block_not_finite<T, D>(qt, nb * 32) || block_not_finite<T, D>(gt, nb * 32);
 #pragma unroll
             for (int s2 = 0; s2 < 2; ++s2) {
                 const frag pf = pack8<T>(s, s2), df = pack8<T>(dp, s2);
@@ -338,7 +347,7 @@ __global__ __launch_bounds__(256, (D == 128 && sizeof(T) == 4 ? 1 : 2)) void cau
                 const float* dp = dbase + (int64_t)gg * a.q_rows;
                 const auto prob = [&](int i) { return exp2_(fmaf(dot_rows<T, D>(qp + (int64_t)i * a.q.row, kp), c2, -lp[i])); };
                 solo_column<T, D>(xv, r0, r1, gp, b.dout.row, prob);
-                solo_column<T, D>(xk, r0, r1, qp, a.q.row, [&](int i) { return prob(i) * (dot_rows<T, D>(gp + (int64_t)i * b.dout.row, vp) - dp[i]); });
+                solo_column<T, D>(xk, r0, r1, qp, a.q.row, [&](int i) { return prob(i) * (dot_rows<T, D>(gp + (int64_t)i * b.dout.row, vp) + dp[i]); });
             }
 #pragma unroll
             for (int e = 0; e < (D + 63) / 64; ++e) {
@@ -423,12 +432,14 @@ template <typename T, int D> hipError_t run(const CausalBwdArgs& b, hipStream_t 
 
 }  // namespace
 
-// Parts the queries (and heads of a group) that a key tile meets are cut into: as many as bring the launch to 6 workgroups per CU, at least 4 tiles of 64
-// queries each.  Lengths are on the device, so the averages over the batch decide.
+// Parts the queries (and heads of a group) that a key tile meets are cut into: as many as bring the launch to 1200 workgroups - some rounds of the 512 to 768
+// that run at once, so that causal tiles of unequal work end together; every part costs a plane of partial sums -, at least 4 tiles of 64 queries each.
+// us of the kernel + the sum, bf16: 8 x 2584 frames, 8/2 heads of 64: 1 part 412, 2: 233 + 10, 3: 173 + 13, 4: 157 + 15, 5: 162 + 18; 8191 + 1326 frames,
+// 16/4 heads of 128: 1 part 1859, 2: 1057 + 16, 3: 782 + 22, 4: 751 + 27, 6: 747 + 39.  Lengths are on the device, so the averages over the batch decide.
 int causal_bwd_parts(int64_t q_rows, int64_t k_rows, int B, int heads, int kv_heads) {
     if (B <= 0 || q_rows <= 0 || k_rows <= 0) return 1;
     const int64_t tiles = (k_rows + KB - 1) / KB > B ? (k_rows + KB - 1) / KB : B;
-    const int64_t want = (1536 + tiles * kv_heads - 1) / (tiles * kv_heads), room = (q_rows / B + 63) / 64 * (heads / kv_heads) / 4;
+    const int64_t want = (1200 + tiles * kv_heads - 1) / (tiles * kv_heads), room = (q_rows / B + 63) / 64 * (heads / kv_heads) / 4;
     const int64_t p = want < room ? want : room;
     return p < 1 ? 1 : p > 16 ? 16 : (int)p;
 }

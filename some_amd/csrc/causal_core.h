@@ -71,6 +71,24 @@ __device__ __forceinline__ f32x16 zero16() {
     return z;
 }
 
+// Instruction order inside a basic block.  Left alone, hipcc places every LDS read directly before the matrix instruction that needs it and waits for it
+// there, one read in flight at a time.  A sequence of these calls at the end of a block asks for `N` instructions of one kind after the other instead:
+// reads some products ahead, exponentials between products.
+template <int N> __device__ __forceinline__ void order_mfma() { __builtin_amdgcn_sched_group_barrier(0x008, N, 0); }
+template <int N> __device__ __forceinline__ void order_lds() { __builtin_amdgcn_sched_group_barrier(0x100, N, 0); }
+template <int N> __device__ __forceinline__ void order_valu() { __builtin_amdgcn_sched_group_barrier(0x002, N, 0); }
+template <int N> __device__ __forceinline__ void order_exp() { __builtin_amdgcn_sched_group_barrier(0x400, N, 0); }
+// MFMAS products, each with READS LDS reads of its own, the reads AHEAD products early
+template <int MFMAS, int READS, int AHEAD> __device__ __forceinline__ void order_products() {
+    order_lds<READS * AHEAD>();
+#pragma unroll
+    for (int i = 0; i < MFMAS - AHEAD; ++i) {
+        order_mfma<1>();
+        order_lds<READS>();
+    }
+    order_mfma<AHEAD>();
+}
+
 // registers 8 s .. 8 s + 7 of a product as a fragment, rounded to the operand type (16-bit: half an ulp, 2^-9 / 2^-12 of the value)
 template <typename T> __device__ __forceinline__ typename Frag<T>::type pack8(const f32x16& x, int s) {
     typename Frag<T>::type f;
@@ -229,10 +247,9 @@ __device__ __forceinline__ void solo_column(float (&acc)[(D + 63) / 64], int r0,
 }
 
 // ---- block map ------------------------------------------------------------------------------------------------------------------------
-// Rows are packed: clip b owns rows [off[b], off[b + 1]) of the queries and of the keys.  The heads of a group share keys, so a query tile holds 128 / group
+// Rows are packed: clip b owns rows [off[b], off[b + 1]) of the queries and of the keys.  The heads of a group share keys, so a query tile holds TR / group
 // frames with all their heads: query n of a clip is frame n / group, head n % group.  A launch has a position for every tile of TR queries (keys) the clips
 // can have (`rows / TR + B` of them cover any lengths); a block finds its clip and tile from its position and the offsets alone, without a table.
-constexpr int TR = 128;
 struct Clip { int b, tile, qf, Tq, kf, Tk; };             // b < 0: no such tile
 
 // sum over the wave of the lanes up to this one (lane 63: of all)
@@ -249,10 +266,10 @@ __device__ __forceinline__ int wave_total(int x) { return __builtin_amdgcn_readl
 
 // Up to 64 clips: positions run through the tiles of all clips by falling work - the keys a query tile sees, or (KEYS) the queries that see a key tile -
 // so the longest blocks start first whichever clip they belong to and the launch ends evenly.  A lane holds a clip; a clip's tiles in falling order of
-// work are its last query tile first (its first key tile first), `at_least(x)` of them with a work of x units of 128 or more; a bisection finds the
+// work are its last query tile first (its first key tile first), `at_least(x)` of them with a work of x units of TR or more; a bisection finds the
 // level position p falls into.  More clips: clip after clip (each is then a small part of the launch), found by counting the clips that begin before.
-// (Query tiles count in units of 128 / group keys, so that a clip's next tile sees one unit more.)
-template <bool KEYS>
+// (Query tiles count in units of TR / group keys, so that a clip's next tile sees one unit more.)
+template <bool KEYS, int TR>
 __device__ __forceinline__ Clip find_clip(const int32_t* __restrict__ q_off, const int32_t* __restrict__ k_off, int B, bool causal, int group, int p) {
     const int lane = threadIdx.x & 63;
     Clip c;

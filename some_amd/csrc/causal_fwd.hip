@@ -14,13 +14,13 @@ using namespace causal;
 // reaches 256, far inside every operand type, and the accumulators are rescaled once or twice per row instead of at every new maximum.
 constexpr float kSlack = 8.f;
 
-template <typename T, int D, int QN> struct Shape {
+constexpr int QB = 128;                          // queries per workgroup
+
+template <typename T, int D> struct Shape {
     static constexpr int KT = (sizeof(T) == 4 && D == 128) ? 32 : 64;      // keys per tile
     static constexpr int TILE_B = KT * D * (int)sizeof(T);
     static constexpr int STAGES = 2;
     static constexpr int LDS_B = STAGES * 2 * TILE_B;
-    static constexpr int QB = 128 * QN;                                    // queries per workgroup
-    static_assert(QB == TR, "one position, one workgroup");
 };
 
 // one query, all its visible keys in [j0, j1) (causal_core.h, "not-a-number and infinities"): unnormalised sums, maximum and sum
@@ -47,17 +47,17 @@ __device__ __forceinline__ void solo_query(const CausalArgs& a, const T* q, cons
     *o1 = D > 64 ? acc[(D + 63) / 64 - 1] : 0.f;
 }
 
-template <typename T, int D, int QN>
-__global__ __launch_bounds__(256, 2) void causal_fwd_kernel(CausalArgs a, int nsub, int positions) {
-    typedef Shape<T, D, QN> SH;
-    constexpr int KT = SH::KT, NB = KT / 32, KS = D / 16, DB = D / 32, TILE_B = SH::TILE_B, STAGES = SH::STAGES, QB = SH::QB;
+template <typename T, int D>
+__global__ __launch_bounds__(256, (sizeof(T) == 2 && D == 64 ? 4 : 2)) void causal_fwd_kernel(CausalArgs a, int nsub, int positions) {
+    typedef Shape<T, D> SH;
+    constexpr int KT = SH::KT, NB = KT / 32, KS = D / 16, DB = D / 32, TILE_B = SH::TILE_B, STAGES = SH::STAGES;
     typedef Tile<T, D> TL;
     typedef typename Frag<T>::type frag;
     extern __shared__ __attribute__((aligned(16))) char lds[];
 
     const Work w = find_work(a.kv_heads, nsub, a.parts);
     if (w.pos >= positions) return;
-    const Clip clip = find_clip<false>(a.q_offsets, a.k_offsets, a.B, a.causal, a.group, w.pos);
+    const Clip clip = find_clip<false, QB>(a.q_offsets, a.k_offsets, a.B, a.causal, a.group, w.pos);
     if (clip.b < 0) return;
     const int qf = clip.qf, Tq = clip.Tq, kf = clip.kf, Tk = clip.Tk, q0 = clip.tile * QB;
     const int shift = a.causal ? Tk - Tq : 0x3fffffff;       // query i sees keys j <= i + shift
@@ -65,25 +65,20 @@ __global__ __launch_bounds__(256, 2) void causal_fwd_kernel(CausalArgs a, int ns
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int l31 = lane & 31, hi = lane >> 5;
-    const int qw = q0 + wave * 32 * QN;                      // the wave's first query; block n holds qw + 32 n ..
-    int row[QN], head[QN];                                   // this lane's frames and heads
-    frag qfr[QN][KS];
+    const int qw = q0 + wave * 32;                           // the wave's first query
+    const unsigned n_lane = (unsigned)min(qw + l31, N - 1);  // this lane's frame and head:
+    const int q = (int)(n_lane / (unsigned)G), head = head0 + (int)(n_lane % (unsigned)G);
+    const T* qrow = static_cast<const T*>(a.q.p) + (int64_t)(qf + q) * a.q.row + (int64_t)head * a.q.head + 8 * hi;
+    frag qfr[KS];
 #pragma unroll
-    for (int n = 0; n < QN; ++n) {
-        const unsigned i = (unsigned)min(qw + 32 * n + l31, N - 1);
-        row[n] = (int)(i / (unsigned)G);
-        head[n] = head0 + (int)(i % (unsigned)G);
-        const T* qrow = static_cast<const T*>(a.q.p) + (int64_t)(qf + row[n]) * a.q.row + (int64_t)head[n] * a.q.head + 8 * hi;
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks) qfr[n][ks] = load8<T>(qrow + 16 * ks);
-    }
+    for (int ks = 0; ks < KS; ++ks) qfr[ks] = load8<T>(qrow + 16 * ks);
 
     const int last_q = (int)((unsigned)(min(q0 + QB, N) - 1) / (unsigned)G);
     const int nkeys = min(Tk, max(0, last_q + shift + 1));   // keys anybody here sees
     const int ntiles = (nkeys + KT - 1) / KT;
     // this part's tiles
     const int t_begin = (int)((int64_t)ntiles * part / a.parts), t_end = (int)((int64_t)ntiles * (part + 1) / a.parts);
-    const int seen_w = min(Tk, max(0, (int)((unsigned)min(qw + 32 * QN - 1, N - 1) / (unsigned)G) + shift + 1));        // keys this wave sees
+    const int seen_w = min(Tk, max(0, (int)((unsigned)min(qw + 31, N - 1) / (unsigned)G) + shift + 1));        // keys this wave sees
     const int full_w = min(Tk, max(0, (int)((unsigned)qw / (unsigned)G) + shift + 1));      // keys every query of the wave sees
 
     const char* kbase = reinterpret_cast<const char*>(static_cast<const T*>(a.k.p) + (int64_t)kf * a.k.row + (int64_t)w.kvh * a.k.head);
@@ -99,15 +94,10 @@ __global__ __launch_bounds__(256, 2) void causal_fwd_kernel(CausalArgs a, int ns
         cv.run(st + TILE_B, vbase + (int64_t)(t * KT) * vbytes, left, tid);
     };
 
-    f32x16 o[QN][DB];
-    float m[QN], l[QN];                                      // running maximum (of the raw products) and this half's share of the sum
+    f32x16 o[DB];
 #pragma unroll
-    for (int n = 0; n < QN; ++n) {
-        m[n] = -INFINITY;
-        l[n] = 0.f;
-#pragma unroll
-        for (int d = 0; d < DB; ++d) o[n][d] = zero16();
-    }
+    for (int d = 0; d < DB; ++d) o[d] = zero16();
+    float m = -INFINITY, l = 0.f;                            // running maximum (of the raw products) and this half's share of the sum
     const float c2 = a.scale * 1.4426950408889634f, slack = kSlack / c2;
     bool bad = false;
 
@@ -120,119 +110,100 @@ __global__ __launch_bounds__(256, 2) void causal_fwd_kernel(CausalArgs a, int ns
         const char* vt = kt + TILE_B;
         const int key0 = t * KT;
         if (key0 >= seen_w) continue;
-        f32x16 s[QN][NB];
+        f32x16 s[NB];
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
+            s[nb] = zero16();
 #pragma unroll
-            for (int n = 0; n < QN; ++n) s[n][nb] = zero16();
-#pragma unroll
-            for (int ks = 0; ks < KS; ++ks) {
-                const frag kfr = TL::row_frag(kt, nb * 32 + l31, ks, hi);
-#pragma unroll
-                for (int n = 0; n < QN; ++n) s[n][nb] = mma<T>(kfr, qfr[n][ks], s[n][nb]);
-            }
+            for (int ks = 0; ks < KS; ++ks) s[nb] = mma<T>(TL::row_frag(kt, nb * 32 + l31, ks, hi), qfr[ks], s[nb]);
         }
+        if constexpr (sizeof(T) == 2) order_products<NB * KS, 1, 4>();
         if (key0 + KT > full_w) {                            // some masked place in here
+            const int limit = min(q + shift, Tk - 1);
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb) {
                 bad |= block_not_finite<T, D>(vt, nb * 32);
 #pragma unroll
-                for (int n = 0; n < QN; ++n) {
-                    const int limit = min(row[n] + shift, Tk - 1);
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) s[n][nb][r] = key0 + nb * 32 + crow(r, hi) <= limit ? s[n][nb][r] : -INFINITY;
-                }
+                for (int r = 0; r < 16; ++r) s[nb][r] = key0 + nb * 32 + crow(r, hi) <= limit ? s[nb][r] : -INFINITY;
             }
         }
+        float mx = s[0][0];
 #pragma unroll
-        for (int n = 0; n < QN; ++n) {
-            float mx = s[n][0][0];
+        for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-            for (int nb = 0; nb < NB; ++nb)
+            for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[nb][r]);
+        mx = halves_max(mx);
+        if (__any(mx > m + slack)) {                         // (the first visible key passes -inf)
+            const float mn = mx > m + slack ? mx : m;
+            const float f = m == -INFINITY ? 0.f : exp2_((m - mn) * c2);
+            m = mn;
+            l *= f;
 #pragma unroll
-                for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[n][nb][r]);
-            mx = halves_max(mx);
-            if (__any(mx > m[n] + slack)) {                  // (the first visible key passes -inf)
-                const float mn = mx > m[n] + slack ? mx : m[n];
-                const float f = m[n] == -INFINITY ? 0.f : exp2_((m[n] - mn) * c2);
-                m[n] = mn;
-                l[n] *= f;
+            for (int d = 0; d < DB; ++d)
 #pragma unroll
-                for (int d = 0; d < DB; ++d)
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) o[n][d][r] *= f;
-            }
-            const float mc = m[n] == -INFINITY ? 0.f : m[n] * c2;
-#pragma unroll
-            for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    s[n][nb][r] = exp2_(fmaf(s[n][nb][r], c2, -mc));
-                    l[n] += s[n][nb][r];
-                }
+                for (int r = 0; r < 16; ++r) o[d][r] *= f;
         }
+        const float mc = m == -INFINITY ? 0.f : m * c2;
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                s[nb][r] = exp2_(fmaf(s[nb][r], c2, -mc));
+                l += s[nb][r];
+            }
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
             for (int s2 = 0; s2 < 2; ++s2) {
-                frag p[QN];
+                const frag p = pack8<T>(s[nb], s2);
 #pragma unroll
-                for (int n = 0; n < QN; ++n) p[n] = pack8<T>(s[n][nb], s2);
-#pragma unroll
-                for (int d = 0; d < DB; ++d) {
-                    const frag vfr = TL::col_frag(vt, nb * 32 + 16 * s2, d, lane);
-#pragma unroll
-                    for (int n = 0; n < QN; ++n) o[n][d] = mma<T>(vfr, p[n], o[n][d]);
-                }
+                for (int d = 0; d < DB; ++d) o[d] = mma<T>(TL::col_frag(vt, nb * 32 + 16 * s2, d, lane), p, o[d]);
             }
+        if constexpr (sizeof(T) == 2) order_products<NB * 2 * DB, 2, 3>();
     }
 
     const int64_t prow = (int64_t)part * a.q_rows * a.kv_heads * a.group;
     if (bad) {                                               // (wave-uniform)
-        for (int n = 0; n < 32 * QN && qw + n < N; ++n) {
-            const int q = (qw + n) / G, hd = head0 + (qw + n) % G, limit = min(q + shift, Tk - 1);
+        for (int n = 0; n < 32 && qw + n < N; ++n) {
+            const int qn = (qw + n) / G, hd = head0 + (qw + n) % G, limit = min(qn + shift, Tk - 1);
             float mm, ll, o0, o1;
-            solo_query<T, D>(a, static_cast<const T*>(a.q.p) + (int64_t)(qf + q) * a.q.row + (int64_t)hd * a.q.head, reinterpret_cast<const T*>(kbase),
+            solo_query<T, D>(a, static_cast<const T*>(a.q.p) + (int64_t)(qf + qn) * a.q.row + (int64_t)hd * a.q.head, reinterpret_cast<const T*>(kbase),
                              reinterpret_cast<const T*>(vbase), t_begin * KT, min(t_end * KT, limit + 1), c2, &mm, &ll, &o0, &o1);
             if (a.parts > 1) {
-                const int64_t i = prow + (int64_t)(qf + q) * a.kv_heads * G + hd;
+                const int64_t i = prow + (int64_t)(qf + qn) * a.kv_heads * G + hd;
                 a.part_o[i * D + lane] = o0;
                 if (D > 64) a.part_o[i * D + 64 + lane] = o1;
                 if (lane == 0) *reinterpret_cast<f32x2*>(a.part_ml + 2 * i) = (f32x2){mm * c2, ll};
             } else {
                 const float inv = limit >= 0 ? 1.f / ll : 0.f;
-                T* orow = static_cast<T*>(a.out.p) + (int64_t)(qf + q) * a.out.row + (int64_t)hd * a.out.head;
+                T* orow = static_cast<T*>(a.out.p) + (int64_t)(qf + qn) * a.out.row + (int64_t)hd * a.out.head;
                 orow[lane] = (T)(o0 * inv);
                 if (D > 64) orow[64 + lane] = (T)(o1 * inv);
-                if (a.lse && lane == 0) a.lse[(int64_t)hd * a.q_rows + qf + q] = limit >= 0 ? mm * c2 + log2_(ll) : -INFINITY;
+                if (a.lse && lane == 0) a.lse[(int64_t)hd * a.q_rows + qf + qn] = limit >= 0 ? mm * c2 + log2_(ll) : -INFINITY;
             }
         }
         return;
     }
+    if (qw + l31 >= N) return;
+    const float sum = halves_sum(l);
+    if (a.parts > 1) {
+        const int64_t i = prow + (int64_t)(qf + q) * a.kv_heads * G + head;
 #pragma unroll
-    for (int n = 0; n < QN; ++n) {
-        if (qw + 32 * n + l31 >= N) continue;
-        const int q = row[n];
-        const float sum = halves_sum(l[n]);
-        if (a.parts > 1) {
-            const int64_t i = prow + (int64_t)(qf + q) * a.kv_heads * G + head[n];
+        for (int d = 0; d < DB; ++d)
 #pragma unroll
-            for (int d = 0; d < DB; ++d)
+            for (int r4 = 0; r4 < 4; ++r4)
+                store4<float>(a.part_o + i * D + 32 * d + 8 * r4 + 4 * hi, o[d][4 * r4], o[d][4 * r4 + 1], o[d][4 * r4 + 2], o[d][4 * r4 + 3]);
+        if (hi == 0) *reinterpret_cast<f32x2*>(a.part_ml + 2 * i) = (f32x2){m * c2, sum};
+    } else {
+        const bool any = q + shift >= 0 && Tk > 0;
+        const float inv = any ? 1.f / sum : 0.f;             // no visible key: zero
+        T* orow = static_cast<T*>(a.out.p) + (int64_t)(qf + q) * a.out.row + (int64_t)head * a.out.head;
 #pragma unroll
-                for (int r4 = 0; r4 < 4; ++r4)
-                    store4<float>(a.part_o + i * D + 32 * d + 8 * r4 + 4 * hi, o[n][d][4 * r4], o[n][d][4 * r4 + 1], o[n][d][4 * r4 + 2], o[n][d][4 * r4 + 3]);
-            if (hi == 0) *reinterpret_cast<f32x2*>(a.part_ml + 2 * i) = (f32x2){m[n] * c2, sum};
-        } else {
-            const bool any = q + shift >= 0 && Tk > 0;
-            const float inv = any ? 1.f / sum : 0.f;         // no visible key: zero
-            T* orow = static_cast<T*>(a.out.p) + (int64_t)(qf + q) * a.out.row + (int64_t)head[n] * a.out.head;
+        for (int d = 0; d < DB; ++d)
 #pragma unroll
-            for (int d = 0; d < DB; ++d)
-#pragma unroll
-                for (int r4 = 0; r4 < 4; ++r4)
-                    store4<T>(orow + 32 * d + 8 * r4 + 4 * hi, o[n][d][4 * r4] * inv, o[n][d][4 * r4 + 1] * inv, o[n][d][4 * r4 + 2] * inv, o[n][d][4 * r4 + 3] * inv);
-            if (a.lse && hi == 0) a.lse[(int64_t)head[n] * a.q_rows + qf + q] = any ? m[n] * c2 + log2_(sum) : -INFINITY;
-        }
+            for (int r4 = 0; r4 < 4; ++r4)
+                store4<T>(orow + 32 * d + 8 * r4 + 4 * hi, o[d][4 * r4] * inv, o[d][4 * r4 + 1] * inv, o[d][4 * r4 + 2] * inv, o[d][4 * r4 + 3] * inv);
+        if (a.lse && hi == 0) a.lse[(int64_t)head * a.q_rows + qf + q] = any ? m * c2 + log2_(sum) : -INFINITY;
     }
 }
 
@@ -266,39 +237,39 @@ template <typename T, int D> __global__ __launch_bounds__(256) void causal_join_
     }
 }
 
-template <typename T, int D, int QN> hipError_t run(const CausalArgs& a, hipStream_t s) {
-    typedef Shape<T, D, QN> SH;
+template <typename T, int D> hipError_t run(const CausalArgs& a, hipStream_t s) {
+    constexpr int lds = Shape<T, D>::LDS_B;
     static DeviceOnce once;
     if (once.need()) {
-        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(&causal_fwd_kernel<T, D, QN>), hipFuncAttributeMaxDynamicSharedMemorySize, SH::LDS_B);
+        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(&causal_fwd_kernel<T, D>), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
         if (e != hipSuccess) return e;
         once.mark();
     }
-    const int positions = (int)(a.q_rows * a.group / TR) + a.B;
-    hipLaunchKernelGGL((causal_fwd_kernel<T, D, QN>), dim3((unsigned)work_blocks(a.kv_heads, a.parts, positions)), dim3(256), SH::LDS_B, s, a,
-                       work_subs(a.kv_heads), positions);
+    const int positions = (int)(a.q_rows * a.group / QB) + a.B;
+    hipLaunchKernelGGL((causal_fwd_kernel<T, D>), dim3((unsigned)work_blocks(a.kv_heads, a.parts, positions)), dim3(256), lds, s, a, work_subs(a.kv_heads),
+                       positions);
     if (a.parts > 1) hipLaunchKernelGGL((causal_join_kernel<T, D>), dim3((unsigned)a.q_rows), dim3(256), 0, s, a);
     return hipGetLastError();
 }
 
-template <typename T, int D> hipError_t pick(const CausalArgs& a, hipStream_t s) { return run<T, D, 1>(a, s); }
-
 }  // namespace
 
-int64_t causal_fwd_blocks(const CausalArgs& a) { return causal::work_blocks(a.kv_heads, a.parts, (int)(a.q_rows * a.group / causal::TR) + a.B); }
+int64_t causal_fwd_blocks(const CausalArgs& a) { return causal::work_blocks(a.kv_heads, a.parts, (int)(a.q_rows * a.group / 128) + a.B); }
 
-// Parts the keys are cut into: 1 unless the queries alone give too few workgroups (below 3 per CU) AND the keys are long (256 of them per part at
-// least).  Lengths are on the device, so the averages over the batch decide.
+// Parts the keys are cut into: 1 unless the queries alone give too few workgroups AND the keys are long (256 of them per part at least).  Every part costs
+// a plane of partial sums, so the launch is only brought to about 576 workgroups (2 per CU and a few more for balance): an f16 chunk of 766 frames, 16/4
+// heads of 128, over 20 000 cached ones takes 4 parts 164 + 9 us, 5: 143 + 11, 6: 135 + 13, 8: 152 + 16, 12: 137 + 22.  Lengths are on the device, so the
+// averages over the batch decide.
 int causal_fwd_parts(int64_t q_rows, int64_t k_rows, int B, int heads, int kv_heads) {
     if (B <= 0 || q_rows <= 0) return 1;
     const int64_t queries = q_rows * (heads / kv_heads), tiles = (queries + 127) / 128 > B ? (queries + 127) / 128 : B;
-    const int64_t want = 768 / (tiles * kv_heads), room = k_rows / B / 256;
+    const int64_t want = 576 / (tiles * kv_heads), room = k_rows / B / 256;
     const int64_t p = want < room ? want : room;
     return p < 1 ? 1 : p > 32 ? 32 : (int)p;
 }
 
 hipError_t launch_causal_fwd(int dtype, int head_dim, const CausalArgs& a, hipStream_t s) {
     if (a.B <= 0 || a.q_rows <= 0) return hipSuccess;
-    if (head_dim == 64) return dtype == 0 ? pick<float, 64>(a, s) : dtype == 1 ? pick<f16_t, 64>(a, s) : pick<bf16_t, 64>(a, s);
-    return dtype == 0 ? pick<float, 128>(a, s) : dtype == 1 ? pick<f16_t, 128>(a, s) : pick<bf16_t, 128>(a, s);
+    if (head_dim == 64) return dtype == 0 ? run<float, 64>(a, s) : dtype == 1 ? run<f16_t, 64>(a, s) : run<bf16_t, 64>(a, s);
+    return dtype == 0 ? run<float, 128>(a, s) : dtype == 1 ? run<f16_t, 128>(a, s) : run<bf16_t, 128>(a, s);
 }

@@ -184,7 +184,7 @@ struct CausalArgs {
 struct CausalBwdArgs {
     CausalArgs f;                  // as in the forward call (out and lse read)
     Rows3 dout, dq, dk, dv;
-    float* dsum;                   // [heads, q_rows] scratch: rowsum(dout out)
+    float* dsum;                   // [heads, q_rows] scratch: -rowsum(dout out)
     float* part_k; float* part_v;  // parts > 1: [parts, k_rows, kv_heads, head_dim] each
     int64_t k_rows;
     int parts;
