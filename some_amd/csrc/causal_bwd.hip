@@ -87,7 +87,7 @@ __global__ __launch_bounds__(256, (D == 64 ? (sizeof(T) == 2 ? 4 : 2) : sizeof(T
     const int last_q = (int)((unsigned)(min(q0 + QB, N) - 1) / (unsigned)G);
     const int nkeys = min(Tk, max(0, last_q + shift + 1));
     const int ntiles = (nkeys + KT - 1) / KT;
-    const int seen_w = min(Tk, max(0, (int)((unsigned)min(qw + 31, N - 1) / (unsigned)G) + shift + 1));
+    const int seen_w = qw < N ? min(Tk, max(0, (int)((unsigned)min(qw + 31, N - 1) / (unsigned)G) + shift + 1)) : 0;
     const int limit = min(q + shift, Tk - 1);
     const int full_w = min(Tk, max(0, (int)((unsigned)qw / (unsigned)G) + shift + 1));
 
@@ -275,7 +275,7 @@ __global__ __launch_bounds__(256, (D == 64 ? (sizeof(T) == 2 ? 3 : 2) : sizeof(T
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
             const int qb0 = t * QT + nb * 32;
-            if (qb0 >= Tq || qb0 + 31 + shift < kw) continue;             // nobody here / nobody sees this wave's first key
+            if (kw >= Tk || qb0 >= Tq || qb0 + 31 + shift < kw) continue;  // no key of the wave's, no query here, or none that sees its first key
             // 16-bit: the product dP starts from -D, which saves the subtraction (f32, bound by its matrix products: 80 -> 88 us at 8 x 520 frames)
             f32x16 s = zero16(), dp = zero16();
 #pragma unroll

@@ -2,9 +2,9 @@
 // the end: the queries are the clip's last Tq frames), heads in groups that share keys and values.  A row that sees no key is 0 (log-sum -inf).
 //
 // One pass over the keys with a running maximum and sum (base 2, the scale folded into the exponent's multiplier).  A workgroup is 128 queries - 128 /
-// group frames with all heads of a group, which read every key tile together -, a wave 32 of them; S^T = K Q^T puts a query in every lane's column, so its maximum and sum are the lane's own registers plus one exchange
-// with the other half, and P^T is already the B operand of O^T += V^T P^T (causal_core.h): no probability touches LDS.  K and V tiles go global ->
-// LDS by DMA into a ring; V is read transposed by ds_read_b64_tr_b16.
+// group frames with all heads of a group, which read every key tile together -, a wave 32 of them; S^T = K Q^T puts a query in every lane's column, so its
+// maximum and sum are the lane's own registers plus one exchange with the other half, and P^T is already the B operand of O^T += V^T P^T (causal_core.h):
+// no probability touches LDS.  K and V tiles go global -> LDS by DMA into a ring; V is read transposed by ds_read_b64_tr_b16.
 #include "causal_core.h"
 
 namespace {
@@ -17,7 +17,7 @@ constexpr float kSlack = 8.f;
 constexpr int QB = 128;                          // queries per workgroup
 
 template <typename T, int D> struct Shape {
-    static constexpr int KT = (sizeof(T) == 4 && D == 128) ? 32 : 64;      // keys per tile
+    static constexpr int KT = sizeof(T) == 4 ? 32 : 64;      // keys per tile (f32, 8 x 520 frames, heads of 64: 64 keys 53 us, 32: 48)
     static constexpr int TILE_B = KT * D * (int)sizeof(T);
     static constexpr int STAGES = 2;
     static constexpr int LDS_B = STAGES * 2 * TILE_B;
@@ -78,7 +78,8 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 && D == 64 ? 4 : 2)) void caus
     const int ntiles = (nkeys + KT - 1) / KT;
     // this part's tiles
     const int t_begin = (int)((int64_t)ntiles * part / a.parts), t_end = (int)((int64_t)ntiles * (part + 1) / a.parts);
-    const int seen_w = min(Tk, max(0, (int)((unsigned)min(qw + 31, N - 1) / (unsigned)G) + shift + 1));        // keys this wave sees
+    // keys this wave sees (a wave behind the clip's last query: none)
+    const int seen_w = qw < N ? min(Tk, max(0, (int)((unsigned)min(qw + 31, N - 1) / (unsigned)G) + shift + 1)) : 0;
     const int full_w = min(Tk, max(0, (int)((unsigned)qw / (unsigned)G) + shift + 1));      // keys every query of the wave sees
 
     const char* kbase = reinterpret_cast<const char*>(static_cast<const T*>(a.k.p) + (int64_t)kf * a.k.row + (int64_t)w.kvh * a.k.head);

@@ -132,6 +132,25 @@ def test_attention(ops, eng, dtype, H, G, D, ql, kl, causal):
     assert all(torch.equal(a, b) for a, b in zip(grads, again))
 
 
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('H,G,D,clips', [(16, 16, 64, 40), (48, 16, 128, 40), (4, 2, 64, 640)])
+@pytest.mark.parametrize('ql,kl', LENGTHS + [([513, 70, 129], [513, 70, 129])])
+@pytest.mark.parametrize('causal', [True, False])
+def test_attention_among_empty_clips(ops, eng, dtype, H, G, D, clips, ql, kl, causal):
+    """Clips without frames, fewer and more than the block map takes in one wave, and more heads than one workgroup's worth."""
+    ql, kl = ql + [0] * clips, kl + [0] * clips
+    q, k, v = _qkv(131, sum(ql), sum(kl), H, G, D, dtype)
+    dout = _normal(135, sum(ql), H, D, dtype=dtype)
+    leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+    out = ops.causal_attention(*leaves, _batch(ql), kv_batch=_batch(kl), causal_mask=causal)
+    grads = torch.autograd.grad(out, leaves, dout)
+    w = oracle.attention(q, k, v, ql, kl, causal, dout=dout)
+    for i, (name, got) in enumerate(zip(('out', 'dq', 'dk', 'dv'), (out.detach(), *grads))):
+        oracle.check(got, w[2 * i], w[2 * i + 1], name)
+    again = torch.autograd.grad(ops.causal_attention(*leaves, _batch(ql), kv_batch=_batch(kl), causal_mask=causal), leaves, dout)
+    assert all(torch.equal(a, b) for a, b in zip(grads, again))
+
+
 @pytest.mark.parametrize('B', [2, 63, 64, 65, 150])
 @pytest.mark.parametrize('past', [False, True])
 def test_attention_of_many_clips(ops, B, past):
@@ -177,9 +196,10 @@ def test_attention_of_slices_and_scale(ops, eng, dtype):
 
 @pytest.mark.parametrize('dtype', TYPES)
 @pytest.mark.parametrize('D', [64, 128])
-def test_attention_large_logits(ops, dtype, D):
+@pytest.mark.parametrize('clips', [0, 640])
+def test_attention_large_logits(ops, dtype, D, clips):
     """Logits of some hundreds, one key far above the rest, rows whose maximum arrives in the last tile."""
-    lens, H, G = [333], 2, 1
+    lens, H, G = [333] + [0] * clips, 2, 1
     q, k, v = _qkv(51, 333, 333, H, G, D, dtype)
     q, k = q * 4, k * 4
     k[200] *= 3
@@ -191,9 +211,10 @@ def test_attention_large_logits(ops, dtype, D):
 @pytest.mark.parametrize('dtype', TYPES)
 @pytest.mark.parametrize('D', [64, 128])
 @pytest.mark.parametrize('bad', [math.nan, math.inf, -math.inf])
-def test_attention_is_blind_to_masked_places(eng, dtype, D, bad):
+@pytest.mark.parametrize('clips', [0, 640])
+def test_attention_is_blind_to_masked_places(eng, dtype, D, bad, clips):
     """Whatever stands at a later frame of the clip, in another clip or behind the last one does not reach an earlier frame."""
-    lens, H, G = [97, 40, 66], 4, 2
+    lens, H, G = [97, 40, 66] + [0] * clips, 4, 2
     M = sum(lens)
     q, k, v = _qkv(61, M + 9, M + 9, H, G, D, dtype)
     clean = eng.causal_attention(q[:M], k[:M], v[:M], _batch(lens))
@@ -216,9 +237,10 @@ def test_attention_is_blind_to_masked_places(eng, dtype, D, bad):
 
 
 @pytest.mark.parametrize('magnitude', [1e-7, 1e-3, 1.0, 3e4])
-def test_half_precision_gradients_of_any_magnitude(ops, magnitude):
+@pytest.mark.parametrize('clips', [0, 640])
+def test_half_precision_gradients_of_any_magnitude(ops, magnitude, clips):
     """f16 holds dO itself to a step; dS, far below or above f16's range, must not lose more."""
-    lens, H, G, D = [200, 65], 4, 2, 64
+    lens, H, G, D = [200, 65] + [0] * clips, 4, 2, 64
     M = sum(lens)
     q, k, v = _qkv(71, M, M, H, G, D, torch.float16)
     dout = (_normal(75, M, H, D) * magnitude).half()
@@ -527,9 +549,10 @@ def test_refusals_on_the_device(eng, ops):
 
 @pytest.mark.parametrize('dtype', TYPES)
 @pytest.mark.parametrize('D', [64, 128])
-def test_gradients_are_blind_to_masked_places(ops, dtype, D):
+@pytest.mark.parametrize('clips', [0, 640])
+def test_gradients_are_blind_to_masked_places(ops, dtype, D, clips):
     """A value that is not finite makes the gradients of what it meets non-finite - and of nothing else."""
-    lens, H, G = [97, 66], 4, 2
+    lens, H, G = [97, 66] + [0] * clips, 4, 2
     M = sum(lens)
     q, k, v = _qkv(301, M, M, H, G, D, dtype)
     dout = _normal(305, M, H, D, dtype=dtype)
