@@ -84,7 +84,8 @@ int some_op_qk_norm_rope(SomeHandle* h, int32_t dtype, int32_t head_dim, const v
 size_t some_train_qk_norm_rope_bytes(const SomeHandle* h, int64_t rows, int32_t heads, int32_t kv_heads, int32_t head_dim) {
     (void)h;
     if (rows < 0 || rows >= kMaxRows || heads <= 0 || kv_heads <= 0 || (head_dim != 64 && head_dim != 128)) return 256;
-    return (size_t)norm_rope_bwd_blocks(rows, heads + kv_heads, head_dim) * 2 * head_dim * sizeof(float);
+    const size_t n = (size_t)norm_rope_bwd_blocks(rows, heads, kv_heads, head_dim) * head_dim * sizeof(float);
+    return n < 256 ? 256 : n;
 }
 
 int some_train_qk_norm_rope_bwd(SomeHandle* h, int32_t dtype, int32_t head_dim, const void* q_dev, int64_t q_row, int64_t q_head, int32_t heads,
@@ -106,8 +107,8 @@ int some_train_qk_norm_rope_bwd(SomeHandle* h, int32_t dtype, int32_t head_dim, 
     C_CHECK(laid_out(dtype, a.q) && laid_out(dtype, a.k) && laid_out(dtype, a.dq_in) && laid_out(dtype, a.dk_in) && laid_out(dtype, a.q_out) &&
             laid_out(dtype, a.k_out), kLayout);
     C_CHECK(((reinterpret_cast<uintptr_t>(gamma_q_dev) | reinterpret_cast<uintptr_t>(gamma_k_dev)) & 15) == 0, "gains must be 16-byte aligned");
-    C_CHECK(((reinterpret_cast<uintptr_t>(dgamma_q_dev) | reinterpret_cast<uintptr_t>(dgamma_k_dev) | reinterpret_cast<uintptr_t>(scratch_dev)) & 3) == 0,
-            "gain gradients and scratch must be 4-byte aligned");
+    C_CHECK(((reinterpret_cast<uintptr_t>(dgamma_q_dev) | reinterpret_cast<uintptr_t>(dgamma_k_dev)) & 3) == 0, "gain gradients must be 4-byte aligned");
+    C_CHECK((reinterpret_cast<uintptr_t>(scratch_dev) & 15) == 0, "scratch must be 16-byte aligned");
     C_CHECK((reinterpret_cast<uintptr_t>(positions_dev) & (positions64 ? 7 : 3)) == 0, "positions must be aligned");
     C_CHECK(eps >= 0.f && std::isfinite(eps), "eps must be finite and not negative");
     C_CHECK(fill_turns(a, theta, head_dim), "theta must be finite and positive");

@@ -204,13 +204,13 @@ struct NormRopeArgs {
     Rows3 dq_in, dk_in;            // backward: dy
     const float* gamma_q; const float* gamma_k;
     const void* positions;         // [rows] int32, or int64 if positions64
-    float* partial;                // backward: [blocks, 2, head_dim]
+    float* partial;                // backward: [blocks, head_dim], those of q first
     int64_t rows;
-    int heads, kv_heads, positions64, parts;
+    int heads, kv_heads, positions64, parts, kv_parts, q_blocks;
     float eps;
     double turns[64];              // theta^(-2 i / head_dim) / (2 pi)
 };
-int norm_rope_bwd_blocks(int64_t rows, int heads, int head_dim);
+int norm_rope_bwd_blocks(int64_t rows, int heads, int kv_heads, int head_dim);
 hipError_t launch_norm_rope(int dtype, int head_dim, NormRopeArgs a, hipStream_t s);
 hipError_t launch_norm_rope_bwd(int dtype, int head_dim, NormRopeArgs a, float* dgq, float* dgk, int accumulate, hipStream_t s);
 int64_t causal_fwd_blocks(const CausalArgs& a);
