@@ -555,7 +555,8 @@ int some_train_qk_norm_rope_bwd(SomeHandle* h, int32_t dtype, int32_t head_dim, 
  * causal = 0 every key.  A query that sees no key gets 0, and nothing in a masked place - infinities and NaN included - reaches an output.
  * scale > 0.  lse_dev: NULL, or fp32 [heads, q_rows] for the backward (base-2 log-sum-exp, -inf where no key is seen).  workspace_dev:
  * some_op_causal_attention_bytes bytes (0 unless few queries meet many keys), 16-byte aligned, not shared with a call that may run at the same time. */
-size_t some_op_causal_attention_bytes(const SomeHandle* h, int32_t heads, int32_t kv_heads, int32_t head_dim, int32_t B, int64_t q_rows, int64_t k_rows);
+size_t some_op_causal_attention_bytes(const SomeHandle* h, int32_t dtype, int32_t heads, int32_t kv_heads, int32_t head_dim, int32_t B, int64_t q_rows,
+                                      int64_t k_rows);
 int some_op_causal_attention(SomeHandle* h, int32_t dtype, int32_t head_dim, const void* q_dev, int64_t q_row, int64_t q_head, int32_t heads,
                              const void* k_dev, int64_t k_row, int64_t k_head, const void* v_dev, int64_t v_row, int64_t v_head, int32_t kv_heads,
                              const int32_t* q_offsets_dev, const int32_t* k_offsets_dev, int32_t B, int64_t q_rows, int64_t k_rows, int32_t causal,

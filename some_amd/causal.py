@@ -185,7 +185,7 @@ def attention_forward(lib, h, stream, q, k, v, batch, kv, causal, scale, want_ls
     (M, H, D), (N, G, _) = q.shape, k.shape
     out = q.new_empty((M, H, D))
     lse = torch.empty((H, M), dtype=torch.float32, device=q.device) if want_lse else None
-    n = lib.some_op_causal_attention_bytes(h, H, G, D, batch.B, M, N)
+    n = lib.some_op_causal_attention_bytes(h, DTYPES[q.dtype], H, G, D, batch.B, M, N)
     work = torch.empty(n, dtype=torch.uint8, device=q.device) if n else None
     rc = lib.some_op_causal_attention(h, DTYPES[q.dtype], D, *_place(q), H, *_place(k), *_place(v), G, batch.frame_offsets_dev.data_ptr(),
                                       kv.frame_offsets_dev.data_ptr(), batch.B, M, N, causal, scale, out.data_ptr(), H * D, D,

@@ -121,10 +121,10 @@ int some_train_qk_norm_rope_bwd(SomeHandle* h, int32_t dtype, int32_t head_dim, 
     return SOME_OK;
 }
 
-size_t some_op_causal_attention_bytes(const SomeHandle* h, int32_t heads, int32_t kv_heads, int32_t head_dim, int32_t B, int64_t q_rows, int64_t k_rows) {
+size_t some_op_causal_attention_bytes(const SomeHandle* h, int32_t dtype, int32_t heads, int32_t kv_heads, int32_t head_dim, int32_t B, int64_t q_rows, int64_t k_rows) {
     (void)h;
     if (!heads_ok(heads, kv_heads) || head_dim <= 0 || B <= 0 || q_rows <= 0 || k_rows <= 0 || q_rows >= kMaxRows || k_rows >= kMaxRows) return 0;
-    const int parts = causal_fwd_parts(q_rows, k_rows, B, heads, kv_heads);
+    const int parts = causal_fwd_parts(dtype, q_rows, k_rows, B, heads, kv_heads);
     return parts > 1 ? (size_t)parts * q_rows * heads * (head_dim + 2) * sizeof(float) : 0;
 }
 
@@ -152,9 +152,9 @@ int some_op_causal_attention(SomeHandle* h, int32_t dtype, int32_t head_dim, con
     C_CHECK(laid_out(dtype, a.q) && laid_out(dtype, a.k) && laid_out(dtype, a.v) && laid_out(dtype, a.out), kLayout);
     a.lse = lse_dev; a.q_offsets = q_offsets_dev; a.k_offsets = k_offsets_dev; a.q_rows = q_rows;
     a.B = B; a.kv_heads = kv_heads; a.group = heads / kv_heads; a.causal = causal; a.scale = scale;
-    a.parts = k_rows > 0 ? causal_fwd_parts(q_rows, k_rows, B, heads, kv_heads) : 1;
+    a.parts = k_rows > 0 ? causal_fwd_parts(dtype, q_rows, k_rows, B, heads, kv_heads) : 1;
     if (a.parts > 1) {
-        if (!workspace_dev || workspace_bytes < some_op_causal_attention_bytes(h, heads, kv_heads, head_dim, B, q_rows, k_rows))
+        if (!workspace_dev || workspace_bytes < some_op_causal_attention_bytes(h, dtype, heads, kv_heads, head_dim, B, q_rows, k_rows))
             return cfail(h, SOME_ENOMEM, __func__, "workspace too small (some_op_causal_attention_bytes)");
         C_CHECK((reinterpret_cast<uintptr_t>(workspace_dev) & 15) == 0, "workspace must be 16-byte aligned");
         a.part_o = static_cast<float*>(workspace_dev);

@@ -331,18 +331,6 @@ __device__ __forceinline__ Clip find_clip(const int32_t* __restrict__ q_off, con
     if ((int64_t)c.tile * TR >= (KEYS ? c.Tk : c.Tq) * mul) c.b = -1;
     return c;
 }
-// the clip of a packed row (off[0] <= row < off[B])
-__device__ __forceinline__ int find_row(const int32_t* __restrict__ off, int B, int row) {
-    const int lane = threadIdx.x & 63;
-    int n = 0;
-    for (int base = 0; base < B; base += 64) {
-        const int b = base + lane;
-        const int c = __popcll(__ballot(b < B && off[b] <= row));
-        n += c;
-        if (c < 64) break;
-    }
-    return __builtin_amdgcn_readfirstlane(n - 1);
-}
 // blockIdx -> (kv head, position, head of the group and part): the blocks of one kv head run on as few of the 8 XCDs as balance allows (they read the same
 // K and V through that XCD's L2), neighbouring positions at the same time.
 struct Work { int kvh, pos, g; };

@@ -174,7 +174,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 && D == 64 ? 4 : 2)) void caus
                 const int64_t i = prow + (int64_t)(qf + qn) * a.kv_heads * G + hd;
                 a.part_o[i * D + lane] = o0;
                 if (D > 64) a.part_o[i * D + 64 + lane] = o1;
-                if (lane == 0) *reinterpret_cast<f32x2*>(a.part_ml + 2 * i) = (f32x2){mm * c2, ll};
+                if (lane == 0) *reinterpret_cast<f32x2*>(a.part_ml + 2 * i) = (f32x2){mm * c2, part == 0 && limit < 0 ? -1.f : ll};
             } else {
                 const float inv = limit >= 0 ? 1.f / ll : 0.f;
                 T* orow = static_cast<T*>(a.out.p) + (int64_t)(qf + qn) * a.out.row + (int64_t)hd * a.out.head;
@@ -187,6 +187,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 && D == 64 ? 4 : 2)) void caus
     }
     if (qw + l31 >= N) return;
     const float sum = halves_sum(l);
+    const bool any = q + shift >= 0 && Tk > 0;
     if (a.parts > 1) {
         const int64_t i = prow + (int64_t)(qf + q) * a.kv_heads * G + head;
 #pragma unroll
@@ -194,9 +195,8 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 && D == 64 ? 4 : 2)) void caus
 #pragma unroll
             for (int r4 = 0; r4 < 4; ++r4)
                 store4<float>(a.part_o + i * D + 32 * d + 8 * r4 + 4 * hi, o[d][4 * r4], o[d][4 * r4 + 1], o[d][4 * r4 + 2], o[d][4 * r4 + 3]);
-        if (hi == 0) *reinterpret_cast<f32x2*>(a.part_ml + 2 * i) = (f32x2){m * c2, sum};
+        if (hi == 0) *reinterpret_cast<f32x2*>(a.part_ml + 2 * i) = (f32x2){m * c2, part == 0 && !any ? -1.f : sum};
     } else {
-        const bool any = q + shift >= 0 && Tk > 0;
         const float inv = any ? 1.f / sum : 0.f;             // no visible key: zero
         T* orow = static_cast<T*>(a.out.p) + (int64_t)(qf + q) * a.out.row + (int64_t)head * a.out.head;
 #pragma unroll
@@ -208,34 +208,48 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 && D == 64 ? 4 : 2)) void caus
     }
 }
 
-// Joins the parts of the keys, in order: a block is one query row, its threads walk the heads' channels.
+// Joins the parts of the keys, in order, four channels a thread and four parts in flight (a clip's rows see keys in the first part or in none: it says so by
+// a sum of -1).  Bound by latency where parts are few: 4160 rows of 8 heads of 64 in two parts take 6 us in f32 and 5 in bf16.
 template <typename T, int D> __global__ __launch_bounds__(256) void causal_join_kernel(CausalArgs a) {
     const int heads = a.kv_heads * a.group;
-    const int64_t row = blockIdx.x;
+    const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x, i0 = id / (D / 4), row = i0 / heads;
+    const int h = (int)(i0 - row * heads), d = (int)(id % (D / 4)) * 4;
     if (row < a.q_offsets[0] || row >= a.q_offsets[a.B]) return;
-    const int b = find_row(a.q_offsets, a.B, (int)row);
-    const int i = (int)row - a.q_offsets[b], Tq = a.q_offsets[b + 1] - a.q_offsets[b], Tk = a.k_offsets[b + 1] - a.k_offsets[b];
-    const bool any = Tk > 0 && (!a.causal || i + Tk - Tq >= 0);
     const int64_t step = a.q_rows * heads;
-    for (int c = threadIdx.x; c < heads * (D / 4); c += 256) {
-        const int h = c / (D / 4), d = c % (D / 4) * 4;
-        const int64_t i0 = row * heads + h;
-        float mm = -INFINITY, sum = 0.f;
-        for (int p = 0; p < a.parts; ++p) mm = fmaxf(mm, a.part_ml[2 * (i0 + p * step)]);
-        f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-        for (int p = 0; p < a.parts; ++p) {
-            const f32x2 ml = *reinterpret_cast<const f32x2*>(a.part_ml + 2 * (i0 + p * step));
-            if (ml[1] == 0.f) continue;                      // nothing visible in this part
-            const float f = ml[0] == -INFINITY ? 1.f : exp2_(ml[0] - mm);
-            const f32x4 x = *reinterpret_cast<const f32x4*>(a.part_o + (i0 + p * step) * D + d);
+    float m = -INFINITY, sum = 0.f;
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+    bool any = true;
+    for (int p0 = 0; p0 < a.parts; p0 += 4) {
+        f32x2 ml[4];
+        f32x4 x[4];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) acc[k] = fmaf(x[k], f, acc[k]);
-            sum = fmaf(ml[1], f, sum);
+        for (int p = 0; p < 4; ++p) {
+            const int64_t i = i0 + min(p0 + p, a.parts - 1) * step;
+            ml[p] = *reinterpret_cast<const f32x2*>(a.part_ml + 2 * i);
+            x[p] = *reinterpret_cast<const f32x4*>(a.part_o + i * D + d);
         }
-        const float inv = any ? 1.f / sum : 0.f;
-        store4<T>(static_cast<T*>(a.out.p) + row * a.out.row + (int64_t)h * a.out.head + d, acc[0] * inv, acc[1] * inv, acc[2] * inv, acc[3] * inv);
-        if (a.lse && d == 0) a.lse[(int64_t)h * a.q_rows + row] = any ? mm + log2_(sum) : -INFINITY;
+        if (p0 == 0) any = !(ml[0][1] < 0.f);
+        float mm = m;
+#pragma unroll
+        for (int p = 0; p < 4; ++p) {
+            if (p0 + p >= a.parts || ml[p][1] <= 0.f) ml[p][0] = -INFINITY, ml[p][1] = 0.f, x[p] = (f32x4){0.f, 0.f, 0.f, 0.f};      // adds nothing
+            mm = fmaxf(mm, ml[p][0]);
+        }
+        const float f0 = m == -INFINITY ? 1.f : exp2_(m - mm);
+        m = mm;
+        sum *= f0;
+        acc *= f0;
+#pragma unroll
+        for (int p = 0; p < 4; ++p) {
+            const float f = ml[p][0] == -INFINITY ? 1.f : exp2_(ml[p][0] - mm);
+            sum = fmaf(ml[p][1], f, sum);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) acc[k] = fmaf(x[p][k], f, acc[k]);
+        }
     }
+    const float inv = any ? 1.f / sum : 0.f;
+    store4<T>(static_cast<T*>(a.out.p) + row * a.out.row + (int64_t)h * a.out.head + d, acc[0] * inv, acc[1] * inv, acc[2] * inv, acc[3] * inv);
+    if (a.lse && d == 0) a.lse[(int64_t)h * a.q_rows + row] = any ? m + log2_(sum) : -INFINITY;
 }
 
 template <typename T, int D> hipError_t run(const CausalArgs& a, hipStream_t s) {
@@ -249,7 +263,7 @@ template <typename T, int D> hipError_t run(const CausalArgs& a, hipStream_t s) 
     const int positions = (int)(a.q_rows * a.group / QB) + a.B;
     hipLaunchKernelGGL((causal_fwd_kernel<T, D>), dim3((unsigned)work_blocks(a.kv_heads, a.parts, positions)), dim3(256), lds, s, a, work_subs(a.kv_heads),
                        positions);
-    if (a.parts > 1) hipLaunchKernelGGL((causal_join_kernel<T, D>), dim3((unsigned)a.q_rows), dim3(256), 0, s, a);
+    if (a.parts > 1) hipLaunchKernelGGL((causal_join_kernel<T, D>), dim3((unsigned)((a.q_rows * a.kv_heads * a.group * (D / 4) + 255) / 256)), dim3(256), 0, s, a);
     return hipGetLastError();
 }
 
@@ -257,14 +271,15 @@ template <typename T, int D> hipError_t run(const CausalArgs& a, hipStream_t s) 
 
 int64_t causal_fwd_blocks(const CausalArgs& a) { return causal::work_blocks(a.kv_heads, a.parts, (int)(a.q_rows * a.group / 128) + a.B); }
 
-// Parts the keys are cut into: 1 unless the queries alone give too few workgroups AND the keys are long (256 of them per part at least).  Every part costs
-// a plane of partial sums, so the launch is only brought to about 576 workgroups (2 per CU and a few more for balance): an f16 chunk of 766 frames, 16/4
-// heads of 128, over 20 000 cached ones takes 4 parts 164 + 9 us, 5: 143 + 11, 6: 135 + 13, 8: 152 + 16, 12: 137 + 22.  Lengths are on the device, so the
-// averages over the batch decide.
-int causal_fwd_parts(int64_t q_rows, int64_t k_rows, int B, int heads, int kv_heads) {
+// Parts the keys are cut into: 1 unless the queries alone give too few workgroups AND the keys are long (256 of them per part at least in f32, 512 in the
+// 16-bit types).  Every part costs a plane of partial sums, so the launch is only brought to about 576 workgroups (2 per CU and a few more for balance): an f16
+// chunk of 766 frames, 16/4 heads of 128, over 20 000 cached ones takes 4 parts 164 + 9 us, 5: 143 + 11, 6: 135 + 13, 8: 152 + 16, 12: 137 + 22.  8 x 520
+// frames, 8 heads of 64: f32 1 part 63 us, 2: 48 + 6; bf16 17, 15 + 5.  2 x 1000, 8/1 heads of 128: f32 1 part 239, 3: 102 + 7; bf16 27, 22 + 6.  2 x 1500,
+// 8/2 heads of 64, bf16: 1 part 30, 2: 21 + 5, 3: 19 + 5.  Lengths are on the device, so the averages over the batch decide.
+int causal_fwd_parts(int dtype, int64_t q_rows, int64_t k_rows, int B, int heads, int kv_heads) {
     if (B <= 0 || q_rows <= 0) return 1;
     const int64_t queries = q_rows * (heads / kv_heads), tiles = (queries + 127) / 128 > B ? (queries + 127) / 128 : B;
-    const int64_t want = 576 / (tiles * kv_heads), room = k_rows / B / 256;
+    const int64_t want = 576 / (tiles * kv_heads), room = k_rows / B / (dtype == 0 ? 256 : 512);
     const int64_t p = want < room ? want : room;
     return p < 1 ? 1 : p > 32 ? 32 : (int)p;
 }

@@ -214,7 +214,7 @@ int norm_rope_bwd_blocks(int64_t rows, int heads, int kv_heads, int head_dim);
 hipError_t launch_norm_rope(int dtype, int head_dim, NormRopeArgs a, hipStream_t s);
 hipError_t launch_norm_rope_bwd(int dtype, int head_dim, NormRopeArgs a, float* dgq, float* dgk, int accumulate, hipStream_t s);
 int64_t causal_fwd_blocks(const CausalArgs& a);
-int causal_fwd_parts(int64_t q_rows, int64_t k_rows, int B, int heads, int kv_heads);
+int causal_fwd_parts(int dtype, int64_t q_rows, int64_t k_rows, int B, int heads, int kv_heads);
 hipError_t launch_causal_fwd(int dtype, int head_dim, const CausalArgs& a, hipStream_t s);
 int causal_bwd_parts(int64_t q_rows, int64_t k_rows, int B, int heads, int kv_heads);
 int64_t causal_bwd_blocks(const CausalBwdArgs& b);

@@ -133,7 +133,7 @@ def test_c_abi_refuses():
     assert step(work=None) == _lib.SOME_ENOMEM
     assert bwd(n=16) == _lib.SOME_ENOMEM and b'workspace' in lib.some_last_error(h)
     assert attn(N=100000) == _lib.SOME_ENOMEM and attn(N=100000, work=4096) == _lib.SOME_ENOMEM         # few queries over many keys: cut into parts
-    assert lib.some_op_causal_attention_bytes(h, 4, 2, 64, 1, 10, 100000) > 0 == lib.some_op_causal_attention_bytes(h, 8, 8, 64, 32, 82688, 82688)
+    assert lib.some_op_causal_attention_bytes(h, 2, 4, 2, 64, 1, 10, 100000) > 0 == lib.some_op_causal_attention_bytes(h, 2, 8, 8, 64, 32, 82688, 82688)
     assert rope_bwd(n=16) == _lib.SOME_ENOMEM and b'scratch' in lib.some_last_error(h)
     # nothing to do: no launch, no error
     assert attn(M=0) == attn(B=0) == step(B=0) == rope(rows=0) == _lib.SOME_OK

@@ -274,7 +274,7 @@ def test_few_queries_over_many_keys(ops, eng, dtype, H, G, D):
     """The keys are cut into parts here (and the queries of a key tile in the backward): unequal clips, parts that see nothing, values that are not finite."""
     import some_amd._lib as _lib
     ql, kl = [130, 3, 1, 40], [3001, 2, 1500, 40]
-    assert _lib.load().some_op_causal_attention_bytes(None, H, G, D, 4, sum(ql), sum(kl)) > 0
+    assert _lib.load().some_op_causal_attention_bytes(None, TYPES.index(dtype), H, G, D, 4, sum(ql), sum(kl)) > 0
     q, k, v = _qkv(84, sum(ql), sum(kl), H, G, D, dtype)
     dout = _normal(87, sum(ql), H, D, dtype=dtype)
     leaves = [t.detach().requires_grad_() for t in (q, k, v)]
