@@ -564,7 +564,8 @@ int some_op_causal_attention(SomeHandle* h, int32_t dtype, int32_t head_dim, con
                              void* stream);
 /* Its gradients (dk, dv summed over the heads of a group), without atomics: the same bits every time.  out_dev, lse_dev: the forward's;
  * workspace_dev: some_train_causal_attention_bytes bytes, as above.  Here too nothing in a masked place reaches an output. */
-size_t some_train_causal_attention_bytes(const SomeHandle* h, int32_t heads, int32_t kv_heads, int32_t head_dim, int32_t B, int64_t q_rows, int64_t k_rows);
+size_t some_train_causal_attention_bytes(const SomeHandle* h, int32_t dtype, int32_t heads, int32_t kv_heads, int32_t head_dim, int32_t B, int64_t q_rows,
+                                         int64_t k_rows);
 int some_train_causal_attention_bwd(SomeHandle* h, int32_t dtype, int32_t head_dim, const void* q_dev, int64_t q_row, int64_t q_head, int32_t heads,
                                     const void* k_dev, int64_t k_row, int64_t k_head, const void* v_dev, int64_t v_row, int64_t v_head,
                                     int32_t kv_heads, const int32_t* q_offsets_dev, const int32_t* k_offsets_dev, int32_t B, int64_t q_rows,

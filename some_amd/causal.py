@@ -199,7 +199,7 @@ def attention_backward(lib, h, stream, q, k, v, batch, kv, causal, scale, out, l
     dout = readable(dout)
     (M, H, D), (N, G, _) = q.shape, k.shape
     dq, dk, dv = q.new_empty((M, H, D)), k.new_empty((N, G, D)), v.new_empty((N, G, D))
-    n = lib.some_train_causal_attention_bytes(h, H, G, D, batch.B, M, N)
+    n = lib.some_train_causal_attention_bytes(h, DTYPES[q.dtype], H, G, D, batch.B, M, N)
     work = torch.empty(n, dtype=torch.uint8, device=q.device)
     rc = lib.some_train_causal_attention_bwd(h, DTYPES[q.dtype], D, *_place(q), H, *_place(k), *_place(v), G, batch.frame_offsets_dev.data_ptr(),
                                              kv.frame_offsets_dev.data_ptr(), batch.B, M, N, causal, scale, out.data_ptr(), H * D, D, lse.data_ptr(),

@@ -128,11 +128,14 @@ size_t some_op_causal_attention_bytes(const SomeHandle* h, int32_t dtype, int32_
     return parts > 1 ? (size_t)parts * q_rows * heads * (head_dim + 2) * sizeof(float) : 0;
 }
 
-size_t some_train_causal_attention_bytes(const SomeHandle* h, int32_t heads, int32_t kv_heads, int32_t head_dim, int32_t B, int64_t q_rows, int64_t k_rows) {
+size_t some_train_causal_attention_bytes(const SomeHandle* h, int32_t dtype, int32_t heads, int32_t kv_heads, int32_t head_dim, int32_t B, int64_t q_rows,
+                                         int64_t k_rows) {
     (void)h;
     if (!heads_ok(heads, kv_heads) || head_dim <= 0 || B <= 0 || q_rows < 0 || k_rows < 0 || q_rows >= kMaxRows || k_rows >= kMaxRows) return 256;
     const int parts = causal_bwd_parts(q_rows, k_rows, B, heads, kv_heads);
-    return dsum_bytes(heads, q_rows) + (parts > 1 ? (size_t)parts * k_rows * kv_heads * head_dim * 2 * sizeof(float) : 0);
+    const size_t keys = parts > 1 ? (size_t)parts * k_rows * kv_heads * head_dim * 2 * sizeof(float) : 0;
+    const size_t queries = some_op_causal_attention_bytes(h, dtype, heads, kv_heads, head_dim, B, q_rows, k_rows);
+    return dsum_bytes(heads, q_rows) + (keys > queries ? keys : queries);
 }
 
 int some_op_causal_attention(SomeHandle* h, int32_t dtype, int32_t head_dim, const void* q_dev, int64_t q_row, int64_t q_head, int32_t heads,
@@ -188,14 +191,14 @@ int some_train_causal_attention_bwd(SomeHandle* h, int32_t dtype, int32_t head_d
             laid_out(dtype, b.dk) && laid_out(dtype, b.dv), kLayout);
     a.lse = const_cast<float*>(lse_dev); a.q_offsets = q_offsets_dev; a.k_offsets = k_offsets_dev; a.q_rows = q_rows;
     a.B = B; a.kv_heads = kv_heads; a.group = heads / kv_heads; a.causal = causal; a.scale = scale;
-    a.parts = 1;
+    a.parts = k_rows > 0 ? causal_fwd_parts(dtype, q_rows, k_rows, B, heads, kv_heads) : 1;
     b.k_rows = k_rows;
     b.parts = causal_bwd_parts(q_rows, k_rows, B, heads, kv_heads);
-    if (workspace_bytes < some_train_causal_attention_bytes(h, heads, kv_heads, head_dim, B, q_rows, k_rows))
+    if (workspace_bytes < some_train_causal_attention_bytes(h, dtype, heads, kv_heads, head_dim, B, q_rows, k_rows))
         return cfail(h, SOME_ENOMEM, __func__, "workspace too small (some_train_causal_attention_bytes)");
     C_CHECK((reinterpret_cast<uintptr_t>(workspace_dev) & 15) == 0, "workspace must be 16-byte aligned");
     b.dsum = static_cast<float*>(workspace_dev);
-    b.part_k = reinterpret_cast<float*>(static_cast<char*>(workspace_dev) + dsum_bytes(heads, q_rows));
+    b.part_q = b.part_k = reinterpret_cast<float*>(static_cast<char*>(workspace_dev) + dsum_bytes(heads, q_rows));
     b.part_v = b.part_k + (int64_t)b.parts * k_rows * kv_heads * head_dim;
     C_CHECK(q_rows * a.group < 0x7fffffffll && causal_fwd_blocks(a) < 0x7fffffffll && causal_bwd_blocks(b) < 0x7fffffffll && k_rows * kv_heads * (head_dim / 4) / 256 < 0x7ffffff0ll, "too many rows, clips and heads for one launch");
     C_TRY(launch_causal_bwd(dtype, head_dim, b, static_cast<hipStream_t>(stream)));

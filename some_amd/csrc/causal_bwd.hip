@@ -50,7 +50,7 @@ __global__ __launch_bounds__(256, (D == 64 ? (sizeof(T) == 2 ? 4 : 2) : sizeof(T
     extern __shared__ __attribute__((aligned(16))) char lds[];
     const CausalArgs& a = b.f;
 
-    const Work w = find_work(a.kv_heads, nsub, 1);
+    const Work w = find_work(a.kv_heads, nsub, a.parts);
     if (w.pos >= positions) return;
     const Clip clip = find_clip<false, QB>(a.q_offsets, a.k_offsets, a.B, a.causal, a.group, w.pos);
     if (clip.b < 0) return;
@@ -82,11 +82,12 @@ __global__ __launch_bounds__(256, (D == 64 ? (sizeof(T) == 2 ? 4 : 2) : sizeof(T
     }
     dsum = halves_sum(dsum);
     const float lse = a.lse[(int64_t)head * a.q_rows + qr];
-    if (mine && hi == 0) b.dsum[(int64_t)head * a.q_rows + qr] = -dsum;
+    if (w.g == 0 && mine && hi == 0) b.dsum[(int64_t)head * a.q_rows + qr] = -dsum;
 
     const int last_q = (int)((unsigned)(min(q0 + QB, N) - 1) / (unsigned)G);
     const int nkeys = min(Tk, max(0, last_q + shift + 1));
     const int ntiles = (nkeys + KT - 1) / KT;
+    const int t_begin = (int)((int64_t)ntiles * w.g / a.parts), t_end = (int)((int64_t)ntiles * (w.g + 1) / a.parts);      // this part's tiles
     const int seen_w = qw < N ? min(Tk, max(0, (int)((unsigned)min(qw + 31, N - 1) / (unsigned)G) + shift + 1)) : 0;
     const int limit = min(q + shift, Tk - 1);
     const int full_w = min(Tk, max(0, (int)((unsigned)qw / (unsigned)G) + shift + 1));
@@ -111,11 +112,11 @@ __global__ __launch_bounds__(256, (D == 64 ? (sizeof(T) == 2 ? 4 : 2) : sizeof(T
     const float c2 = a.scale * 1.4426950408889634f;
     bool bad = false;
 
-    if (ntiles > 0) fetch(0);
-    for (int t = 0; t < ntiles; ++t) {
+    if (t_begin < t_end) fetch(t_begin);
+    for (int t = t_begin; t < t_end; ++t) {
         wait_vm<0>();
         __syncthreads();
-        if (t + 1 < ntiles) fetch(t + 1);
+        if (t + 1 < t_end) fetch(t + 1);
         const char* kt = lds + (t & 1) * 2 * TILE_B;
         const char* vt = kt + TILE_B;
 #pragma unroll
@@ -160,22 +161,31 @@ __global__ __launch_bounds__(256, (D == 64 ? (sizeof(T) == 2 ? 4 : 2) : sizeof(T
             const T* gp = static_cast<const T*>(b.dout.p) + row * b.dout.row + (int64_t)hd * b.dout.head;
             const float lse_n = __shfl(lse, n, 64), dsum_n = __shfl(dsum, n, 64);
             float x[(D + 63) / 64] = {};
-            solo_column<T, D>(x, 0, min(qn + shift, Tk - 1) + 1, kp, a.k.row, [&](int j) {
+            solo_column<T, D>(x, t_begin * KT, min(t_end * KT, min(qn + shift, Tk - 1) + 1), kp, a.k.row, [&](int j) {
                 return exp2_(fmaf(dot_rows<T, D>(qp, kp + (int64_t)j * a.k.row), c2, -lse_n)) * (dot_rows<T, D>(gp, vp + (int64_t)j * a.v.row) - dsum_n);
             });
             T* dst = static_cast<T*>(b.dq.p) + row * b.dq.row + (int64_t)hd * b.dq.head;
+            float* pdst = b.part_q + ((w.g * a.q_rows + row) * a.kv_heads * G + hd) * D;
 #pragma unroll
-            for (int e = 0; e < (D + 63) / 64; ++e) dst[lane + 64 * e] = (T)(x[e] * a.scale);
+            for (int e = 0; e < (D + 63) / 64; ++e) {
+                if (a.parts > 1) pdst[lane + 64 * e] = x[e] * a.scale;
+                else dst[lane + 64 * e] = (T)(x[e] * a.scale);
+            }
         }
         return;
     }
     if (mine) {
         const float f = a.scale / F;
         T* dst = static_cast<T*>(b.dq.p) + qr * b.dq.row + (int64_t)head * b.dq.head + 4 * hi;
+        float* pdst = b.part_q + ((w.g * a.q_rows + qr) * a.kv_heads * G + head) * D + 4 * hi;
 #pragma unroll
         for (int d = 0; d < DB; ++d)
 #pragma unroll
-            for (int r4 = 0; r4 < 4; ++r4) store4<T>(dst + 32 * d + 8 * r4, acc[d][4 * r4] * f, acc[d][4 * r4 + 1] * f, acc[d][4 * r4 + 2] * f, acc[d][4 * r4 + 3] * f);
+            for (int r4 = 0; r4 < 4; ++r4) {
+                const float x0 = acc[d][4 * r4] * f, x1 = acc[d][4 * r4 + 1] * f, x2 = acc[d][4 * r4 + 2] * f, x3 = acc[d][4 * r4 + 3] * f;
+                if (a.parts > 1) store4<float>(pdst + 32 * d + 8 * r4, x0, x1, x2, x3);
+                else store4<T>(dst + 32 * d + 8 * r4, x0, x1, x2, x3);
+            }
     }
 }
 
@@ -387,22 +397,25 @@ __global__ __launch_bounds__(256, (D == 64 ? (sizeof(T) == 2 ? 3 : 2) : sizeof(T
     }
 }
 
-// dK and dV: the parts summed in order, four channels a thread (blockIdx.y: 0 dK, 1 dV)
-template <typename T, int D> __global__ __launch_bounds__(256) void causal_sum_kernel(CausalBwdArgs b) {
-    const int G = b.f.kv_heads;
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, plane = b.k_rows * G * D;
-    const int64_t row = i / (G * (D / 4));
-    if (row < b.f.k_offsets[0] || row >= b.f.k_offsets[b.f.B]) return;
-    const int h = (int)(i % (G * (D / 4))) / (D / 4), d = (int)(i % (D / 4)) * 4;
-    const float* src = (blockIdx.y ? b.part_v : b.part_k) + i * 4;
+// dQ, or dK and dV (blockIdx.y): the parts summed in order, four channels a thread.
+struct SumArgs { const float* src[2]; Rows3 out[2]; const int32_t* offsets; int64_t rows; int B, heads, parts; };
+template <typename T, int D> __global__ __launch_bounds__(256) void causal_sum_kernel(SumArgs a) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, plane = a.rows * a.heads * D;
+    const int64_t row = i / (a.heads * (D / 4));
+    if (row < a.offsets[0] || row >= a.offsets[a.B]) return;
+    const int h = (int)(i % (a.heads * (D / 4))) / (D / 4), d = (int)(i % (D / 4)) * 4;
+    const float* src = a.src[blockIdx.y] + i * 4;
     f32x4 x = *reinterpret_cast<const f32x4*>(src);
-    for (int p = 1; p < b.parts; ++p) {
+    for (int p = 1; p < a.parts; ++p) {
         const f32x4 y = *reinterpret_cast<const f32x4*>(src + p * plane);
 #pragma unroll
         for (int k = 0; k < 4; ++k) x[k] += y[k];
     }
-    const Rows3& out = blockIdx.y ? b.dv : b.dk;
+    const Rows3& out = a.out[blockIdx.y];
     store4<T>(static_cast<T*>(out.p) + row * out.row + (int64_t)h * out.head + d, x[0], x[1], x[2], x[3]);
+}
+template <typename T, int D> void sum_parts(const SumArgs& a, unsigned planes, hipStream_t s) {
+    hipLaunchKernelGGL((causal_sum_kernel<T, D>), dim3((unsigned)((a.rows * a.heads * (D / 4) + 255) / 256), planes), dim3(256), 0, s, a);
 }
 
 template <typename T, int D> hipError_t run(const CausalBwdArgs& b, hipStream_t s) {
@@ -418,14 +431,14 @@ template <typename T, int D> hipError_t run(const CausalBwdArgs& b, hipStream_t 
     const int nsub = work_subs(a.kv_heads);
     if (a.q_rows > 0) {
         const int positions = (int)(a.q_rows * a.group / QB) + a.B;
-        hipLaunchKernelGGL((causal_dq_kernel<T, D>), dim3((unsigned)work_blocks(a.kv_heads, 1, positions)), dim3(256), (DqShape<T, D>::LDS_B), s, b, nsub, positions);
+        hipLaunchKernelGGL((causal_dq_kernel<T, D>), dim3((unsigned)work_blocks(a.kv_heads, a.parts, positions)), dim3(256), (DqShape<T, D>::LDS_B), s, b, nsub, positions);
+        if (a.parts > 1) sum_parts<T, D>({{b.part_q}, {b.dq}, a.q_offsets, a.q_rows, a.B, a.kv_heads * a.group, a.parts}, 1, s);
     }
     if (b.k_rows > 0) {
         const int positions = (int)(b.k_rows / KB) + a.B;
         hipLaunchKernelGGL((causal_dkv_kernel<T, D>), dim3((unsigned)work_blocks(a.kv_heads, b.parts, positions)), dim3(256), (DkvShape<T, D>::LDS_B), s, b, nsub,
                            positions);
-        if (b.parts > 1)
-            hipLaunchKernelGGL((causal_sum_kernel<T, D>), dim3((unsigned)((b.k_rows * a.kv_heads * (D / 4) + 255) / 256), 2), dim3(256), 0, s, b);
+        if (b.parts > 1) sum_parts<T, D>({{b.part_k, b.part_v}, {b.dk, b.dv}, a.k_offsets, b.k_rows, a.B, a.kv_heads, b.parts}, 2, s);
     }
     return hipGetLastError();
 }

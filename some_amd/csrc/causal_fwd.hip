@@ -275,7 +275,8 @@ int64_t causal_fwd_blocks(const CausalArgs& a) { return causal::work_blocks(a.kv
 // 16-bit types).  Every part costs a plane of partial sums, so the launch is only brought to about 576 workgroups (2 per CU and a few more for balance): an f16
 // chunk of 766 frames, 16/4 heads of 128, over 20 000 cached ones takes 4 parts 164 + 9 us, 5: 143 + 11, 6: 135 + 13, 8: 152 + 16, 12: 137 + 22.  8 x 520
 // frames, 8 heads of 64: f32 1 part 63 us, 2: 48 + 6; bf16 17, 15 + 5.  2 x 1000, 8/1 heads of 128: f32 1 part 239, 3: 102 + 7; bf16 27, 22 + 6.  2 x 1500,
-// 8/2 heads of 64, bf16: 1 part 30, 2: 21 + 5, 3: 19 + 5.  Lengths are on the device, so the averages over the batch decide.
+// 8/2 heads of 64, bf16: 1 part 30, 2: 21 + 5, 3: 19 + 5.  The gradient of the queries takes the same parts (and a sum): 2 x 1000, 8/1 heads of 128, f32 1 part
+// 225, 3: 93 + 6; 2 x 2000, bf16 68, 2: 48 + 8.  Lengths are on the device, so the averages over the batch decide.
 int causal_fwd_parts(int dtype, int64_t q_rows, int64_t k_rows, int B, int heads, int kv_heads) {
     if (B <= 0 || q_rows <= 0) return 1;
     const int64_t queries = q_rows * (heads / kv_heads), tiles = (queries + 127) / 128 > B ? (queries + 127) / 128 : B;

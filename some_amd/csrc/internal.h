@@ -185,6 +185,7 @@ struct CausalBwdArgs {
     CausalArgs f;                  // as in the forward call (out and lse read)
     Rows3 dout, dq, dk, dv;
     float* dsum;                   // [heads, q_rows] scratch: -rowsum(dout out)
+    float* part_q;                 // f.parts > 1: [f.parts, q_rows, heads, head_dim]; read before part_k and part_v, in the same memory, are written
     float* part_k; float* part_v;  // parts > 1: [parts, k_rows, kv_heads, head_dim] each
     int64_t k_rows;
     int parts;
