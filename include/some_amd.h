@@ -553,16 +553,18 @@ int some_train_qk_norm_rope_bwd(SomeHandle* h, int32_t dtype, int32_t head_dim, 
 /* out = softmax(scale q k^T) v per clip.  Clip b's queries are rows [q_offsets[b], q_offsets[b + 1]) and its keys rows [k_offsets[b], ...): with
  * causal != 0 the queries are the clip's LAST frames, i.e. query i of Tq sees keys j <= i + Tk - Tq (a chunk over what is cached already); with
  * causal = 0 every key.  A query that sees no key gets 0, and nothing in a masked place - infinities and NaN included - reaches an output.
- * scale > 0.  lse_dev: NULL, or fp32 [heads, q_rows] for the backward (base-2 log-sum-exp, -inf where no key is seen).  workspace_dev:
+ * scale > 0.  For the backward, each NULL if there is none: rest_dev [q_rows, heads, head_dim] of the type, what rounding to a 16-bit type took from out
+ * (f16: times 2^10; not used for fp32), and lse_dev fp32 [heads, q_rows] (base-2 log-sum-exp, -inf where no key is seen).  workspace_dev:
  * some_op_causal_attention_bytes bytes (0 unless few queries meet many keys), 16-byte aligned, not shared with a call that may run at the same time. */
 size_t some_op_causal_attention_bytes(const SomeHandle* h, int32_t dtype, int32_t heads, int32_t kv_heads, int32_t head_dim, int32_t B, int64_t q_rows,
                                       int64_t k_rows);
 int some_op_causal_attention(SomeHandle* h, int32_t dtype, int32_t head_dim, const void* q_dev, int64_t q_row, int64_t q_head, int32_t heads,
                              const void* k_dev, int64_t k_row, int64_t k_head, const void* v_dev, int64_t v_row, int64_t v_head, int32_t kv_heads,
                              const int32_t* q_offsets_dev, const int32_t* k_offsets_dev, int32_t B, int64_t q_rows, int64_t k_rows, int32_t causal,
-                             float scale, void* out_dev, int64_t o_row, int64_t o_head, float* lse_dev, void* workspace_dev, size_t workspace_bytes,
-                             void* stream);
-/* Its gradients (dk, dv summed over the heads of a group), without atomics: the same bits every time.  out_dev, lse_dev: the forward's;
+                             float scale, void* out_dev, int64_t o_row, int64_t o_head, void* rest_dev, float* lse_dev, void* workspace_dev,
+                             size_t workspace_bytes, void* stream);
+/* Its gradients (dk, dv summed over the heads of a group), without atomics: the same bits every time.  out_dev, rest_dev, lse_dev: the forward's
+ * (without rest_dev a row that sees few keys loses precision in 16-bit types);
  * workspace_dev: some_train_causal_attention_bytes bytes, as above.  Here too nothing in a masked place reaches an output. */
 size_t some_train_causal_attention_bytes(const SomeHandle* h, int32_t dtype, int32_t heads, int32_t kv_heads, int32_t head_dim, int32_t B, int64_t q_rows,
                                          int64_t k_rows);
@@ -570,7 +572,7 @@ int some_train_causal_attention_bwd(SomeHandle* h, int32_t dtype, int32_t head_d
                                     const void* k_dev, int64_t k_row, int64_t k_head, const void* v_dev, int64_t v_row, int64_t v_head,
                                     int32_t kv_heads, const int32_t* q_offsets_dev, const int32_t* k_offsets_dev, int32_t B, int64_t q_rows,
                                     int64_t k_rows, int32_t causal, float scale, const void* out_dev, int64_t o_row, int64_t o_head,
-                                    const float* lse_dev, const void* dout_dev, int64_t do_row, int64_t do_head, void* dq_dev, int64_t dq_row,
+                                    const void* rest_dev, const float* lse_dev, const void* dout_dev, int64_t do_row, int64_t do_head, void* dq_dev, int64_t dq_row,
                                     int64_t dq_head, void* dk_dev, int64_t dk_row, int64_t dk_head, void* dv_dev, int64_t dv_row, int64_t dv_head,
                                     void* workspace_dev, size_t workspace_bytes, void* stream);
 

@@ -180,29 +180,31 @@ def check_attention(device, q, k, v, batch, kv_batch, head_dim):
     return q, k, v, kv
 
 
-def attention_forward(lib, h, stream, q, k, v, batch, kv, causal, scale, want_lse):
-    """Launch on checked, readable views -> (out, lse or None)."""
+def attention_forward(lib, h, stream, q, k, v, batch, kv, causal, scale, for_backward):
+    """Launch on checked, readable views -> (out, rest, lse), the last two None unless ``for_backward`` (rest: 16-bit types alone)."""
     (M, H, D), (N, G, _) = q.shape, k.shape
     out = q.new_empty((M, H, D))
-    lse = torch.empty((H, M), dtype=torch.float32, device=q.device) if want_lse else None
+    lse = torch.empty((H, M), dtype=torch.float32, device=q.device) if for_backward else None
+    rest = torch.empty_like(out) if for_backward and q.dtype is not torch.float32 else None
     n = lib.some_op_causal_attention_bytes(h, DTYPES[q.dtype], H, G, D, batch.B, M, N)
     work = torch.empty(n, dtype=torch.uint8, device=q.device) if n else None
     rc = lib.some_op_causal_attention(h, DTYPES[q.dtype], D, *_place(q), H, *_place(k), *_place(v), G, batch.frame_offsets_dev.data_ptr(),
                                       kv.frame_offsets_dev.data_ptr(), batch.B, M, N, causal, scale, out.data_ptr(), H * D, D,
-                                      lse.data_ptr() if want_lse else None, work.data_ptr() if n else None, n, stream)
+                                      rest.data_ptr() if rest is not None else None, lse.data_ptr() if for_backward else None, work.data_ptr() if n else None, n, stream)
     if rc:
         _lib.check(h, rc)
-    return out, lse
+    return out, rest, lse
 
 
-def attention_backward(lib, h, stream, q, k, v, batch, kv, causal, scale, out, lse, dout):
+def attention_backward(lib, h, stream, q, k, v, batch, kv, causal, scale, out, rest, lse, dout):
     dout = readable(dout)
     (M, H, D), (N, G, _) = q.shape, k.shape
     dq, dk, dv = q.new_empty((M, H, D)), k.new_empty((N, G, D)), v.new_empty((N, G, D))
     n = lib.some_train_causal_attention_bytes(h, DTYPES[q.dtype], H, G, D, batch.B, M, N)
     work = torch.empty(n, dtype=torch.uint8, device=q.device)
     rc = lib.some_train_causal_attention_bwd(h, DTYPES[q.dtype], D, *_place(q), H, *_place(k), *_place(v), G, batch.frame_offsets_dev.data_ptr(),
-                                             kv.frame_offsets_dev.data_ptr(), batch.B, M, N, causal, scale, out.data_ptr(), H * D, D, lse.data_ptr(),
+                                             kv.frame_offsets_dev.data_ptr(), batch.B, M, N, causal, scale, out.data_ptr(), H * D, D,
+                                             rest.data_ptr() if rest is not None else None, lse.data_ptr(),
                                              *_place(dout), dq.data_ptr(), H * D, D, dk.data_ptr(), G * D, D, dv.data_ptr(), G * D, D, work.data_ptr(), n,
                                              stream)
     if rc:

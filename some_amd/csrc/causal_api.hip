@@ -19,6 +19,7 @@ int cfail(SomeHandle* h, int code, const char* fn, const char* msg) {
     } while (0)
 
 constexpr int64_t kMaxRows = (int64_t)1 << 29;
+constexpr int64_t kMaxBlocks = ((int64_t)1 << 24) - 1;       // a launch has fewer than 2^32 threads a dimension; blocks are of 256
 constexpr int kMaxHeads = 1024;
 
 // 16-byte aligned rows and heads; a tile of 128 rows stays inside 31 bits
@@ -76,7 +77,7 @@ int some_op_qk_norm_rope(SomeHandle* h, int32_t dtype, int32_t head_dim, const v
     C_CHECK(fill_turns(a, theta, head_dim), "theta must be finite and positive");
     a.gamma_q = gamma_q_dev; a.gamma_k = gamma_k_dev; a.positions = positions_dev; a.positions64 = positions64;
     a.rows = rows; a.heads = heads; a.kv_heads = kv_heads; a.eps = eps;
-    C_CHECK(rows * (heads + kv_heads) * (head_dim / 16) / 256 < 0x7ffffff0ll, "too many rows");
+    C_CHECK(norm_rope_blocks(rows, heads, kv_heads, head_dim) <= kMaxBlocks, "too many rows and heads for one launch");
     C_TRY(launch_norm_rope(dtype, head_dim, a, static_cast<hipStream_t>(stream)));
     return SOME_OK;
 }
@@ -85,7 +86,7 @@ size_t some_train_qk_norm_rope_bytes(const SomeHandle* h, int64_t rows, int32_t 
     (void)h;
     if (rows < 0 || rows >= kMaxRows || heads <= 0 || kv_heads <= 0 || (head_dim != 64 && head_dim != 128)) return 256;
     const size_t n = (size_t)norm_rope_bwd_blocks(rows, heads, kv_heads, head_dim) * head_dim * sizeof(float);
-    return n < 256 ? 256 : n;
+    return n < 1024 ? 1024 : n;
 }
 
 int some_train_qk_norm_rope_bwd(SomeHandle* h, int32_t dtype, int32_t head_dim, const void* q_dev, int64_t q_row, int64_t q_head, int32_t heads,
@@ -141,8 +142,8 @@ size_t some_train_causal_attention_bytes(const SomeHandle* h, int32_t dtype, int
 int some_op_causal_attention(SomeHandle* h, int32_t dtype, int32_t head_dim, const void* q_dev, int64_t q_row, int64_t q_head, int32_t heads,
                              const void* k_dev, int64_t k_row, int64_t k_head, const void* v_dev, int64_t v_row, int64_t v_head, int32_t kv_heads,
                              const int32_t* q_offsets_dev, const int32_t* k_offsets_dev, int32_t B, int64_t q_rows, int64_t k_rows, int32_t causal,
-                             float scale, void* out_dev, int64_t o_row, int64_t o_head, float* lse_dev, void* workspace_dev, size_t workspace_bytes,
-                             void* stream) {
+                             float scale, void* out_dev, int64_t o_row, int64_t o_head, void* rest_dev, float* lse_dev, void* workspace_dev,
+                             size_t workspace_bytes, void* stream) {
     if (!h) return SOME_EINVAL;
     C_CHECK(type_ok(dtype, head_dim), kType);
     C_CHECK(heads_ok(heads, kv_heads), kHeadsMsg);
@@ -153,7 +154,8 @@ int some_op_causal_attention(SomeHandle* h, int32_t dtype, int32_t head_dim, con
     CausalArgs a{};
     a.q = rows3(q_dev, q_row, q_head); a.k = rows3(k_dev, k_row, k_head); a.v = rows3(v_dev, v_row, v_head); a.out = rows3(out_dev, o_row, o_head);
     C_CHECK(laid_out(dtype, a.q) && laid_out(dtype, a.k) && laid_out(dtype, a.v) && laid_out(dtype, a.out), kLayout);
-    a.lse = lse_dev; a.q_offsets = q_offsets_dev; a.k_offsets = k_offsets_dev; a.q_rows = q_rows;
+    C_CHECK((reinterpret_cast<uintptr_t>(rest_dev) & 15) == 0, "rest must be 16-byte aligned");
+    a.rest = dtype ? rest_dev : nullptr; a.lse = lse_dev; a.q_offsets = q_offsets_dev; a.k_offsets = k_offsets_dev; a.q_rows = q_rows;
     a.B = B; a.kv_heads = kv_heads; a.group = heads / kv_heads; a.causal = causal; a.scale = scale;
     a.parts = k_rows > 0 ? causal_fwd_parts(dtype, q_rows, k_rows, B, heads, kv_heads) : 1;
     if (a.parts > 1) {
@@ -163,7 +165,7 @@ int some_op_causal_attention(SomeHandle* h, int32_t dtype, int32_t head_dim, con
         a.part_o = static_cast<float*>(workspace_dev);
         a.part_ml = a.part_o + (int64_t)a.parts * q_rows * heads * head_dim;
     }
-    C_CHECK(q_rows * a.group < 0x7fffffffll && causal_fwd_blocks(a) < 0x7fffffffll, "too many rows, clips and heads for one launch");
+    C_CHECK(q_rows * a.group < 0x7fffffffll && causal_fwd_blocks(a) <= kMaxBlocks, "too many rows, clips and heads for one launch");
     C_TRY(launch_causal_fwd(dtype, head_dim, a, static_cast<hipStream_t>(stream)));
     return SOME_OK;
 }
@@ -171,8 +173,8 @@ int some_op_causal_attention(SomeHandle* h, int32_t dtype, int32_t head_dim, con
 int some_train_causal_attention_bwd(SomeHandle* h, int32_t dtype, int32_t head_dim, const void* q_dev, int64_t q_row, int64_t q_head, int32_t heads,
                                     const void* k_dev, int64_t k_row, int64_t k_head, const void* v_dev, int64_t v_row, int64_t v_head, int32_t kv_heads,
                                     const int32_t* q_offsets_dev, const int32_t* k_offsets_dev, int32_t B, int64_t q_rows, int64_t k_rows, int32_t causal,
-                                    float scale, const void* out_dev, int64_t o_row, int64_t o_head, const float* lse_dev, const void* dout_dev,
-                                    int64_t do_row, int64_t do_head, void* dq_dev, int64_t dq_row, int64_t dq_head, void* dk_dev, int64_t dk_row,
+                                    float scale, const void* out_dev, int64_t o_row, int64_t o_head, const void* rest_dev, const float* lse_dev,
+                                    const void* dout_dev, int64_t do_row, int64_t do_head, void* dq_dev, int64_t dq_row, int64_t dq_head, void* dk_dev, int64_t dk_row,
                                     int64_t dk_head, void* dv_dev, int64_t dv_row, int64_t dv_head, void* workspace_dev, size_t workspace_bytes, void* stream) {
     if (!h) return SOME_EINVAL;
     C_CHECK(type_ok(dtype, head_dim), kType);
@@ -189,7 +191,8 @@ int some_train_causal_attention_bwd(SomeHandle* h, int32_t dtype, int32_t head_d
     b.dout = rows3(dout_dev, do_row, do_head); b.dq = rows3(dq_dev, dq_row, dq_head); b.dk = rows3(dk_dev, dk_row, dk_head); b.dv = rows3(dv_dev, dv_row, dv_head);
     C_CHECK(laid_out(dtype, a.q) && laid_out(dtype, a.k) && laid_out(dtype, a.v) && laid_out(dtype, a.out) && laid_out(dtype, b.dout) && laid_out(dtype, b.dq) &&
             laid_out(dtype, b.dk) && laid_out(dtype, b.dv), kLayout);
-    a.lse = const_cast<float*>(lse_dev); a.q_offsets = q_offsets_dev; a.k_offsets = k_offsets_dev; a.q_rows = q_rows;
+    C_CHECK((reinterpret_cast<uintptr_t>(rest_dev) & 15) == 0, "rest must be 16-byte aligned");
+    a.rest = dtype ? const_cast<void*>(rest_dev) : nullptr; a.lse = const_cast<float*>(lse_dev); a.q_offsets = q_offsets_dev; a.k_offsets = k_offsets_dev; a.q_rows = q_rows;
     a.B = B; a.kv_heads = kv_heads; a.group = heads / kv_heads; a.causal = causal; a.scale = scale;
     a.parts = k_rows > 0 ? causal_fwd_parts(dtype, q_rows, k_rows, B, heads, kv_heads) : 1;
     b.k_rows = k_rows;
@@ -200,7 +203,8 @@ int some_train_causal_attention_bwd(SomeHandle* h, int32_t dtype, int32_t head_d
     b.dsum = static_cast<float*>(workspace_dev);
     b.part_q = b.part_k = reinterpret_cast<float*>(static_cast<char*>(workspace_dev) + dsum_bytes(heads, q_rows));
     b.part_v = b.part_k + (int64_t)b.parts * k_rows * kv_heads * head_dim;
-    C_CHECK(q_rows * a.group < 0x7fffffffll && causal_fwd_blocks(a) < 0x7fffffffll && causal_bwd_blocks(b) < 0x7fffffffll && k_rows * kv_heads * (head_dim / 4) / 256 < 0x7ffffff0ll, "too many rows, clips and heads for one launch");
+    C_CHECK(q_rows * a.group < 0x7fffffffll && causal_fwd_blocks(a) <= kMaxBlocks && causal_bwd_blocks(b) <= kMaxBlocks,
+            "too many rows, clips and heads for one launch");
     C_TRY(launch_causal_bwd(dtype, head_dim, b, static_cast<hipStream_t>(stream)));
     return SOME_OK;
 }
@@ -239,7 +243,7 @@ int some_op_attention_step(SomeHandle* h, int32_t dtype, int32_t head_dim, const
     a.k_batch = k_batch; a.v_batch = v_batch; a.lengths = lengths_dev; a.B = B; a.capacity = max_length;
     a.kv_heads = kv_heads; a.group = heads / kv_heads; a.scale = scale;
     a.chunks = step_chunks(B, kv_heads, a.group, max_length, &a.chunk);
-    C_CHECK((int64_t)a.chunks * B * kv_heads * ((a.group + 31) / 32) < 0x7fffffffll && (int64_t)heads * B < 0x7fffffffll, "too many streams and heads for one launch");
+    C_CHECK((int64_t)a.chunks * B * kv_heads * ((a.group + 31) / 32) <= kMaxBlocks, "too many streams and heads for one launch");
     if (a.chunks > 1) {
         if (!workspace_dev || workspace_bytes < some_op_attention_step_bytes(h, B, heads, kv_heads, head_dim, max_length))
             return cfail(h, SOME_ENOMEM, __func__, "workspace too small (some_op_attention_step_bytes)");

@@ -73,11 +73,13 @@ __global__ __launch_bounds__(256, (D == 64 ? (sizeof(T) == 2 ? 4 : 2) : sizeof(T
     for (int ks = 0; ks < KS; ++ks) {
         qfr[ks] = load8<T>(qrow + 16 * ks);
         gfr[ks] = load8<T>(grow + 16 * ks);
-        const frag of = load8<T>(orow + 16 * ks);
+        dsum += dot8<T>(gfr[ks], load8<T>(orow + 16 * ks));
+    }
+    if constexpr (sizeof(T) == 2) {
+        if (a.rest) {
+            const T* rrow = static_cast<const T*>(a.rest) + (qr * a.kv_heads * G + head) * D + 8 * hi;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            if constexpr (sizeof(T) == 4) dsum = fmaf(gfr[ks][j], of[j], dsum);
-            else dsum = fmaf((float)__builtin_bit_cast(T, (short)gfr[ks][j]), (float)__builtin_bit_cast(T, (short)of[j]), dsum);
+            for (int ks = 0; ks < KS; ++ks) dsum = fmaf(dot8<T>(gfr[ks], load8<T>(rrow + 16 * ks)), 1.f / kRestScale<T>, dsum);
         }
     }
     dsum = halves_sum(dsum);

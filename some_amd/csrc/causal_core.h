@@ -128,6 +128,18 @@ template <typename T> __device__ __forceinline__ void store4(T* p, float a, floa
     }
 }
 
+// What a 16-bit type loses of x, to be kept in a second value of that type (f16: times 2^10, as it would be subnormal otherwise; never beyond x in size).
+// D = rowsum(dO O) needs it: every key of a row gets D's error, and where a row sees few keys dP - D is far smaller than its terms - with D from the rounded
+// O alone the gradients of clips of two frames are off by 5.6e-3 in bf16, with the rest by 2.4e-3, of which dS's own rounding is 2.3e-3.
+template <typename T> constexpr float kRestScale = __is_same(T, f16_t) ? 1024.f : 1.f;
+template <typename T> __device__ __forceinline__ float rest_of(float x) {
+    const float r = x - (float)(T)x;
+    return r - r == 0.f ? r * kRestScale<T> : 0.f;           // (x not finite: nothing)
+}
+template <typename T> __device__ __forceinline__ void store4_rest(T* p, float a, float b, float c, float d) {
+    store4<T>(p, rest_of<T>(a), rest_of<T>(b), rest_of<T>(c), rest_of<T>(d));
+}
+
 // ---- LDS tiles: ROWS rows of D values, row pitch D sizeof(T) bytes, 16-byte chunk c of row r stored at chunk c ^ swz(r) --------------------
 // The copy global -> LDS writes lane-linear chunks, so the permutation is applied to its per-lane source address.  swz is chosen so that both
 // reads touch every LDS bank equally often: row fragments (32 rows, one chunk) and column fragments (ds_read_b64_tr_b16: 8 rows x 64 bytes; f32:
@@ -244,6 +256,16 @@ __device__ __forceinline__ void solo_column(float (&acc)[(D + 63) / 64], int r0,
             for (int e = 0; e < (D + 63) / 64; ++e) acc[e] = fmaf(wj, to_f32(m[(int64_t)(base + j) * stride + lane + 64 * e]), acc[e]);
         }
     }
+}
+
+template <typename T> __device__ __forceinline__ float dot8(typename Frag<T>::type x, typename Frag<T>::type y) {
+    float s = 0.f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        if constexpr (sizeof(T) == 4) s = fmaf(x[j], y[j], s);
+        else s = fmaf((float)__builtin_bit_cast(T, (short)x[j]), (float)__builtin_bit_cast(T, (short)y[j]), s);
+    }
+    return s;
 }
 
 // ---- block map ------------------------------------------------------------------------------------------------------------------------

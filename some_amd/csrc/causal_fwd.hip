@@ -180,6 +180,13 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 && D == 64 ? 4 : 2)) void caus
                 T* orow = static_cast<T*>(a.out.p) + (int64_t)(qf + qn) * a.out.row + (int64_t)hd * a.out.head;
                 orow[lane] = (T)(o0 * inv);
                 if (D > 64) orow[64 + lane] = (T)(o1 * inv);
+                if constexpr (sizeof(T) == 2) {
+                    if (a.rest) {
+                        T* rrow = static_cast<T*>(a.rest) + ((int64_t)(qf + qn) * a.kv_heads * G + hd) * D;
+                        rrow[lane] = (T)rest_of<T>(o0 * inv);
+                        if (D > 64) rrow[64 + lane] = (T)rest_of<T>(o1 * inv);
+                    }
+                }
                 if (a.lse && lane == 0) a.lse[(int64_t)hd * a.q_rows + qf + qn] = limit >= 0 ? mm * c2 + log2_(ll) : -INFINITY;
             }
         }
@@ -204,6 +211,16 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 && D == 64 ? 4 : 2)) void caus
 #pragma unroll
             for (int r4 = 0; r4 < 4; ++r4)
                 store4<T>(orow + 32 * d + 8 * r4 + 4 * hi, o[d][4 * r4] * inv, o[d][4 * r4 + 1] * inv, o[d][4 * r4 + 2] * inv, o[d][4 * r4 + 3] * inv);
+        if constexpr (sizeof(T) == 2) {
+            if (a.rest) {
+                T* rrow = static_cast<T*>(a.rest) + ((int64_t)(qf + q) * a.kv_heads * G + head) * D;
+#pragma unroll
+                for (int d = 0; d < DB; ++d)
+#pragma unroll
+                    for (int r4 = 0; r4 < 4; ++r4)
+                        store4_rest<T>(rrow + 32 * d + 8 * r4 + 4 * hi, o[d][4 * r4] * inv, o[d][4 * r4 + 1] * inv, o[d][4 * r4 + 2] * inv, o[d][4 * r4 + 3] * inv);
+            }
+        }
         if (a.lse && hi == 0) a.lse[(int64_t)head * a.q_rows + qf + q] = any ? m * c2 + log2_(sum) : -INFINITY;
     }
 }
@@ -249,6 +266,9 @@ template <typename T, int D> __global__ __launch_bounds__(256) void causal_join_
     }
     const float inv = any ? 1.f / sum : 0.f;
     store4<T>(static_cast<T*>(a.out.p) + row * a.out.row + (int64_t)h * a.out.head + d, acc[0] * inv, acc[1] * inv, acc[2] * inv, acc[3] * inv);
+    if constexpr (sizeof(T) == 2) {
+        if (a.rest) store4_rest<T>(static_cast<T*>(a.rest) + i0 * D + d, acc[0] * inv, acc[1] * inv, acc[2] * inv, acc[3] * inv);
+    }
     if (a.lse && d == 0) a.lse[(int64_t)h * a.q_rows + row] = any ? m + log2_(sum) : -INFINITY;
 }
 

@@ -174,6 +174,7 @@ hipError_t launch_attn_plan(const int32_t* frame_offsets, int B, int rows_cover,
 struct Rows3 { void* p; int64_t row, head; };
 struct CausalArgs {
     Rows3 q, k, v, out;
+    void* rest;                    // optional, 16-bit types: [q_rows, heads, head_dim] what rounding took from out (causal_core.h, rest_of)
     float* lse;                    // optional [heads, q_rows]: base-2 log-sum-exp of the scaled scores (-inf: no visible key)
     const int32_t* q_offsets; const int32_t* k_offsets;
     int64_t q_rows;
@@ -211,6 +212,7 @@ struct NormRopeArgs {
     float eps;
     double turns[64];              // theta^(-2 i / head_dim) / (2 pi)
 };
+int64_t norm_rope_blocks(int64_t rows, int heads, int kv_heads, int head_dim);
 int norm_rope_bwd_blocks(int64_t rows, int heads, int kv_heads, int head_dim);
 hipError_t launch_norm_rope(int dtype, int head_dim, NormRopeArgs a, hipStream_t s);
 hipError_t launch_norm_rope_bwd(int dtype, int head_dim, NormRopeArgs a, float* dgq, float* dgk, int accumulate, hipStream_t s);

@@ -220,6 +220,14 @@ constexpr int64_t kBwdBlocks = 1536;                         // two rounds of wh
 
 }  // namespace
 
+int64_t norm_rope_blocks(int64_t rows, int heads, int kv_heads, int head_dim) {
+    NormRopeArgs a;
+    a.rows = rows;
+    a.heads = heads;
+    a.kv_heads = kv_heads;
+    return share(a, head_dim, 2, (int64_t)1 << 40);
+}
+
 int norm_rope_bwd_blocks(int64_t rows, int heads, int kv_heads, int head_dim) {
     NormRopeArgs a;
     a.rows = rows;

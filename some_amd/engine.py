@@ -342,7 +342,7 @@ class Engine:
         causal.no_gradient_lost('Engine.causal_attention', q, k, v)
         scale = causal.default_scale(scale, q3.shape[2])
         with causal.on_device(q3):
-            out, _ = causal.attention_forward(lib, h, causal.stream_of(q3), causal.readable(q3), causal.readable(k3), causal.readable(v3), batch, kv,
+            out, _, _ = causal.attention_forward(lib, h, causal.stream_of(q3), causal.readable(q3), causal.readable(k3), causal.readable(v3), batch, kv,
                                               bool(causal_mask), scale, False)
         return out if q3 is q else out.view(q.shape)
 

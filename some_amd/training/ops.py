@@ -1290,7 +1290,7 @@ class _QkNormRope(torch.autograd.Function):
 
 
 class _CausalAttention(torch.autograd.Function):
-    """Forward keeps q, k, v, the output and the log-sum-exp; backward recomputes the probabilities (csrc/causal_bwd.hip)."""
+    """Forward keeps q, k, v, the output (in 16-bit types with what its rounding took) and the log-sum-exp; backward recomputes the probabilities (csrc/causal_bwd.hip)."""
 
     @staticmethod
     def forward(ctx, ops, q, k, v, batch, kv, causal_mask, scale, head_dim):
@@ -1298,19 +1298,19 @@ class _CausalAttention(torch.autograd.Function):
         flat = q3 is not q
         q3, k3, v3 = causal.readable(q3), causal.readable(k3), causal.readable(v3)
         with causal.on_device(q3):
-            out, lse = causal.attention_forward(ops.lib, ops.h, _stream_for(ops, q3), q3, k3, v3, batch, kv, causal_mask, scale, True)
+            out, rest, lse = causal.attention_forward(ops.lib, ops.h, _stream_for(ops, q3), q3, k3, v3, batch, kv, causal_mask, scale, True)
         ctx.ops, ctx.batch, ctx.kv, ctx.causal_mask, ctx.scale = ops, batch, kv, causal_mask, scale
         ctx.shapes = q.shape, k.shape, v.shape
-        ctx.save_for_backward(q3, k3, v3, out, lse)
+        ctx.save_for_backward(q3, k3, v3, out, rest, lse)
         return out.view(q.shape) if flat else out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
         ops: TrainOps = ctx.ops
-        q, k, v, out, lse = ctx.saved_tensors
+        q, k, v, out, rest, lse = ctx.saved_tensors
         with causal.on_device(q):
-            grads = causal.attention_backward(ops.lib, ops.h, _stream_for(ops, q), q, k, v, ctx.batch, ctx.kv, ctx.causal_mask, ctx.scale, out.view(q.shape), lse,
+            grads = causal.attention_backward(ops.lib, ops.h, _stream_for(ops, q), q, k, v, ctx.batch, ctx.kv, ctx.causal_mask, ctx.scale, out.view(q.shape), rest, lse,
                                               dout if dout.dim() == 3 else dout.reshape(q.shape))
         dq, dk, dv = (g if len(s) == 3 else g.view(s) for g, s in zip(grads, ctx.shapes))
         return None, dq, dk, dv, None, None, None, None, None

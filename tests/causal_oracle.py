@@ -86,8 +86,9 @@ def attention(q, k, v, q_lens, k_lens, causal=True, scale=None, dout=None):
                 dp = do @ vs.t()
                 dsum = (do * o).sum(-1, keepdim=True)
                 ds = p * (dp - dsum)
-                # dS: the saved output's rounding in D, fp32 sums of dP and D, the recomputed probability, its own rounding
-                errd = (e + 2 * rel + 4 * math.sqrt(D) * U) * (do.abs() * (p @ vs.abs())).sum(-1, keepdim=True)
+                # dS: the probabilities' rounding in the output that D is made of (the output's own is kept), fp32 sums of dP and D, the
+                # recomputed probability, its own rounding
+                errd = (ep + e * e + 2 * rel + 4 * math.sqrt(D) * U) * (do.abs() * (p @ vs.abs())).sum(-1, keepdim=True)
                 errp = 4 * math.sqrt(D) * U * (do.abs() @ vs.abs().t())
                 eds = p * (errd + errp) + (ep + 2 * rel) * ds.abs()
                 acc = 4 * math.sqrt(max(t, n * R)) * U

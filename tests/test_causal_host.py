@@ -95,12 +95,12 @@ def test_c_abi_refuses():
     eng = Engine(get_config('two_head_model', lay=0), host_only=True)
     h, p = eng.handle, C.c_void_p(4096)                   # never dereferenced: every call below fails validation
 
-    def attn(dtype=2, D=64, q=p, qs=(256, 64), H=4, k=p, ks=(128, 64), G=2, off=p, B=1, M=10, N=10, scale=0.125, out=p, work=0):
-        return lib.some_op_causal_attention(h, dtype, D, q, *qs, H, k, *ks, k, *ks, G, off, off, B, M, N, 1, scale, out, *qs, None, p if work else None, work, None)
+    def attn(dtype=2, D=64, q=p, qs=(256, 64), H=4, k=p, ks=(128, 64), G=2, off=p, B=1, M=10, N=10, scale=0.125, out=p, work=0, rest=None):
+        return lib.some_op_causal_attention(h, dtype, D, q, *qs, H, k, *ks, k, *ks, G, off, off, B, M, N, 1, scale, out, *qs, rest, None, p if work else None, work, None)
 
-    def bwd(dtype=2, D=64, H=4, G=2, work=p, n=1 << 30, N=10, scale=0.125, ds=(256, 64)):
+    def bwd(dtype=2, D=64, H=4, G=2, work=p, n=1 << 30, N=10, scale=0.125, ds=(256, 64), rest=p):
         r = (p, 256, 64)
-        return lib.some_train_causal_attention_bwd(h, dtype, D, *r, H, *r, *r, G, p, p, 1, 10, N, 1, scale, *r, p, p, *ds, *r, *r, *r, work, n, None)
+        return lib.some_train_causal_attention_bwd(h, dtype, D, *r, H, *r, *r, G, p, p, 1, 10, N, 1, scale, *r, rest, p, p, *ds, *r, *r, *r, work, n, None)
 
     def step(dtype=2, D=64, H=4, G=2, B=3, m=2000, work=p, n=1 << 30, kb=128 * 2000, scale=0.125, lengths=p):
         return lib.some_op_attention_step(h, dtype, D, p, 256, 64, H, p, kb, 128, 64, p, kb, 128, 64, G, lengths, B, m, scale, p, 256, 64, work, n, None)
@@ -121,7 +121,7 @@ def test_c_abi_refuses():
              (attn, dict(B=1 << 28, H=1024, G=1), b'one launch'),
              (bwd, dict(dtype=5), b'dtype'), (bwd, dict(H=3), b'multiple'), (bwd, dict(work=None), b'null'), (bwd, dict(work=odd), b'aligned'), (bwd, dict(N=1 << 29), b'2^29'), (bwd, dict(scale=-1.0), b'scale'),
              (bwd, dict(ds=(255, 64)), b'aligned'),
-             (step, dict(dtype=3), b'dtype'), (step, dict(H=5), b'multiple'), (step, dict(B=65536), b'65535'), (step, dict(B=-1), b'65535'), (step, dict(m=-1), b'max_length'),
+             (step, dict(dtype=3), b'dtype'), (step, dict(H=5), b'multiple'), (step, dict(B=65536), b'65535'), (step, dict(B=65535, H=1024, G=1024, m=1), b'one launch'), (rope, dict(rows=(1 << 29) - 1, H=1024, G=1), b'one launch'), (step, dict(B=-1), b'65535'), (step, dict(m=-1), b'max_length'),
              (step, dict(kb=4), b'aligned'), (step, dict(kb=-128), b'aligned'), (step, dict(lengths=None), b'null'), (step, dict(scale=0.0), b'scale'), (step, dict(work=odd), b'aligned'),
              (rope, dict(D=32), b'head_dim'), (rope, dict(H=0), b'heads'), (rope, dict(rows=-1), b'rows'), (rope, dict(pos=None), b'null'),
              (rope, dict(pos=C.c_void_p(4100), p64=1), b'positions'), (rope, dict(theta=0.0), b'theta'), (rope, dict(theta=float('inf')), b'theta'),
@@ -131,6 +131,7 @@ def test_c_abi_refuses():
         assert msg in lib.some_last_error(h), (fn.__name__, kw, lib.some_last_error(h))
     assert step(n=16) == _lib.SOME_ENOMEM and b'workspace' in lib.some_last_error(h)
     assert step(work=None) == _lib.SOME_ENOMEM
+    assert attn(rest=odd) == bwd(rest=odd) == _lib.SOME_EINVAL and b'rest must be' in lib.some_last_error(h)
     assert bwd(n=16) == _lib.SOME_ENOMEM and b'workspace' in lib.some_last_error(h)
     assert attn(N=100000) == _lib.SOME_ENOMEM and attn(N=100000, work=4096) == _lib.SOME_ENOMEM         # few queries over many keys: cut into parts
     assert lib.some_op_causal_attention_bytes(h, 2, 4, 2, 64, 1, 10, 100000) > 0 == lib.some_op_causal_attention_bytes(h, 2, 8, 8, 64, 32, 82688, 82688)

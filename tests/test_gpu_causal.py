@@ -236,6 +236,24 @@ def test_attention_is_blind_to_masked_places(eng, dtype, D, bad, clips):
             assert torch.isnan(got[at:end]).all()
 
 
+@pytest.mark.parametrize('dtype', [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize('D', [64, 128])
+@pytest.mark.parametrize('frames,past', [(2, 0), (3, 0), (1, 1), (2, 3000)])
+def test_gradients_of_short_clips_keep_their_precision(ops, dtype, D, frames, past):
+    """A row of few keys: dP - D is far smaller than its two terms, so D must not come from the rounded output alone.  Three independent roundings (the
+    probabilities, dS, the result), each of a relative mean square of at most (half step)^2 / 3, leave a relative mean square of (half step)^2."""
+    ql, H = [frames] * 60, 2
+    kl = [frames + past] * 60
+    q, k, v = _qkv(141, sum(ql), sum(kl), H, H, D, dtype)
+    dout = _normal(145, sum(ql), H, D, dtype=dtype)
+    leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+    grads = torch.autograd.grad(ops.causal_attention(*leaves, _batch(ql), kv_batch=_batch(kl)), leaves, dout)
+    w = oracle.attention(q, k, v, ql, kl, dout=dout)
+    for name, got, want in zip(('dq', 'dk', 'dv'), grads, w[2::2]):
+        off = ((got.double() - want).pow(2).sum() / want.pow(2).sum()).sqrt().item()
+        assert off < oracle.half_step(dtype), (name, off)
+
+
 @pytest.mark.parametrize('magnitude', [1e-7, 1e-3, 1.0, 3e4])
 @pytest.mark.parametrize('clips', [0, 640])
 def test_half_precision_gradients_of_any_magnitude(ops, magnitude, clips):
@@ -297,19 +315,19 @@ def test_rows_behind_the_last_clip_stay(eng):
     lens, H, G, D, extra = [40, 100], 2, 1, 64, 13
     M = sum(lens)
     q, k, v = _qkv(91, M + extra, M + extra, H, G, D, torch.bfloat16)
-    out = torch.full_like(q, 7.0)
+    out, rest = torch.full_like(q, 7.0), torch.full_like(q, 7.0)
     lse = torch.full((H, M + extra), 7.0, device='cuda')
     b = _batch(lens)
     lib, h = _lib.fast(), eng.handle.value
     st = torch.cuda.current_stream().cuda_stream
     s3 = lambda t: (t.data_ptr(), t.stride(0), t.stride(1))          # noqa: E731
     off = b.frame_offsets_dev.data_ptr()
-    _lib.check(h, lib.some_op_causal_attention(h, 2, D, *s3(q), H, *s3(k), *s3(v), G, off, off, b.B, M + extra, M + extra, 1, 0.125, *s3(out), lse.data_ptr(), None, 0, st))
-    assert (out[M:] == 7).all() and (lse[:, M:] == 7).all()
+    _lib.check(h, lib.some_op_causal_attention(h, 2, D, *s3(q), H, *s3(k), *s3(v), G, off, off, b.B, M + extra, M + extra, 1, 0.125, *s3(out), rest.data_ptr(), lse.data_ptr(), None, 0, st))
+    assert (out[M:] == 7).all() and (rest[M:] == 7).all() and (lse[:, M:] == 7).all()
     assert torch.equal(out[:M], eng.causal_attention(q[:M], k[:M], v[:M], b))
     dout, work = torch.ones_like(q), torch.empty(1 << 24, dtype=torch.uint8, device='cuda')
     d = [torch.full_like(t, 7.0) for t in (q, k, v)]
-    _lib.check(h, lib.some_train_causal_attention_bwd(h, 2, D, *s3(q), H, *s3(k), *s3(v), G, off, off, b.B, M + extra, M + extra, 1, 0.125, *s3(out), lse.data_ptr(),
+    _lib.check(h, lib.some_train_causal_attention_bwd(h, 2, D, *s3(q), H, *s3(k), *s3(v), G, off, off, b.B, M + extra, M + extra, 1, 0.125, *s3(out), rest.data_ptr(), lse.data_ptr(),
                                                       *s3(dout), *s3(d[0]), *s3(d[1]), *s3(d[2]), work.data_ptr(), work.numel(), st))
     assert all((t[M:] == 7).all() for t in d) and not any((t[:M] == 7).all() for t in d)
 
