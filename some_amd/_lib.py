@@ -148,7 +148,7 @@ SYMBOLS = {
     'some_train_causal_attention_bwd': (C.c_int, [_P, C.c_int32, C.c_int32, _P, C.c_int64, C.c_int64, C.c_int32, _P, C.c_int64, C.c_int64, _P, C.c_int64, C.c_int64, C.c_int32, _P, _P,
                                                   C.c_int32, C.c_int64, C.c_int64, C.c_int32, C.c_float, _P, C.c_int64, C.c_int64, _P, _P, _P, C.c_int64, C.c_int64, _P, C.c_int64, C.c_int64, _P, C.c_int64, C.c_int64,
                                                   _P, C.c_int64, C.c_int64, _P, C.c_size_t, _P]),
-    'some_op_attention_step_bytes': (C.c_size_t, [_P, C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_int32]),
+    'some_op_attention_step_bytes': (C.c_size_t, [_P, C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_int32]),
     'some_op_attention_step': (C.c_int, [_P, C.c_int32, C.c_int32, _P, C.c_int64, C.c_int64, C.c_int32, _P, C.c_int64, C.c_int64, C.c_int64, _P, C.c_int64, C.c_int64,
                                          C.c_int64, C.c_int32, _P, C.c_int32, C.c_int32, C.c_float, _P, C.c_int64, C.c_int64, _P, C.c_size_t, _P]),
     'some_profile_enable': (C.c_int, [_P, C.c_int32]),

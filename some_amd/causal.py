@@ -243,10 +243,10 @@ def attention_step(lib, h, stream, q, places, G, lengths, max_length, scale):
     q, lengths = readable(q), lengths.contiguous()
     B, H, D = q.shape
     out = q.new_empty((B, H, D))
-    n = lib.some_op_attention_step_bytes(h, B, H, G, D, max_length)
-    work = torch.empty(n, dtype=torch.uint8, device=q.device)
+    n = lib.some_op_attention_step_bytes(h, DTYPES[q.dtype], B, H, G, D, max_length)
+    work = torch.empty(n, dtype=torch.uint8, device=q.device) if n else None
     rc = lib.some_op_attention_step(h, DTYPES[q.dtype], D, *_place(q), H, *places, G, lengths.data_ptr(), B, max_length, scale, out.data_ptr(), H * D, D,
-                                    work.data_ptr(), n, stream)
+                                    work.data_ptr() if n else None, n, stream)
     if rc:
         _lib.check(h, rc)
     return out

@@ -209,18 +209,11 @@ int some_train_causal_attention_bwd(SomeHandle* h, int32_t dtype, int32_t head_d
     return SOME_OK;
 }
 
-static int step_chunks(int B, int kv_heads, int group, int max_len, int* chunk) {
-    *chunk = step_chunk(B, kv_heads, group, max_len);
-    const int n = (max_len + *chunk - 1) / *chunk;
-    return n < 1 ? 1 : n;
-}
-
-size_t some_op_attention_step_bytes(const SomeHandle* h, int32_t B, int32_t heads, int32_t kv_heads, int32_t head_dim, int32_t max_length) {
+size_t some_op_attention_step_bytes(const SomeHandle* h, int32_t dtype, int32_t B, int32_t heads, int32_t kv_heads, int32_t head_dim, int32_t max_length) {
     (void)h;
-    int chunk;
     if (B <= 0 || !heads_ok(heads, kv_heads) || head_dim <= 0 || max_length <= 0) return 256;
-    const int n = step_chunks(B, kv_heads, heads / kv_heads, max_length, &chunk);
-    return n > 1 ? (size_t)B * heads * n * (head_dim + 2) * sizeof(float) : 256;
+    const int n = step_plan(dtype, head_dim, B, kv_heads, heads / kv_heads, max_length).chunks;
+    return n > 1 ? (size_t)B * heads * n * (head_dim + 2) * sizeof(float) : 0;
 }
 
 int some_op_attention_step(SomeHandle* h, int32_t dtype, int32_t head_dim, const void* q_dev, int64_t q_row, int64_t q_head, int32_t heads,
@@ -242,10 +235,11 @@ int some_op_attention_step(SomeHandle* h, int32_t dtype, int32_t head_dim, const
     C_CHECK(k_batch >= 0 && v_batch >= 0 && (k_batch * size) % 16 == 0 && (v_batch * size) % 16 == 0, kLayout);
     a.k_batch = k_batch; a.v_batch = v_batch; a.lengths = lengths_dev; a.B = B; a.capacity = max_length;
     a.kv_heads = kv_heads; a.group = heads / kv_heads; a.scale = scale;
-    a.chunks = step_chunks(B, kv_heads, a.group, max_length, &a.chunk);
+    const StepPlan plan = step_plan(dtype, head_dim, B, kv_heads, a.group, max_length);
+    a.chunk = plan.chunk; a.chunks = plan.chunks;
     C_CHECK((int64_t)a.chunks * B * kv_heads * ((a.group + 31) / 32) <= kMaxBlocks, "too many streams and heads for one launch");
     if (a.chunks > 1) {
-        if (!workspace_dev || workspace_bytes < some_op_attention_step_bytes(h, B, heads, kv_heads, head_dim, max_length))
+        if (!workspace_dev || workspace_bytes < some_op_attention_step_bytes(h, dtype, B, heads, kv_heads, head_dim, max_length))
             return cfail(h, SOME_ENOMEM, __func__, "workspace too small (some_op_attention_step_bytes)");
         C_CHECK((reinterpret_cast<uintptr_t>(workspace_dev) & 15) == 0, "workspace must be 16-byte aligned");
         a.part_o = static_cast<float*>(workspace_dev);

@@ -199,7 +199,8 @@ struct StepArgs {
     int B, capacity, kv_heads, group, chunk, chunks;
     float scale;
 };
-int step_chunk(int B, int kv_heads, int group, int max_len);
+struct StepPlan { int chunk, chunks; };
+StepPlan step_plan(int dtype, int head_dim, int B, int kv_heads, int group, int max_len);
 hipError_t launch_attention_step(int dtype, int head_dim, const StepArgs& a, hipStream_t s);
 struct NormRopeArgs {
     Rows3 q, k, q_out, k_out;      // forward: x -> y; backward: x, dx

@@ -138,7 +138,7 @@ def test_c_abi_refuses():
     assert rope_bwd(n=16) == _lib.SOME_ENOMEM and b'scratch' in lib.some_last_error(h)
     # nothing to do: no launch, no error
     assert attn(M=0) == attn(B=0) == step(B=0) == rope(rows=0) == _lib.SOME_OK
-    assert lib.some_op_attention_step_bytes(h, 3, 4, 2, 64, 2000) >= 3 * 4 * 2 * 66 * 4
+    assert lib.some_op_attention_step_bytes(h, 2, 3, 4, 2, 64, 2000) >= 3 * 4 * 2 * 66 * 4
     for bad in ((0, 4, 2, 64, 10), (1, 3, 2, 64, 10), (1, 4, 0, 64, 10), (1, 4, 2, 64, 0)):
-        assert lib.some_op_attention_step_bytes(h, *bad) == 256
+        assert lib.some_op_attention_step_bytes(h, 2, *bad) == 256
     assert lib.some_train_qk_norm_rope_bytes(h, -1, 4, 2, 64) == 256 and lib.some_train_qk_norm_rope_bytes(h, 0, 4, 2, 64) >= 2 * 64 * 4
