@@ -601,3 +601,124 @@ def test_gradients_are_blind_to_masked_places(ops, dtype, D, clips):
         before = torch.ones(M, dtype=torch.bool, device='cuda')
         before[at:end] = False
         assert torch.isfinite(dq[before]).all() and (dq[before].double() - clean[0][before].double()).abs().max() <= scale[0]
+
+
+@pytest.mark.parametrize('dtype', TYPES)
+def test_rows_behind_the_last_clip_stay_where_parts_are_joined(eng, dtype):
+    """Few queries over many keys, offsets that begin and end inside the arrays: the joins write the clips' rows alone."""
+    import some_amd._lib as _lib
+    code, H, G, D, n, t, edge = TYPES.index(dtype), 4, 2, 64, 40, 3000, 5
+    lib, h = _lib.fast(), eng.handle.value
+    q, k, v = _qkv(401, n + 2 * edge, t + 2 * edge, H, G, D, dtype)
+    dout = _normal(405, n + 2 * edge, H, D, dtype=dtype)
+    qo = torch.tensor([edge, edge + 1, edge + n], dtype=torch.int32, device='cuda')
+    ko = torch.tensor([edge, edge + 1000, edge + t], dtype=torch.int32, device='cuda')
+    M, N = len(q), len(k)
+    s3 = lambda x: (x.data_ptr(), x.stride(0), x.stride(1))                                   # noqa: E731
+    out, rest, lse = torch.full_like(q, 7.0), torch.full_like(q, 7.0), torch.full((H, M), 7.0, device='cuda')
+    nb = lib.some_op_causal_attention_bytes(h, code, H, G, D, 2, M, N)
+    assert nb > 0
+    work = torch.full((lib.some_train_causal_attention_bytes(h, code, H, G, D, 2, M, N),), 255, dtype=torch.uint8, device='cuda')
+    st = torch.cuda.current_stream().cuda_stream
+    _lib.check(h, lib.some_op_causal_attention(h, code, D, *s3(q), H, *s3(k), *s3(v), G, qo.data_ptr(), ko.data_ptr(), 2, M, N, 1, 0.125, *s3(out), rest.data_ptr(),
+                                               lse.data_ptr(), work.data_ptr(), work.numel(), st))
+    d = [torch.full_like(x, 7.0) for x in (q, k, v)]
+    work.fill_(255)
+    _lib.check(h, lib.some_train_causal_attention_bwd(h, code, D, *s3(q), H, *s3(k), *s3(v), G, qo.data_ptr(), ko.data_ptr(), 2, M, N, 1, 0.125, *s3(out), rest.data_ptr(),
+                                                      lse.data_ptr(), *s3(dout), *s3(d[0]), *s3(d[1]), *s3(d[2]), work.data_ptr(), work.numel(), st))
+    for x in (out, *d) if dtype == torch.float32 else (out, rest, *d):
+        assert (x[:edge] == 7).all() and (x[-edge:] == 7).all()
+    assert (lse[:, :edge] == 7).all() and (lse[:, -edge:] == 7).all()
+    inner = [x[edge:-edge] for x in (q, k, v, dout)]
+    w = oracle.attention(*inner[:3], [1, n - 1], [1000, t - 1000], dout=inner[3])
+    for i, (name, got) in enumerate(zip(('out', 'dq', 'dk', 'dv'), (out, *d))):
+        oracle.check(got[edge:-edge], w[2 * i], w[2 * i + 1], name)
+
+
+def test_norm_rope_past_32_bit_offsets(ops):
+    n, H, D = 700, 2, 64
+    big = torch.empty(n * 4_000_000, dtype=torch.bfloat16, device='cuda')
+    q = big.as_strided((n, H, D), (4_000_000, D, 1))
+    k = big.as_strided((n, 1, D), (4_000_000, D, 1), H * D)
+    q.copy_(_normal(411, n, H, D))
+    k.copy_(_normal(412, n, 1, D))
+    assert q[-1].storage_offset() > 2 ** 31
+    g = 1 + _normal(413, D, scale=0.2)
+    pos = torch.arange(n, device='cuda')
+    dy = _normal(414, n, H, D, dtype=torch.bfloat16)
+    leaves = [q.detach().requires_grad_(), g.requires_grad_()]
+    yq, yk = ops.qk_norm_rope(leaves[0], k, g, g, pos)
+    dq, dg = torch.autograd.grad(yq, leaves, dy)
+    w = oracle.norm_rope(q, g, pos, dy=dy)
+    oracle.check(yq.detach(), w[0], w[1], 'q')
+    oracle.check(yk.detach(), *oracle.norm_rope(k, g, pos), 'k')
+    oracle.check(dq, w[2], w[3], 'dq')
+    oracle.check(dg, w[4], w[5], 'dgamma')                         # the keys' share of the common gain is zero: no cotangent
+
+
+def test_one_gain_for_both_and_one_array_for_keys_and_values(ops):
+    """The same leaf twice in a call: its gradients add up."""
+    M, H, G, D = 130, 4, 2, 64
+    q, k, _ = _qkv(421, M, M, H, G, D, torch.float32)
+    g, pos = 1 + _normal(424, D, scale=0.2), torch.arange(M, device='cuda')
+    dq, dk = _normal(425, M, H, D), _normal(426, M, G, D)
+    a = g.clone().requires_grad_()
+    got, = torch.autograd.grad(ops.qk_norm_rope(q, k, a, a, pos), a, (dq, dk))
+    b, c = g.clone().requires_grad_(), g.clone().requires_grad_()
+    want = torch.autograd.grad(ops.qk_norm_rope(q, k, b, c, pos), (b, c), (dq, dk))
+    assert torch.equal(got, want[0] + want[1])
+    a = k.clone().requires_grad_()
+    got, = torch.autograd.grad(ops.causal_attention(q, a, a, _batch([M])), a, dq)
+    b, c = k.clone().requires_grad_(), k.clone().requires_grad_()
+    want = torch.autograd.grad(ops.causal_attention(q, b, c, _batch([M])), (b, c), dq)
+    assert torch.equal(got, want[0] + want[1])
+
+
+@pytest.mark.parametrize('cap', [300, 5000])
+def test_step_replayed_with_other_lengths(eng, cap):
+    """Lengths are read on the device: one capture serves a stream from its first frame to a full cache."""
+    B, H, G, D = 3, 8, 2, 128
+    q, kc, vc = _normal(431, B, H, D, dtype=torch.float16), _normal(432, B, cap, G, D, dtype=torch.float16), _normal(433, B, cap, G, D, dtype=torch.float16)
+    ln = torch.tensor([1, 1, 1], dtype=torch.int32, device='cuda')
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        eng.attention_step(q, kc, vc, ln)
+    side.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=side):
+        out = eng.attention_step(q, kc, vc, ln)
+    for lens in ([1, 0, 2], [cap, cap - 1, 129], [0, 0, 0], [33, cap, 257]):
+        ln.copy_(torch.tensor(lens, dtype=torch.int32))
+        eager = eng.attention_step(q, kc, vc, ln)
+        torch.cuda.synchronize()
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, eager)
+        kk, vv = (torch.cat([c[b, :lens[b]] for b in range(B)]) for c in (kc, vc))
+        oracle.check(eager, *oracle.attention(q, kk, vv, [1] * B, lens), str(lens))
+
+
+def test_two_streams_at_once(ops, eng):
+    """Calls that overlap on two streams share nothing: each gives what it gives alone."""
+    cases = []
+    for i, (lens, H, G) in enumerate((([1500, 900], 4, 1), ([2000], 8, 2))):
+        q, k, v = _qkv(441 + 10 * i, sum(lens), sum(lens), H, G, 64, torch.bfloat16)
+        dout = _normal(445 + 10 * i, sum(lens), H, 64, dtype=torch.bfloat16)
+        cases.append(([t.requires_grad_() for t in (q, k, v)], _batch(lens), dout))
+
+    def run(case):
+        leaves, batch, dout = case
+        out = ops.causal_attention(*leaves, batch)
+        return (out.detach(), *torch.autograd.grad(out, leaves, dout))
+    want = [run(c) for c in cases]
+    streams = [torch.cuda.Stream() for _ in cases]
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(4):
+        for c, s in zip(cases, streams):
+            with torch.cuda.stream(s):
+                got.append(run(c))
+    torch.cuda.synchronize()
+    for i, g in enumerate(got):
+        assert all(torch.equal(a, b) for a, b in zip(g, want[i % 2]))
