@@ -126,11 +126,13 @@ __global__ __launch_bounds__(256, (D == 64 ? (sizeof(T) == 2 ? 4 : 2) : sizeof(T
             const int key0 = t * KT + nb * 32;
             if (key0 >= seen_w) break;
             f32x16 s = zero16(), dp = zero16();
+            products_first();
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
                 s = mma<T>(TL::row_frag(kt, nb * 32 + l31, ks, hi), qfr[ks], s);
                 dp = mma<T>(TL::row_frag(vt, nb * 32 + l31, ks, hi), gfr[ks], dp);
             }
+            products_done();
 #pragma unroll
             for (int r = 0; r < 16; ++r) s[r] = exp2_(fmaf(s[r], c2, -lse)) * (dp[r] - dsum);
             const bool edge = key0 + 32 > full_w;
@@ -144,12 +146,14 @@ __global__ __launch_bounds__(256, (D == 64 ? (sizeof(T) == 2 ? 4 : 2) : sizeof(T
                 for (int r = 0; r < 16; ++r) s[r] *= F;
             }
             if (edge) bad |= block_not_finite<T, D>(kt, nb * 32);
+            products_first();
 #pragma unroll
             for (int s2 = 0; s2 < 2; ++s2) {
                 const frag p = pack8<T>(s, s2);
 #pragma unroll
                 for (int d = 0; d < DB; ++d) acc[d] = mma<T>(TL::col_frag(kt, nb * 32 + 16 * s2, d, lane), p, acc[d]);
             }
+            products_done();
         }
     }
 
@@ -296,11 +300,13 @@ __global__ __launch_bounds__(256, (D == 64 ? (sizeof(T) == 2 ? 3 : 2) : sizeof(T
 #pragma unroll
                 for (int i = 0; i < 4; ++i) dp[4 * r4 + i] = d4[i];
             }
+            products_first();
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
                 s = mma<T>(TL::row_frag(qt, nb * 32 + l31, ks, hi), kfr[ks], s);
                 dp = mma<T>(TL::row_frag(gt, nb * 32 + l31, ks, hi), vfr(ks), dp);
             }
+            products_done();
             const bool edge = qb0 + shift < kw + 31 || qb0 + 32 > Tq || kw + 32 > Tk;
 #pragma unroll
             for (int r4 = 0; r4 < 4; ++r4) {
@@ -329,6 +335,7 @@ __global__ __launch_bounds__(256, (D == 64 ? (sizeof(T) == 2 ? 3 : 2) : sizeof(T
 #pragma unroll
                 for (int r = 0; r < 16; ++r) dp[r] *= F;
             }
+            products_first();
 #pragma unroll
             for (int s2 = 0; s2 < 2; ++s2) {
                 const frag pf = pack8<T>(s, s2), df = pack8<T>(dp, s2);
@@ -338,6 +345,7 @@ __global__ __launch_bounds__(256, (D == 64 ? (sizeof(T) == 2 ? 3 : 2) : sizeof(T
                     dk[d] = mma<T>(TL::col_frag(qt, nb * 32 + 16 * s2, d, lane), df, dk[d]);
                 }
             }
+            products_done();
         }
         g = gn;
         t = tn;

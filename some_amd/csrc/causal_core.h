@@ -71,13 +71,17 @@ __device__ __forceinline__ f32x16 zero16() {
     return z;
 }
 
+// Around a run of products: the wave goes before the others of its SIMD, whose exponentials then fill the gaps between the products instead of delaying them.
+// us without and with: backward, 8 x 2584 frames, 8/2 heads of 64: dK/dV bf16 146, 140, f16 170, 159, dQ 108, 106.5 and 120, 116; forward, 3 clips up to 8191,
+// 16/4 heads of 128, bf16: 340, 315, but 4 x 4096 frames in f32 1416, 1446 and heads of 64, bf16, 84.4, 86.6 - there the forward goes without.
+__device__ __forceinline__ void products_first() { __builtin_amdgcn_s_setprio(1); }
+__device__ __forceinline__ void products_done() { __builtin_amdgcn_s_setprio(0); }
+
 // Instruction order inside a basic block.  Left alone, hipcc places every LDS read directly before the matrix instruction that needs it and waits for it
 // there, one read in flight at a time.  A sequence of these calls at the end of a block asks for `N` instructions of one kind after the other instead:
-// reads some products ahead, exponentials between products.
+// reads some products ahead.
 template <int N> __device__ __forceinline__ void order_mfma() { __builtin_amdgcn_sched_group_barrier(0x008, N, 0); }
 template <int N> __device__ __forceinline__ void order_lds() { __builtin_amdgcn_sched_group_barrier(0x100, N, 0); }
-template <int N> __device__ __forceinline__ void order_valu() { __builtin_amdgcn_sched_group_barrier(0x002, N, 0); }
-template <int N> __device__ __forceinline__ void order_exp() { __builtin_amdgcn_sched_group_barrier(0x400, N, 0); }
 // MFMAS products, each with READS LDS reads of its own, the reads AHEAD products early
 template <int MFMAS, int READS, int AHEAD> __device__ __forceinline__ void order_products() {
     order_lds<READS * AHEAD>();
@@ -89,7 +93,7 @@ template <int MFMAS, int READS, int AHEAD> __device__ __forceinline__ void order
     order_mfma<AHEAD>();
 }
 
-// registers 8 s .. 8 s + 7 of a product as a fragment, rounded to the operand type (16-bit: half an ulp, 2^-9 / 2^-12 of the value)
+// registers 8 s .. 8 s + 7 of a product as a fragment, rounded to the operand type (16-bit: half a step, 2^-8 or 2^-11 of the value)
 template <typename T> __device__ __forceinline__ typename Frag<T>::type pack8(const f32x16& x, int s) {
     typename Frag<T>::type f;
     if constexpr (sizeof(T) == 4) {

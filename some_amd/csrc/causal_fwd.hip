@@ -112,6 +112,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 && D == 64 ? 4 : 2)) void caus
         const int key0 = t * KT;
         if (key0 >= seen_w) continue;
         f32x16 s[NB];
+        if constexpr (sizeof(T) == 2 && D == 128) products_first();
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
             s[nb] = zero16();
@@ -119,6 +120,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 && D == 64 ? 4 : 2)) void caus
             for (int ks = 0; ks < KS; ++ks) s[nb] = mma<T>(TL::row_frag(kt, nb * 32 + l31, ks, hi), qfr[ks], s[nb]);
         }
         if constexpr (sizeof(T) == 2) order_products<NB * KS, 1, 4>();
+        if constexpr (sizeof(T) == 2 && D == 128) products_done();
         if (key0 + KT > full_w) {                            // some masked place in here
             const int limit = min(q + shift, Tk - 1);
 #pragma unroll
@@ -152,6 +154,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 && D == 64 ? 4 : 2)) void caus
                 s[nb][r] = exp2_(fmaf(s[nb][r], c2, -mc));
                 l += s[nb][r];
             }
+        if constexpr (sizeof(T) == 2 && D == 128) products_first();
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
@@ -161,6 +164,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 && D == 64 ? 4 : 2)) void caus
                 for (int d = 0; d < DB; ++d) o[d] = mma<T>(TL::col_frag(vt, nb * 32 + 16 * s2, d, lane), p, o[d]);
             }
         if constexpr (sizeof(T) == 2) order_products<NB * 2 * DB, 2, 3>();
+        if constexpr (sizeof(T) == 2 && D == 128) products_done();
     }
 
     const int64_t prow = (int64_t)part * a.q_rows * a.kv_heads * a.group;
