@@ -70,11 +70,11 @@ def _place(x: torch.Tensor):
 
 
 def check_device(device: torch.device, *tensors):
-    first = tensors[0].device
+    first, want = tensors[0].get_device(), device.index            # (get_device: -1 on the host; a torch.device per tensor is 2 us of a 12 us call)
     for t in tensors:
-        d = t.device
-        if d.type != 'cuda' or d.index != first.index or (device.index is not None and d.index != device.index):
-            raise ValueError(f'a tensor is on {d}: the operators run on {device}, all tensors of a call on one device')
+        i = t.get_device()
+        if i != first or i < 0 or (want is not None and i != want):
+            raise ValueError(f'a tensor is on {t.device}: the operators run on {device}, all tensors of a call on one device')
 
 
 _get_device, _raw_stream = torch._C._cuda_getDevice if hasattr(torch._C, '_cuda_getDevice') else torch.cuda.current_device, getattr(torch._C, '_cuda_getCurrentRawStream', None)
@@ -216,12 +216,13 @@ def check_step(device, q, k_cache, v_cache, lengths, max_length):
     """-> (q, the caches' places, max_length), checked."""
     q = heads_view(q, 'q', 0)
     B, H, D = q.shape
+    shape = k_cache.shape if isinstance(k_cache, torch.Tensor) else ()
     for name, c in (('k_cache', k_cache), ('v_cache', v_cache)):
-        if not isinstance(c, torch.Tensor) or c.dim() != 4 or c.shape[0] != B or c.shape[3] != D or c.shape != k_cache.shape or c.shape[2] == 0:
+        if not isinstance(c, torch.Tensor) or c.shape != shape or len(shape) != 4 or shape[0] != B or shape[2] == 0 or shape[3] != D:
             raise ValueError(f'{name} must be [{B}, capacity, kv_heads, {D}], k and v alike')
-        if c.dtype != q.dtype:
+        if c.dtype is not q.dtype:
             raise TypeError(f'q and {name} must have one type, got {q.dtype} and {c.dtype}')
-    capacity, G = k_cache.shape[1:3]
+    _, capacity, G, _ = shape
     if H % G:
         raise ValueError(f'{H} query heads are not a multiple of {G} key / value heads')
     if not isinstance(lengths, torch.Tensor) or lengths.dtype != torch.int32 or lengths.shape != (B,):
