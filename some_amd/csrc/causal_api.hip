@@ -7,8 +7,11 @@
 
 namespace {
 
-int cfail(SomeHandle* h, int code, const char* fn, const char* msg) {
-    h->err = std::string(fn) + ": " + msg;
+int cfail(SomeHandle* h, int code, const char* fn, const char* msg) noexcept {
+    try {
+        h->err = std::string(fn) + ": " + msg;
+    } catch (...) {                                          // (no memory for the text: the code alone)
+    }
     return code;
 }
 #define C_CHECK(cond, msg) do { if (!(cond)) return cfail(h, SOME_EINVAL, __func__, msg); } while (0)

@@ -5,6 +5,8 @@
 // group frames with all heads of a group, which read every key tile together -, a wave 32 of them; S^T = K Q^T puts a query in every lane's column, so its
 // maximum and sum are the lane's own registers plus one exchange with the other half, and P^T is already the B operand of O^T += V^T P^T (causal_core.h):
 // no probability touches LDS.  K and V tiles go global -> LDS by DMA into a ring; V is read transposed by ds_read_b64_tr_b16.
+// Bound by the products at heads of 128 - 2 clips up to 16384, 32/8 heads, bf16: 2.42 ms, 1040 TF/s, where a large matrix product reaches 1120 under the power
+// limit - and at heads of 64 by the exponentials and what stands around them (8 x 2584, 8/2 heads, bf16: 84 us, 650 TF/s, VALU 60 % and products 29 % busy).
 #include "causal_core.h"
 
 namespace {
@@ -165,6 +167,31 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 && D == 64 ? 4 : 2)) void caus
             }
         if constexpr (sizeof(T) == 2) order_products<NB * 2 * DB, 2, 3>();
         if constexpr (sizeof(T) == 2 && D == 128) products_done();
+    }
+
+    // A wave that sees one tile in all: where a row sees few keys, nothing averages the rounding of P out of O (nor of the gradients' D), so what it took goes
+    // in too.  The tile still lies in the first stage, nobody writes there any more, and the maximum is the loop's.
+    if constexpr (sizeof(T) == 2) {
+        if (t_begin == 0 && t_end <= STAGES && seen_w > 0 && seen_w <= KT && !bad) {
+            const float mc = m == -INFINITY ? 0.f : m * c2;
+            const int limit = min(q + shift, Tk - 1);
+            for (int nb = 0; nb * 32 < seen_w; ++nb) {
+                f32x16 s = zero16();
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks) s = mma<T>(TL::row_frag(lds, nb * 32 + l31, ks, hi), qfr[ks], s);
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const float p = nb * 32 + crow(r, hi) <= limit ? exp2_(fmaf(s[r], c2, -mc)) : 0.f;
+                    s[r] = p - (float)(T)p;
+                }
+#pragma unroll
+                for (int s2 = 0; s2 < 2; ++s2) {
+                    const frag p = pack8<T>(s, s2);
+#pragma unroll
+                    for (int d = 0; d < DB; ++d) o[d] = mma<T>(TL::col_frag(lds + TILE_B, nb * 32 + 16 * s2, d, lane), p, o[d]);
+                }
+            }
+        }
     }
 
     const int64_t prow = (int64_t)part * a.q_rows * a.kv_heads * a.group;

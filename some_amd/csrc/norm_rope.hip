@@ -5,7 +5,7 @@
 // bf16 80 us forward (4.2 TB/s) and 128 + 4 us backward (4.0 TB/s; no less without sines and cosines); a large copy runs at 5.0 TB/s.
 // A thread holds 8 channels of the lower half of a head and their partners in the upper half, so the rotation needs no exchange and D / 16 neighbouring lanes
 // hold a head; it keeps its 8 sines and cosines for every head of its row that it works on.  The queries' heads and the keys' go to different blocks: in one,
-// a thread would need both gains and two sets of gain gradients (backward: 157 registers instead of 125, 152 us).
+// a thread would need both gains and two sets of gain gradients (backward, bf16: 152 us).
 // The angle is reduced in 64 bits (position x turns-per-position, minus the whole turns): at position 10^6 a 32-bit product is off by 0.06 rad.
 #include "causal_core.h"
 
