@@ -168,7 +168,7 @@ int some_op_causal_attention(SomeHandle* h, int32_t dtype, int32_t head_dim, con
         a.part_o = static_cast<float*>(workspace_dev);
         a.part_ml = a.part_o + (int64_t)a.parts * q_rows * heads * head_dim;
     }
-    C_CHECK(q_rows * a.group < 0x7fffff00ll && causal_fwd_blocks(a) <= kMaxBlocks, "too many rows, clips and heads for one launch");
+    C_CHECK(q_rows * a.group < 0x7fffff00ll && k_rows * a.group < (1ll << 36) && causal_fwd_blocks(a) <= kMaxBlocks, "too many rows, clips and heads for one launch");
     C_TRY(launch_causal_fwd(dtype, head_dim, a, static_cast<hipStream_t>(stream)));
     return SOME_OK;
 }
@@ -206,7 +206,7 @@ int some_train_causal_attention_bwd(SomeHandle* h, int32_t dtype, int32_t head_d
     b.dsum = static_cast<float*>(workspace_dev);
     b.part_q = b.part_k = reinterpret_cast<float*>(static_cast<char*>(workspace_dev) + dsum_bytes(heads, q_rows));
     b.part_v = b.part_k + (int64_t)b.parts * k_rows * kv_heads * head_dim;
-    C_CHECK(q_rows * a.group < 0x7fffff00ll && causal_fwd_blocks(a) <= kMaxBlocks && causal_bwd_blocks(b) <= kMaxBlocks,
+    C_CHECK(q_rows * a.group < 0x7fffff00ll && k_rows * a.group < (1ll << 36) && causal_fwd_blocks(a) <= kMaxBlocks && causal_bwd_blocks(b) <= kMaxBlocks,
             "too many rows, clips and heads for one launch");
     C_TRY(launch_causal_bwd(dtype, head_dim, b, static_cast<hipStream_t>(stream)));
     return SOME_OK;

@@ -722,3 +722,27 @@ def test_two_streams_at_once(ops, eng):
     torch.cuda.synchronize()
     for i, g in enumerate(got):
         assert all(torch.equal(a, b) for a, b in zip(g, want[i % 2]))
+
+
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('H,G', [(1024, 1), (1024, 1024), (300, 3), (35, 7)])
+def test_many_heads_and_odd_groups(ops, eng, dtype, H, G):
+    """Up to 1024 heads: groups larger than a workgroup's 128 queries (a frame then spans tiles), groups that do not divide them, kv heads that do not divide the XCDs."""
+    D, ql, kl = 64, [3, 0, 9], [5, 2, 9]
+    q, k, v = _qkv(451, sum(ql), sum(kl), H, G, D, dtype)
+    dout = _normal(455, sum(ql), H, D, dtype=dtype)
+    leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+    out = ops.causal_attention(*leaves, _batch(ql), kv_batch=_batch(kl))
+    grads = torch.autograd.grad(out, leaves, dout)
+    w = oracle.attention(q, k, v, ql, kl, dout=dout)
+    for i, (name, got) in enumerate(zip(('out', 'dq', 'dk', 'dv'), (out.detach(), *grads))):
+        oracle.check(got, w[2 * i], w[2 * i + 1], name)
+    cache = [torch.zeros(2, 9, G, D, dtype=dtype, device='cuda') for _ in range(2)]
+    for c, t in zip(cache, (k, v)):
+        c[0, :5], c[1] = t[:5], t[7:]
+    step = eng.attention_step(q[[2, 11]], *cache, torch.tensor([5, 9], dtype=torch.int32, device='cuda'))
+    oracle.check(step, w[0][[2, 11]], w[1][[2, 11]], 'step')
+    gq, gk, pos = 1 + _normal(456, D, scale=0.2), 1 + _normal(457, D, scale=0.2), torch.arange(sum(ql), device='cuda')
+    yq, yk = eng.qk_norm_rope(q, k[:sum(ql)], gq, gk, pos)
+    oracle.check(yq, *oracle.norm_rope(q, gq, pos), 'q')
+    oracle.check(yk, *oracle.norm_rope(k[:sum(ql)], gk, pos), 'k')
