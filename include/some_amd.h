@@ -578,8 +578,8 @@ int some_train_causal_attention_bwd(SomeHandle* h, int32_t dtype, int32_t head_d
 
 /* The next frame of B live streams: out[b, h] = attention of q[b, h] over the first lengths[b] rows (device int32, cut to [0, max_length]; 0: zeros) of
  * stream b's cache, k_dev + b k_batch and v_dev + b v_batch.  Rows from lengths[b] on are not read.  max_length: an upper bound of the lengths the
- * caller knows (at most the cache's capacity); it sizes the launch.  workspace_dev: some_op_attention_step_bytes bytes, 16-byte aligned, not shared
- * with a call that may run at the same time. */
+ * caller knows (at most the cache's capacity); it sizes the launch.  workspace_dev: some_op_attention_step_bytes bytes (0 while the caches are short),
+ * 16-byte aligned, not shared with a call that may run at the same time. */
 size_t some_op_attention_step_bytes(const SomeHandle* h, int32_t dtype, int32_t B, int32_t heads, int32_t kv_heads, int32_t head_dim, int32_t max_length);
 int some_op_attention_step(SomeHandle* h, int32_t dtype, int32_t head_dim, const void* q_dev, int64_t q_row, int64_t q_head, int32_t heads,
                            const void* k_dev, int64_t k_batch, int64_t k_row, int64_t k_head, const void* v_dev, int64_t v_batch, int64_t v_row,
