@@ -746,3 +746,26 @@ def test_many_heads_and_odd_groups(ops, eng, dtype, H, G):
     yq, yk = eng.qk_norm_rope(q, k[:sum(ql)], gq, gk, pos)
     oracle.check(yq, *oracle.norm_rope(q, gq, pos), 'q')
     oracle.check(yk, *oracle.norm_rope(k[:sum(ql)], gk, pos), 'k')
+
+
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('M,H,G', [(7, 4, 2), (3000, 40, 8)])
+def test_norm_rope_in_place(ops, eng, dtype, M, H, G):
+    """The C entries' outputs may be their inputs."""
+    import some_amd._lib as _lib
+    D, code, lib, h = 128, TYPES.index(dtype), _lib.fast(), eng.handle.value
+    q, k = _normal(461, M, H, D, dtype=dtype), _normal(462, M, G, D, dtype=dtype)
+    gq, gk, pos = 1 + _normal(463, D, scale=0.2), 1 + _normal(464, D, scale=0.2), torch.arange(M, device='cuda')
+    dq, dk = _normal(465, M, H, D, dtype=dtype), _normal(466, M, G, D, dtype=dtype)
+    leaves = [t.detach().clone().requires_grad_() for t in (q, k, gq, gk)]
+    y = ops.qk_norm_rope(*leaves, pos)
+    want = torch.autograd.grad(y, leaves, (dq, dk))
+    s3 = lambda t: (t.data_ptr(), t.stride(0), t.stride(1))                                   # noqa: E731
+    head = (h, code, D, *s3(q), H, *s3(k), G, M, gq.data_ptr(), gk.data_ptr(), pos.data_ptr(), 1, 10000.0, 1e-6)
+    st = torch.cuda.current_stream().cuda_stream
+    work = torch.empty(lib.some_train_qk_norm_rope_bytes(h, M, H, G, D), dtype=torch.uint8, device='cuda')
+    dgq, dgk = torch.empty_like(gq), torch.empty_like(gk)
+    _lib.check(h, lib.some_train_qk_norm_rope_bwd(*head, *s3(dq), *s3(dk), *s3(dq), *s3(dk), dgq.data_ptr(), dgk.data_ptr(), 0, work.data_ptr(), work.numel(), st))
+    assert all(torch.equal(a, b) for a, b in zip((dq, dk, dgq, dgk), want))
+    _lib.check(h, lib.some_op_qk_norm_rope(*head, *s3(q), *s3(k), st))
+    assert torch.equal(q, y[0]) and torch.equal(k, y[1])
