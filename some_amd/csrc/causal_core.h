@@ -254,11 +254,14 @@ __device__ __forceinline__ void solo_column(float (&acc)[(D + 63) / 64], int r0,
     const int lane = threadIdx.x & 63;
     for (int base = r0; base < r1; base += 64) {
         const float w = base + lane < r1 ? weight(base + lane) : 0.f;
+        float part[(D + 63) / 64] = {};                      // (64 rows by themselves: equal terms added one by one all round the same way)
         for (int j = 0; j < min(64, r1 - base); ++j) {
             const float wj = __shfl(w, j, 64);
 #pragma unroll
-            for (int e = 0; e < (D + 63) / 64; ++e) acc[e] = fmaf(wj, to_f32(m[(int64_t)(base + j) * stride + lane + 64 * e]), acc[e]);
+            for (int e = 0; e < (D + 63) / 64; ++e) part[e] = fmaf(wj, to_f32(m[(int64_t)(base + j) * stride + lane + 64 * e]), part[e]);
         }
+#pragma unroll
+        for (int e = 0; e < (D + 63) / 64; ++e) acc[e] += part[e];
     }
 }
 

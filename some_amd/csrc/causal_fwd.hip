@@ -50,7 +50,7 @@ __device__ __forceinline__ void solo_query(const CausalArgs& a, const T* q, cons
 }
 
 template <typename T, int D>
-__global__ __launch_bounds__(256, (sizeof(T) == 2 && D == 64 ? 4 : 2)) void causal_fwd_kernel(CausalArgs a, int nsub, int positions) {
+__global__ __launch_bounds__(256, (sizeof(T) == 2 ? (D == 64 ? 4 : 2) : (D == 64 ? 2 : 1))) void causal_fwd_kernel(CausalArgs a, int nsub, int positions) {
     typedef Shape<T, D> SH;
     constexpr int KT = SH::KT, NB = KT / 32, KS = D / 16, DB = D / 32, TILE_B = SH::TILE_B, STAGES = SH::STAGES;
     typedef Tile<T, D> TL;
@@ -100,7 +100,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 && D == 64 ? 4 : 2)) void caus
     f32x16 o[DB];
 #pragma unroll
     for (int d = 0; d < DB; ++d) o[d] = zero16();
-    float m = -INFINITY, l = 0.f;                            // running maximum (of the raw products) and this half's share of the sum
+    float m = -INFINITY, l = 0.f, lost = 0.f;                // running maximum (of the raw products), this half's share of the sum, what rounding added to it last (f32)
     const float c2 = a.scale * 1.4426950408889634f, slack = kSlack / c2;
     bool bad = false;
 
@@ -143,6 +143,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 && D == 64 ? 4 : 2)) void caus
             const float f = m == -INFINITY ? 0.f : exp2_((m - mn) * c2);
             m = mn;
             l *= f;
+            lost *= f;
 #pragma unroll
             for (int d = 0; d < DB; ++d)
 #pragma unroll
@@ -152,19 +153,39 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 && D == 64 ? 4 : 2)) void caus
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                s[nb][r] = exp2_(fmaf(s[nb][r], c2, -mc));
-                l += s[nb][r];
-            }
+            for (int r = 0; r < 16; ++r) s[nb][r] = exp2_(fmaf(s[nb][r], c2, -mc));
+        // 32 keys' weights are summed by themselves: one by one, the equal weights of a long level row all round the same way (65 536 keys: off by 7e-4), and those of a
+        // row with one dominating key are too small to move its sum at all.  f32 carries what the addition to the row's sum rounds as well (65 536 keys: 4e-5)
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+            float w = s[nb][0];
+#pragma unroll
+            for (int r = 1; r < 16; ++r) w += s[nb][r];
+            if constexpr (sizeof(T) == 4) w -= lost;
+            const float sum = l + w;
+            if constexpr (sizeof(T) == 4) lost = (sum - l) - w;
+            l = sum;
+        }
         if constexpr (sizeof(T) == 2 && D == 128) products_first();
+        if constexpr (sizeof(T) == 4) {
+            // f32 products add one key after the other: a tile's by themselves, for the sum's reason (16-bit ones add eight keys at a time, and far below their own
+            // rounding).  At heads of 128 that is too much for two waves a SIMD (59 registers spilled; 4 x 4096 frames, 8/2 heads, 1810 us: one wave 1375)
+            static_assert(NB == 1, "a tile of 32 keys");
 #pragma unroll
-        for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-            for (int s2 = 0; s2 < 2; ++s2) {
-                const frag p = pack8<T>(s[nb], s2);
-#pragma unroll
-                for (int d = 0; d < DB; ++d) o[d] = mma<T>(TL::col_frag(vt, nb * 32 + 16 * s2, d, lane), p, o[d]);
+            for (int d = 0; d < DB; ++d) {
+                o[d] += mma<T>(TL::col_frag(vt, 16, d, lane), pack8<T>(s[0], 1), mma<T>(TL::col_frag(vt, 0, d, lane), pack8<T>(s[0], 0), zero16()));
+                __builtin_amdgcn_sched_barrier(0);           // (one such sum in registers at a time)
             }
+        } else {
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                for (int s2 = 0; s2 < 2; ++s2) {
+                    const frag p = pack8<T>(s[nb], s2);
+#pragma unroll
+                    for (int d = 0; d < DB; ++d) o[d] = mma<T>(TL::col_frag(vt, nb * 32 + 16 * s2, d, lane), p, o[d]);
+                }
+        }
         if constexpr (sizeof(T) == 2) order_products<NB * 2 * DB, 2, 3>();
         if constexpr (sizeof(T) == 2 && D == 128) products_done();
     }
