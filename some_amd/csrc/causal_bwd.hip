@@ -149,11 +149,15 @@ __global__ __launch_bounds__(256, (D == 64 ? (sizeof(T) == 2 ? 4 : 2) : sizeof(T
             }
             if (edge) bad |= block_not_finite<T, D>(kt, nb * 32);
             products_first();
+            if constexpr (sizeof(T) == 4) {
+                add_block<T, D>(acc, kt, nb * 32, s, lane);
+            } else {
 #pragma unroll
-            for (int s2 = 0; s2 < 2; ++s2) {
-                const frag p = pack8<T>(s, s2);
+                for (int s2 = 0; s2 < 2; ++s2) {
+                    const frag p = pack8<T>(s, s2);
 #pragma unroll
-                for (int d = 0; d < DB; ++d) acc[d] = mma<T>(TL::col_frag(kt, nb * 32 + 16 * s2, d, lane), p, acc[d]);
+                    for (int d = 0; d < DB; ++d) acc[d] = mma<T>(TL::col_frag(kt, nb * 32 + 16 * s2, d, lane), p, acc[d]);
+                }
             }
             products_done();
         }
@@ -200,8 +204,9 @@ __global__ __launch_bounds__(256, (D == 64 ? (sizeof(T) == 2 ? 4 : 2) : sizeof(T
 // ---- dK, dV --------------------------------------------------------------------------------------------------------------------------------
 constexpr int KB = 128;                         // keys per workgroup
 template <typename T, int D> struct DkvShape {
-    static constexpr bool V_LDS = D == 128;                                // V fragments from LDS, not registers: lets two waves share a SIMD (f32: no spills)
-    static constexpr int QT = sizeof(T) == 4 || V_LDS ? 32 : 64;           // queries per tile
+    // V fragments from LDS, not registers: at heads of 128 two waves share a SIMD, in f32 nothing spills (4 x 4096 frames, 8/2 heads of 64: 1270 us, with spills 1490)
+    static constexpr bool V_LDS = D == 128 || sizeof(T) == 4;
+    static constexpr int QT = V_LDS ? 32 : 64;                             // queries per tile
     static constexpr int TILE_B = QT * D * (int)sizeof(T);
     static constexpr int STAGE_B = 2 * TILE_B + 2 * 64 * 4;                // Q, dO, lse, D
     static constexpr int LDS_B = 2 * STAGE_B + (V_LDS ? KB * D * (int)sizeof(T) : 0);
@@ -338,13 +343,18 @@ __global__ __launch_bounds__(256, (D == 64 ? (sizeof(T) == 2 ? 3 : 2) : sizeof(T
                 for (int r = 0; r < 16; ++r) dp[r] *= F;
             }
             products_first();
+            if constexpr (sizeof(T) == 4) {
+                add_block<T, D>(dv, gt, nb * 32, s, lane);
+                add_block<T, D>(dk, qt, nb * 32, dp, lane);
+            } else {
 #pragma unroll
-            for (int s2 = 0; s2 < 2; ++s2) {
-                const frag pf = pack8<T>(s, s2), df = pack8<T>(dp, s2);
+                for (int s2 = 0; s2 < 2; ++s2) {
+                    const frag pf = pack8<T>(s, s2), df = pack8<T>(dp, s2);
 #pragma unroll
-                for (int d = 0; d < DB; ++d) {
-                    dv[d] = mma<T>(TL::col_frag(gt, nb * 32 + 16 * s2, d, lane), pf, dv[d]);
-                    dk[d] = mma<T>(TL::col_frag(qt, nb * 32 + 16 * s2, d, lane), df, dk[d]);
+                    for (int d = 0; d < DB; ++d) {
+                        dv[d] = mma<T>(TL::col_frag(gt, nb * 32 + 16 * s2, d, lane), pf, dv[d]);
+                        dk[d] = mma<T>(TL::col_frag(qt, nb * 32 + 16 * s2, d, lane), df, dk[d]);
+                    }
                 }
             }
             products_done();

@@ -220,6 +220,17 @@ template <typename T, int D, int ROWS, int NT> struct Copier {
     }
 };
 
+// f32: acc[d] += the tile's 32 rows from r0 on, transposed, times x.  These products add one row after the other, so a block's are summed by themselves, one
+// sum in registers at a time: added to a long sum one by one, equal terms all round the same way (65 536 of them: off by 7e-4).
+template <typename T, int D> __device__ __forceinline__ void add_block(f32x16 (&acc)[D / 32], const char* tile, int r0, const f32x16& x, int lane) {
+    typedef Tile<T, D> TL;
+#pragma unroll
+    for (int d = 0; d < D / 32; ++d) {
+        acc[d] += mma<T>(TL::col_frag(tile, r0 + 16, d, lane), pack8<T>(x, 1), mma<T>(TL::col_frag(tile, r0, d, lane), pack8<T>(x, 0), zero16()));
+        __builtin_amdgcn_sched_barrier(0);
+    }
+}
+
 // ---- not-a-number and infinities in masked places ----------------------------------------------------------------------------------------------
 // A masked weight is 0, and 0 * inf would reach the sum.  Only a 32 x 32 block on the diagonal (or at a clip's end) mixes masked and visible places.
 // If the 32 tile rows such a block contracts over hold a value that is not finite, the wave remembers it and, when its loop is done, computes its

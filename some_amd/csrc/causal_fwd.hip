@@ -168,14 +168,10 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 ? (D == 64 ? 4 : 2) : (D == 64
         }
         if constexpr (sizeof(T) == 2 && D == 128) products_first();
         if constexpr (sizeof(T) == 4) {
-            // f32 products add one key after the other: a tile's by themselves, for the sum's reason (16-bit ones add eight keys at a time, and far below their own
-            // rounding).  At heads of 128 that is too much for two waves a SIMD (59 registers spilled; 4 x 4096 frames, 8/2 heads, 1810 us: one wave 1375)
+            // (16-bit products add eight keys at a time, and far below their own rounding).  The block's sum is too much for two waves a SIMD at heads of 128: 59
+            // registers spilled, 4 x 4096 frames, 8/2 heads, 1810 us, one wave 1375
             static_assert(NB == 1, "a tile of 32 keys");
-#pragma unroll
-            for (int d = 0; d < DB; ++d) {
-                o[d] += mma<T>(TL::col_frag(vt, 16, d, lane), pack8<T>(s[0], 1), mma<T>(TL::col_frag(vt, 0, d, lane), pack8<T>(s[0], 0), zero16()));
-                __builtin_amdgcn_sched_barrier(0);           // (one such sum in registers at a time)
-            }
+            add_block<T, D>(o, vt, 0, s[0], lane);
         } else {
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb)

@@ -63,3 +63,18 @@ def test_long_rows_of_equal_keys(eng, dtype, D, n, values):
         q, k, v = (t.to(dtype).contiguous() for t in (q, k, v))
         out = eng.causal_attention(q, k, v, _batch(ql), kv_batch=_batch(kl))
         oracle.check(out, *oracle.attention(q, k, v, ql, kl), f'out {gain}')
+
+
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('D', [64, 128])
+@pytest.mark.parametrize('causal', [True, False])
+def test_gradients_of_long_runs_of_equal_frames(ops, dtype, D, causal):
+    n = 12000
+    lens = [n] + ALONE
+    M = sum(lens)
+    _whole(dtype, 1, 1, D, lens, lens)
+    q, k, v, dout = (_normal(61 + i, 1, 1, D).repeat(M, 1, 1).to(dtype) for i in range(4))
+    leaves = [t.requires_grad_() for t in (q, k, v)]
+    out = ops.causal_attention(*leaves, _batch(lens), causal_mask=causal)
+    grads = torch.autograd.grad(out, leaves, dout)
+    _check_all((out, *grads), oracle.attention(*(t.detach() for t in leaves), lens, lens, causal, dout=dout))
