@@ -15,6 +15,18 @@ using namespace causal;
 // The running maximum only has to keep the exponentials in range, so it follows the true one lazily: it moves when a score passes it by 2^8.  P then
 // reaches 256, far inside every operand type, and the accumulators are rescaled once or twice per row instead of at every new maximum.
 constexpr float kSlack = 8.f;
+constexpr float kDrop = 11.f;                    // (f16: row_base)
+
+// What the exponentials of a row are taken relative to: P = exp2(s c2 - row_base(m)).  In f16 the base lies 2^7 below the maximum, so that P runs from 2^15 (the
+// slack included) down to subnormals of 2^-24, and the running maximum follows the true one of a tile DOWN as well when that lies 2^11 below: with the row's
+// maximum and a largest P of 1, the level tail of a peaked row - 16 384 keys 17.4 nats below one - was rounded away altogether.  A weight is off by at most 2^-21
+// of its tile's largest that way (and by 2^-32 of it where that is the row's).  Scores of 2^20 and more, whose base has no digits behind the point left to spare,
+// do without the 2^7: there P needs the room above.
+template <typename T> __device__ __forceinline__ float row_base(float m, float c2) {
+    const float x = m * c2;
+    if constexpr (__is_same(T, f16_t)) return x - (__builtin_fabsf(x) < 0x1p20f ? 7.f : 0.f);
+    else return x;
+}
 
 constexpr int QB = 128;                          // queries per workgroup
 
@@ -101,7 +113,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 ? (D == 64 ? 4 : 2) : (D == 64
 #pragma unroll
     for (int d = 0; d < DB; ++d) o[d] = zero16();
     float m = -INFINITY, l = 0.f, lost = 0.f;                // running maximum (of the raw products), this half's share of the sum, what rounding added to it last (f32)
-    const float c2 = a.scale * 1.4426950408889634f, slack = kSlack / c2;
+    const float c2 = a.scale * 1.4426950408889634f, slack = kSlack / c2, drop = kDrop / c2;
     bool bad = false;
 
     if (t_begin < t_end) fetch(t_begin);
@@ -138,9 +150,14 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 ? (D == 64 ? 4 : 2) : (D == 64
 #pragma unroll
             for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[nb][r]);
         mx = halves_max(mx);
-        if (__any(mx > m + slack)) {                         // (the first visible key passes -inf)
-            const float mn = mx > m + slack ? mx : m;
-            const float f = m == -INFINITY ? 0.f : exp2_((m - mn) * c2);
+        // (the first visible key passes -inf; a sum m + slack would round up where scores are huge)
+        if (__any(__is_same(T, f16_t) ? __builtin_fabsf(mx - m + 0.5f * (drop - slack)) > 0.5f * (drop + slack) : mx - m > slack)) {
+            float mn = mx - m > slack ? mx : m;
+            if constexpr (__is_same(T, f16_t)) {             // down: as far as the row's sum, and with it O, keeps inside f32's range
+                const float room = fmaxf(100.f - log2_(halves_max(l)), 0.f) / c2;
+                if (mx - m < -drop && mx > -INFINITY) mn = fmaxf(mx, m - room);
+            }
+            const float f = m == -INFINITY ? 0.f : exp2_(row_base<T>(m, c2) - row_base<T>(mn, c2));
             m = mn;
             l *= f;
             lost *= f;
@@ -149,7 +166,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 ? (D == 64 ? 4 : 2) : (D == 64
 #pragma unroll
                 for (int r = 0; r < 16; ++r) o[d][r] *= f;
         }
-        const float mc = m == -INFINITY ? 0.f : m * c2;
+        const float mc = m == -INFINITY ? 0.f : row_base<T>(m, c2);
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
@@ -190,7 +207,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 ? (D == 64 ? 4 : 2) : (D == 64
     // in too.  The tile still lies in the first stage, nobody writes there any more, and the maximum is the loop's.
     if constexpr (sizeof(T) == 2) {
         if (t_begin == 0 && t_end <= STAGES && seen_w > 0 && seen_w <= KT && !bad) {
-            const float mc = m == -INFINITY ? 0.f : m * c2;
+            const float mc = m == -INFINITY ? 0.f : row_base<T>(m, c2);
             const int limit = min(q + shift, Tk - 1);
             for (int nb = 0; nb * 32 < seen_w; ++nb) {
                 f32x16 s = zero16();
@@ -250,7 +267,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 ? (D == 64 ? 4 : 2) : (D == 64
 #pragma unroll
             for (int r4 = 0; r4 < 4; ++r4)
                 store4<float>(a.part_o + i * D + 32 * d + 8 * r4 + 4 * hi, o[d][4 * r4], o[d][4 * r4 + 1], o[d][4 * r4 + 2], o[d][4 * r4 + 3]);
-        if (hi == 0) *reinterpret_cast<f32x2*>(a.part_ml + 2 * i) = (f32x2){m * c2, part == 0 && !any ? -1.f : sum};
+        if (hi == 0) *reinterpret_cast<f32x2*>(a.part_ml + 2 * i) = (f32x2){row_base<T>(m, c2), part == 0 && !any ? -1.f : sum};
     } else {
         const float inv = any ? 1.f / sum : 0.f;             // no visible key: zero
         T* orow = static_cast<T*>(a.out.p) + (int64_t)(qf + q) * a.out.row + (int64_t)head * a.out.head;
@@ -269,7 +286,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 ? (D == 64 ? 4 : 2) : (D == 64
                         store4_rest<T>(rrow + 32 * d + 8 * r4 + 4 * hi, o[d][4 * r4] * inv, o[d][4 * r4 + 1] * inv, o[d][4 * r4 + 2] * inv, o[d][4 * r4 + 3] * inv);
             }
         }
-        if (a.lse && hi == 0) a.lse[(int64_t)head * a.q_rows + qf + q] = any ? m * c2 + log2_(sum) : -INFINITY;
+        if (a.lse && hi == 0) a.lse[(int64_t)head * a.q_rows + qf + q] = any ? row_base<T>(m, c2) + log2_(sum) : -INFINITY;
     }
 }
 

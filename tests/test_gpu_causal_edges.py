@@ -47,6 +47,63 @@ def _whole(dtype, H, G, D, ql, kl):
     assert _lib.load().some_op_causal_attention_bytes(None, TYPES.index(dtype), H, G, D, len(ql), sum(ql), sum(kl)) == 0
 
 
+# ---- one dominating key -----------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize('D', [64, 128])
+@pytest.mark.parametrize('n', [16384, 65536])
+@pytest.mark.parametrize('gap,spread', [(17.4, 0.05), (18.0, 1.0), (22.0, 0.05)])
+@pytest.mark.parametrize('where', ['first', 'last'])
+def test_half_precision_rows_with_one_dominating_key(eng, D, n, gap, spread, where):
+    """f16: the weights of all other keys together matter where the dominating key's value is small, and each of them is far below f16's normal range
+    beside a largest weight of 1."""
+    ql, kl = [33] + ALONE, [n] + ALONE
+    _whole(torch.float16, 1, 1, D, ql, kl)
+    q, k = _normal(1, sum(ql), 1, D, scale=0.01), _normal(2, sum(kl), 1, D, scale=0.01)
+    v = 1 + _normal(3, sum(kl), 1, D)
+    top = 0 if where == 'first' else n - 100
+    q[:, :, 0] = 4.0
+    k[:, :, 0] = _normal(4, sum(kl), 1, scale=spread / 4)
+    k[top, :, 0] = gap / 4
+    v[top] *= 0.01
+    q, k, v = q.half(), k.half(), v.half()
+    out = eng.causal_attention(q, k, v, _batch(ql), kv_batch=_batch(kl), scale=1.0)
+    oracle.check(out, *oracle.attention(q, k, v, ql, kl, scale=1.0), 'out')
+
+
+@pytest.mark.parametrize('D', [64, 128])
+@pytest.mark.parametrize('gaps', [(17.4, 30.0, 60.0), (60.0, 30.0, 17.4), (90.0, 12.0, 90.0), (9.0, 9.0, 9.0)])
+def test_half_precision_rows_with_several_dominating_keys(eng, D, gaps):
+    """f16: what the weights are taken relative to goes down behind one key and up again at the next."""
+    n = 4100
+    ql, kl = [33] + ALONE, [n] + ALONE
+    _whole(torch.float16, 1, 1, D, ql, kl)
+    q, k = _normal(6, sum(ql), 1, D, scale=0.01), _normal(7, sum(kl), 1, D, scale=0.05)
+    v = 1 + _normal(8, sum(kl), 1, D)
+    q[:, :, 0] = 5.0
+    for at, gap in zip((70, 2000, n - 1000), gaps):
+        k[at, :, 0] = gap / 5
+        v[at] = 0.0
+    q, k, v = q.half(), k.half(), v.half()
+    out = eng.causal_attention(q, k, v, _batch(ql), kv_batch=_batch(kl), scale=1.0)
+    oracle.check(out, *oracle.attention(q, k, v, ql, kl, scale=1.0), 'out')
+
+
+@pytest.mark.parametrize('D', [64, 128])
+@pytest.mark.parametrize('size', [100.0, 2500.0, 13600.0])
+@pytest.mark.parametrize('rising', [False, True])
+def test_half_precision_rows_of_huge_scores(eng, D, size, rising):
+    """f16: scores of 10^3 to 10^7 nats that leave one key a row; the weights keep inside f16's range."""
+    n, H = 200, 2
+    step = torch.arange(1, n + 1, device='cuda', dtype=torch.float32) * (size / n)
+    q, k, v = torch.zeros(n, H, D, device='cuda'), torch.zeros(n, 1, D, device='cuda'), _normal(5, n, 1, D, dtype=torch.float16)
+    q[:, :, 7] = size
+    k[:, 0, 7] = step if rising else step.flip(0)
+    q, k = q.half(), k.half()
+    out = eng.causal_attention(q, k, v, _batch([n]), scale=0.125)
+    # (the definition's own bound grows with the scores and allows everything here: the weight's rounding and the output's, as the keys lie 6 nats apart at least)
+    want = oracle.attention(q, k, v, [n], [n], scale=0.125)[0]
+    oracle.check(out, want, 2 * oracle.half_step(torch.float16) * want.abs() + 2.0 ** -11 * v.abs().max().double(), 'out')
+
+
 # ---- long runs of equal frames --------------------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize('dtype', TYPES)
 @pytest.mark.parametrize('D', [64, 128])
