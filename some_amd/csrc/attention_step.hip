@@ -13,7 +13,6 @@ namespace {
 using namespace causal;
 
 constexpr int NW = 4;                            // waves of a block
-constexpr float kSlack = 8.f;                    // the running maximum moves when a score passes it by 2^8 (causal_fwd.hip)
 template <typename T, int D> struct StepShape {
     static constexpr int TILE_B = 32 * D * (int)sizeof(T);
     static constexpr int WAVE_B = 2 * TILE_B;                              // two V tiles
@@ -62,7 +61,7 @@ __global__ __launch_bounds__(NW * 64, (sizeof(T) == 4 && D == 128 ? 1 : 2)) void
 #pragma unroll
     for (int d = 0; d < DB; ++d) o[d] = zero16();
     float m = -INFINITY, l = 0.f;
-    const float c2 = a.scale * 1.4426950408889634f, slack = kSlack / c2;
+    const float c2 = a.scale * 1.4426950408889634f, slack = kSlack / c2, drop = kDrop / c2;
 
     if (wave < ntiles) fetch(wave, 0);
     int stage = 0;
@@ -86,9 +85,9 @@ __global__ __launch_bounds__(NW * 64, (sizeof(T) == 4 && D == 128 ? 1 : 2)) void
 #pragma unroll
         for (int r = 1; r < 16; ++r) mx = fmaxf(mx, s[r]);
         mx = halves_max(mx);
-        if (__any(mx > m + slack)) {
-            const float mn = mx > m + slack ? mx : m;
-            const float f = m == -INFINITY ? 0.f : exp2_((m - mn) * c2);
+        if (__any(max_moves<T>(mx, m, slack, drop))) {
+            const float mn = max_moved<T>(mx, m, l, c2, slack, drop);
+            const float f = m == -INFINITY ? 0.f : exp2_(row_base<T>(m, c2) - row_base<T>(mn, c2));
             m = mn;
             l *= f;
 #pragma unroll
@@ -96,7 +95,7 @@ __global__ __launch_bounds__(NW * 64, (sizeof(T) == 4 && D == 128 ? 1 : 2)) void
 #pragma unroll
                 for (int r = 0; r < 16; ++r) o[d][r] *= f;
         }
-        const float mc = m == -INFINITY ? 0.f : m * c2;
+        const float mc = m == -INFINITY ? 0.f : row_base<T>(m, c2);
 #pragma unroll
         for (int r = 0; r < 16; ++r) s[r] = exp2_(fmaf(s[r], c2, -mc));
 #pragma unroll
@@ -110,7 +109,7 @@ __global__ __launch_bounds__(NW * 64, (sizeof(T) == 4 && D == 128 ? 1 : 2)) void
     }
     l = halves_sum(l);
 
-    // join the waves: O [wave][head][D], then m and l [wave][head]
+    // join the waves: O [wave][head][D], then what it is relative to and l [wave][head]
     __syncthreads();
     float* ow = reinterpret_cast<float*>(lds);
     float* ml = ow + NW * 32 * D;
@@ -121,7 +120,7 @@ __global__ __launch_bounds__(NW * 64, (sizeof(T) == 4 && D == 128 ? 1 : 2)) void
             for (int r4 = 0; r4 < 4; ++r4)
                 *reinterpret_cast<f32x4*>(ow + (wave * 32 + l31) * D + 32 * d + 8 * r4 + 4 * hi) = (f32x4){o[d][4 * r4], o[d][4 * r4 + 1], o[d][4 * r4 + 2], o[d][4 * r4 + 3]};
         if (hi == 0) {
-            ml[wave * 32 + l31] = m;
+            ml[wave * 32 + l31] = row_base<T>(m, c2);
             ml[(NW + wave) * 32 + l31] = l;
         }
     }
@@ -135,7 +134,7 @@ __global__ __launch_bounds__(NW * 64, (sizeof(T) == 4 && D == 128 ? 1 : 2)) void
 #pragma unroll
         for (int x = 0; x < NW; ++x) {
             const float mx = ml[x * 32 + h];
-            const float f = mx == -INFINITY ? (ml[(NW + x) * 32 + h] == 0.f ? 0.f : 1.f) : exp2_((mx - mm) * c2);
+            const float f = mx == -INFINITY ? (ml[(NW + x) * 32 + h] == 0.f ? 0.f : 1.f) : exp2_(mx - mm);
             acc = fmaf(ow[(x * 32 + h) * D + d], f, acc);
             ll = fmaf(ml[(NW + x) * 32 + h], f, ll);
         }
@@ -146,7 +145,7 @@ __global__ __launch_bounds__(NW * 64, (sizeof(T) == 4 && D == 128 ? 1 : 2)) void
             const int64_t slot = ((int64_t)b * a.kv_heads * a.group + head0 + h) * a.chunks + chunk;
             a.part_o[slot * D + d] = acc;
             if (d == 0) {
-                a.part_ml[2 * slot] = mm * c2;
+                a.part_ml[2 * slot] = mm;
                 a.part_ml[2 * slot + 1] = ll;
             }
         }

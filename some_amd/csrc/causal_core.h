@@ -220,6 +220,36 @@ template <typename T, int D, int ROWS, int NT> struct Copier {
     }
 };
 
+// ---- the softmax's running maximum -----------------------------------------------------------------------------------------------------------
+// The running maximum only has to keep the exponentials in range, so it follows the true one lazily: it moves when a score passes it by 2^8.  P then
+// reaches 256, far inside every operand type, and the accumulators are rescaled once or twice per row instead of at every new maximum.
+constexpr float kSlack = 8.f;
+constexpr float kDrop = 11.f;                    // (f16: row_base)
+
+// What the exponentials of a row are taken relative to: P = exp2(s c2 - row_base(m)).  In f16 the base lies 2^7 below the maximum, so that P runs from 2^15 (the
+// slack included) down to subnormals of 2^-24, and the running maximum follows the true one of a tile DOWN as well when that lies 2^11 below: with the row's
+// maximum and a largest P of 1, the level tail of a peaked row - 16 384 keys 17.4 nats below one - was rounded away altogether.  A weight is off by at most 2^-21
+// of its tile's largest that way (and by 2^-32 of it where that is the row's).  Scores of 2^20 and more, whose base has no digits behind the point left to spare,
+// do without the 2^7: there P needs the room above.
+template <typename T> __device__ __forceinline__ float row_base(float m, float c2) {
+    const float x = m * c2;
+    if constexpr (__is_same(T, f16_t)) return x - (__builtin_fabsf(x) < 0x1p20f ? 7.f : 0.f);
+    else return x;
+}
+// whether a tile of maximum mx moves the running maximum m (the first visible key passes -inf; a sum m + slack would round up where scores are huge), and where to
+template <typename T> __device__ __forceinline__ bool max_moves(float mx, float m, float slack, float drop) {
+    if constexpr (__is_same(T, f16_t)) return __builtin_fabsf(mx - m + 0.5f * (drop - slack)) > 0.5f * (drop + slack);
+    else return mx - m > slack;
+}
+template <typename T> __device__ __forceinline__ float max_moved(float mx, float m, float l, float c2, float slack, float drop) {
+    float mn = mx - m > slack ? mx : m;
+    if constexpr (__is_same(T, f16_t)) {                     // down: as far as the row's sum, and with it O, keeps inside f32's range
+        const float room = fmaxf(100.f - log2_(halves_max(l)), 0.f) / c2;
+        if (mx - m < -drop && mx > -INFINITY) mn = fmaxf(mx, m - room);
+    }
+    return mn;
+}
+
 // f32: acc[d] += the tile's 32 rows from r0 on, transposed, times x.  These products add one row after the other, so a block's are summed by themselves, one
 // sum in registers at a time: added to a long sum one by one, equal terms all round the same way (65 536 of them: off by 7e-4).
 template <typename T, int D> __device__ __forceinline__ void add_block(f32x16 (&acc)[D / 32], const char* tile, int r0, const f32x16& x, int lane) {

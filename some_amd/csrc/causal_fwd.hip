@@ -12,22 +12,6 @@
 namespace {
 using namespace causal;
 
-// The running maximum only has to keep the exponentials in range, so it follows the true one lazily: it moves when a score passes it by 2^8.  P then
-// reaches 256, far inside every operand type, and the accumulators are rescaled once or twice per row instead of at every new maximum.
-constexpr float kSlack = 8.f;
-constexpr float kDrop = 11.f;                    // (f16: row_base)
-
-// What the exponentials of a row are taken relative to: P = exp2(s c2 - row_base(m)).  In f16 the base lies 2^7 below the maximum, so that P runs from 2^15 (the
-// slack included) down to subnormals of 2^-24, and the running maximum follows the true one of a tile DOWN as well when that lies 2^11 below: with the row's
-// maximum and a largest P of 1, the level tail of a peaked row - 16 384 keys 17.4 nats below one - was rounded away altogether.  A weight is off by at most 2^-21
-// of its tile's largest that way (and by 2^-32 of it where that is the row's).  Scores of 2^20 and more, whose base has no digits behind the point left to spare,
-// do without the 2^7: there P needs the room above.
-template <typename T> __device__ __forceinline__ float row_base(float m, float c2) {
-    const float x = m * c2;
-    if constexpr (__is_same(T, f16_t)) return x - (__builtin_fabsf(x) < 0x1p20f ? 7.f : 0.f);
-    else return x;
-}
-
 constexpr int QB = 128;                          // queries per workgroup
 
 template <typename T, int D> struct Shape {
@@ -150,13 +134,8 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 ? (D == 64 ? 4 : 2) : (D == 64
 #pragma unroll
             for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[nb][r]);
         mx = halves_max(mx);
-        // (the first visible key passes -inf; a sum m + slack would round up where scores are huge)
-        if (__any(__is_same(T, f16_t) ? __builtin_fabsf(mx - m + 0.5f * (drop - slack)) > 0.5f * (drop + slack) : mx - m > slack)) {
-            float mn = mx - m > slack ? mx : m;
-            if constexpr (__is_same(T, f16_t)) {             // down: as far as the row's sum, and with it O, keeps inside f32's range
-                const float room = fmaxf(100.f - log2_(halves_max(l)), 0.f) / c2;
-                if (mx - m < -drop && mx > -INFINITY) mn = fmaxf(mx, m - room);
-            }
+        if (__any(max_moves<T>(mx, m, slack, drop))) {
+            const float mn = max_moved<T>(mx, m, l, c2, slack, drop);
             const float f = m == -INFINITY ? 0.f : exp2_(row_base<T>(m, c2) - row_base<T>(mn, c2));
             m = mn;
             l *= f;

@@ -104,6 +104,24 @@ def test_half_precision_rows_of_huge_scores(eng, D, size, rising):
     oracle.check(out, want, 2 * oracle.half_step(torch.float16) * want.abs() + 2.0 ** -11 * v.abs().max().double(), 'out')
 
 
+@pytest.mark.parametrize('H,G,D', [(2, 2, 64), (5, 1, 128)])
+@pytest.mark.parametrize('gap', [12.0, 17.4, 22.0])
+@pytest.mark.parametrize('capacity', [520, 3000])
+def test_half_precision_step_with_one_dominating_key(eng, H, G, D, gap, capacity):
+    """f16: the step's weights as well, whichever tile, wave and chunk the dominating key falls to."""
+    tops = [0, 1, 40, 200, 511]
+    B, n = len(tops), capacity - 3
+    q, kc, vc = _normal(91, B, H, D, scale=0.01), _normal(92, B, capacity, G, D, scale=0.02), 1 + _normal(93, B, capacity, G, D)
+    q[..., 0] = 4.0
+    for b, at in enumerate(tops):
+        kc[b, at, :, 0] = gap / 4
+        vc[b, at] = 0.0
+    q, kc, vc = q.half(), kc.half(), vc.half()
+    got = eng.attention_step(q, kc, vc, torch.full((B,), n, dtype=torch.int32, device='cuda'), scale=1.0)
+    k, v = (c[:, :n].reshape(B * n, G, D) for c in (kc, vc))
+    oracle.check(got, *oracle.attention(q, k, v, [1] * B, [n] * B, scale=1.0), 'step')
+
+
 # ---- long runs of equal frames --------------------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize('dtype', TYPES)
 @pytest.mark.parametrize('D', [64, 128])
