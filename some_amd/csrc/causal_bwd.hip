@@ -12,13 +12,16 @@
 namespace {
 using namespace causal;
 
-// f16 only: dS has the gradient's scale, which may lie far below (or above) f16's range.  A column's values are multiplied by a power of two F of its
-// own - constant over the contraction, so the accumulators simply carry it - that is lowered (accumulators rescaled) when a block would pass 2^14.
-template <int DB> __device__ __forceinline__ void fit_column(const f32x16& ds, float& F, f32x16 (&acc)[DB]) {
+// f16 only: dS has the gradient's scale, which may lie far below (or above) f16's range.  A column's values (in units of `unit`) are multiplied by a power of two F of
+// its own - constant over the contraction, so the accumulators simply carry it - that is lowered (accumulators rescaled) when a block would pass 2^14.
+__device__ __forceinline__ float block_max(const f32x16& x) {
     float mx = 0.f;
 #pragma unroll
-    for (int r = 0; r < 16; ++r) mx = fmaxf(mx, __builtin_fabsf(ds[r]));
-    mx = halves_max(mx);
+    for (int r = 0; r < 16; ++r) mx = fmaxf(mx, __builtin_fabsf(x[r]));
+    return halves_max(mx);
+}
+template <int DB> __device__ __forceinline__ void fit_column(const f32x16& ds, float unit, float& F, f32x16 (&acc)[DB]) {
+    const float mx = block_max(ds) * unit;
     if (__any(mx * F > 16384.f)) {
         if (mx * F > 16384.f) {
             const float f = __builtin_ldexpf(1.f, min(100, max(-126, 5 - __builtin_amdgcn_frexp_expf(mx))));
@@ -32,8 +35,27 @@ template <int DB> __device__ __forceinline__ void fit_column(const f32x16& ds, f
     }
 }
 constexpr float kFitStart = 0x1p100f;
-// f16 only: probabilities of long clips (about 1 / T) would be subnormal; they enter the products as 2^10 P
-template <typename T> constexpr float kProbLog2 = __is_same(T, f16_t) ? 10.f : 0.f;
+// f16 only: a key's weights may all lie far below f16's range as well, or those of the queries that count may (a key that one row alone looks at).  They too carry a
+// power of two, which follows a block's largest weight down and up, at most 2^80: weights are 1 at most, so the accumulators stay inside f32's range.  It is set where
+// that weight leaves [2^-4, 2^14], to 2^11 or more: a weight is off by at most 2^-21 of its block's largest, and by 2^-36 of the largest that set it.
+constexpr float kProbStart = 80.f;
+template <int DB> __device__ __forceinline__ void fit_probs(f32x16& p, f32x16& ds, float& log2f, f32x16 (&acc)[DB]) {
+    const float mx = block_max(p);
+    const bool off = mx > 16384.f || (mx < 0.0625f && mx > 0.f && log2f < kProbStart);
+    if (__any(off)) {
+        const float by = off ? fminf((float)(12 - __builtin_amdgcn_frexp_expf(mx)), kProbStart - log2f) : 0.f, ratio = exp2_(by);
+        log2f += by;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            p[r] *= ratio;
+            ds[r] *= ratio;
+        }
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) acc[d][r] *= ratio;
+    }
+}
 
 // ---- dQ (and D) ----------------------------------------------------------------------------------------------------------------------------
 constexpr int QB = 128;                          // queries per workgroup
@@ -143,7 +165,7 @@ __global__ __launch_bounds__(256, (D == 64 ? (sizeof(T) == 2 ? 4 : 2) : sizeof(T
                 for (int r = 0; r < 16; ++r) s[r] = key0 + crow(r, hi) <= limit ? s[r] : 0.f;
             }
             if constexpr (F16) {
-                fit_column<DB>(s, F, acc);
+                fit_column<DB>(s, 1.f, F, acc);
 #pragma unroll
                 for (int r = 0; r < 16; ++r) s[r] *= F;
             }
@@ -280,7 +302,7 @@ __global__ __launch_bounds__(256, (D == 64 ? (sizeof(T) == 2 ? 3 : 2) : sizeof(T
         dk[d] = zero16();
         dv[d] = zero16();
     }
-    float F = F16 ? kFitStart : 1.f;
+    float F = F16 ? kFitStart : 1.f, log2p = F16 ? kProbStart : 0.f;       // dk's and dv's powers of two (f16)
     const float c2 = a.scale * 1.4426950408889634f;
     bool bad = false;
 
@@ -323,7 +345,7 @@ __global__ __launch_bounds__(256, (D == 64 ? (sizeof(T) == 2 ? 3 : 2) : sizeof(T
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const int r = 4 * r4 + i;
-                    s[r] = exp2_(kProbLog2<T> == 0.f ? fmaf(s[r], c2, -lv[i]) : fmaf(s[r], c2, kProbLog2<T> - lv[i]));
+                    s[r] = exp2_(fmaf(s[r], c2, F16 ? log2p - lv[i] : -lv[i]));
                     dp[r] = s[r] * (sizeof(T) == 4 ? dp[r] + d4[i] : dp[r]);
                 }
             }
@@ -338,9 +360,11 @@ __global__ __launch_bounds__(256, (D == 64 ? (sizeof(T) == 2 ? 3 : 2) : sizeof(T
                 bad |= block_not_finite<T, D>(qt, nb * 32) || block_not_finite<T, D>(gt, nb * 32);
             }
             if constexpr (F16) {
-                fit_column<DB>(dp, F, dk);
+                fit_probs<DB>(s, dp, log2p, dv);
+                const float unit = exp2_(-log2p);
+                fit_column<DB>(dp, unit, F, dk);
 #pragma unroll
-                for (int r = 0; r < 16; ++r) dp[r] *= F;
+                for (int r = 0; r < 16; ++r) dp[r] *= F * unit;
             }
             products_first();
             if constexpr (sizeof(T) == 4) {
@@ -397,8 +421,8 @@ __global__ __launch_bounds__(256, (D == 64 ? (sizeof(T) == 2 ? 3 : 2) : sizeof(T
         return;
     }
     if (key < Tk) {
-        const float pf = F16 ? 0x1p-10f : 1.f;
-        const float fk = a.scale / F * pf;
+        const float pf = F16 ? exp2_(-log2p) : 1.f;
+        const float fk = a.scale / F;
         const int64_t i = ((prow + kf + key) * a.kv_heads + w.kvh) * D + 4 * hi;
         T* dkd = static_cast<T*>(b.dk.p) + (int64_t)(kf + key) * b.dk.row + (int64_t)w.kvh * b.dk.head + 4 * hi;
         T* dvd = static_cast<T*>(b.dv.p) + (int64_t)(kf + key) * b.dv.row + (int64_t)w.kvh * b.dv.head + 4 * hi;

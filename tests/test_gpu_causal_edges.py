@@ -122,6 +122,50 @@ def test_half_precision_step_with_one_dominating_key(eng, H, G, D, gap, capacity
     oracle.check(got, *oracle.attention(q, k, v, [1] * B, [n] * B, scale=1.0), 'step')
 
 
+@pytest.mark.parametrize('D', [64, 128])
+@pytest.mark.parametrize('gap', [12.0, 22.0, 26.0, 40.0])
+@pytest.mark.parametrize('magnitude', [1.0, 1000.0, 20000.0])
+def test_half_precision_gradients_of_faint_keys(ops, D, gap, magnitude):
+    """f16: the gradient of a value whose weights are all small, over many queries and for gradients of any magnitude."""
+    lens = [2000, 129]
+    M = sum(lens)
+    q, k, v = _normal(11, M, 1, D, scale=0.02), _normal(12, M, 1, D, scale=0.02), _normal(13, M, 1, D)
+    q[:, :, 0] = 4.0
+    k[0, :, 0] = k[2000, :, 0] = gap / 4
+    dout = ((1 + 0.5 * _normal(14, M, 1, D)) * magnitude).half()
+    leaves = [t.half().requires_grad_() for t in (q, k, v)]
+    out = ops.causal_attention(*leaves, _batch(lens), scale=1.0)
+    grads = torch.autograd.grad(out, leaves, dout)
+    w = list(oracle.attention(*(t.detach() for t in leaves), lens, lens, scale=1.0, dout=dout))
+    for i in (2, 4, 6):
+        w[i] = w[i].masked_fill(w[i].abs() >= 65000, math.nan)      # what f16 cannot hold is infinite, as anywhere
+    _check_all((out, *grads), w)
+
+
+@pytest.mark.parametrize('D', [64, 128])
+@pytest.mark.parametrize('gap', [17.4, 24.0])
+def test_half_precision_gradients_of_a_key_only_one_row_looks_at(ops, D, gap):
+    """f16: a key's weight is 1 in its own row, which the loss leaves out, and faint in all others."""
+    lens = [3000]
+    M = sum(lens)
+    q, k, v = _normal(15, M, 2, D, scale=0.02), _normal(16, M, 1, D, scale=0.02), _normal(17, M, 1, D)
+    q[:, :, 0] = 4.0
+    k[0, :, 0] = -gap / 4
+    dout = (1 + 0.5 * _normal(18, M, 2, D)) * 1000
+    dout[0] = 0.0
+    dout = dout.half()
+    leaves = [t.half().requires_grad_() for t in (q, k, v)]
+    out = ops.causal_attention(*leaves, _batch(lens), scale=1.0)
+    grads = torch.autograd.grad(out, leaves, dout)
+    w = list(oracle.attention(*(t.detach() for t in leaves), lens, lens, scale=1.0, dout=dout))
+    for i in (2, 4, 6):
+        w[i] = w[i].masked_fill(w[i].abs() >= 65000, math.nan)
+    # the weights of the 32 rows that share a block (and a power of two) with the key's own row, of both heads: that power brings the weight 1 to 2^11 at least, and
+    # f16's smallest step is 2^-24, so each is off by 2^-25 / 2^11 at most
+    w[7] = w[7] + 2 * 32 * 2.0 ** -36 * dout.abs().max().double()
+    _check_all((out, *grads), w)
+
+
 # ---- long runs of equal frames --------------------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize('dtype', TYPES)
 @pytest.mark.parametrize('D', [64, 128])
