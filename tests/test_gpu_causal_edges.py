@@ -166,6 +166,28 @@ def test_half_precision_gradients_of_a_key_only_one_row_looks_at(ops, D, gap):
     _check_all((out, *grads), w)
 
 
+# ---- parts without keys -------------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('D', [64, 128])
+def test_a_part_without_keys_is_left_zero(eng, dtype, D):
+    """Keys in parts, a clip of fewer tiles than parts: what the parts without a tile hand to the join is zeros, not what lay in LDS."""
+    ql, kl, H = [64, 64], [8000, 30], 1
+    M, N, code = sum(ql), sum(kl), TYPES.index(dtype)
+    lib, h = _lib.fast(), eng.handle.value
+    q, k, v = (_normal(41 + i, n, H, D, dtype=dtype) for i, n in enumerate((M, N, N)))
+    nb = lib.some_op_causal_attention_bytes(h, code, H, H, D, 2, M, N)
+    parts = nb // (M * H * (D + 2) * 4)
+    assert parts > 2 and parts * M * H * (D + 2) * 4 == nb
+    bq, bk = _batch(ql), _batch(kl)                                # (held: the call gets bare addresses of their offsets)
+    work, out = torch.full((nb // 4,), 7.0, device='cuda'), torch.empty_like(q)
+    s3 = lambda t: (t.data_ptr(), t.stride(0), t.stride(1))                                   # noqa: E731
+    _lib.check(h, lib.some_op_causal_attention(h, code, D, *s3(q), H, *s3(k), *s3(v), H, bq.frame_offsets_dev.data_ptr(), bk.frame_offsets_dev.data_ptr(),
+                                               2, M, N, 0, 0.125, *s3(out), None, None, work.data_ptr(), nb, torch.cuda.current_stream().cuda_stream))
+    sums = work[:parts * M * H * D].view(parts, M, H, D)
+    assert not sums[:parts - 1, ql[0]:].any()                      # the one tile of the second clip belongs to the last part
+    oracle.check(out, *oracle.attention(q, k, v, ql, kl, False, scale=0.125), 'out')
+
+
 # ---- long runs of equal frames --------------------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize('dtype', TYPES)
 @pytest.mark.parametrize('D', [64, 128])
