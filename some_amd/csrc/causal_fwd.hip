@@ -185,7 +185,16 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 ? (D == 64 ? 4 : 2) : (D == 64
     // A wave that sees one tile in all: where a row sees few keys, nothing averages the rounding of P out of O (nor of the gradients' D), so what it took goes
     // in too.  The tile still lies in the first stage, nobody writes there any more, and the maximum is the loop's.
     if constexpr (sizeof(T) == 2) {
-        if (t_begin == 0 && t_end > 0 && t_end <= STAGES && seen_w > 0 && seen_w <= KT && !bad) {
+        const bool few = t_begin == 0 && t_end > 0 && t_end <= STAGES && seen_w > 0 && seen_w <= KT && !bad;
+        if (few) {                                           // (the rest of a weight may be nought or negative: an infinity of V that is seen must not meet it)
+            bool lost = false;
+#pragma unroll
+            for (int d = 0; d < DB; ++d)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) lost |= o[d][r] - o[d][r] != 0.f;
+            bad = __any(lost);
+        }
+        if (few && !bad) {
             const float mc = m == -INFINITY ? 0.f : row_base<T>(m, c2);
             const int limit = min(q + shift, Tk - 1);
             for (int nb = 0; nb * 32 < seen_w; ++nb) {

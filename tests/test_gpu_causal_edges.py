@@ -166,6 +166,40 @@ def test_half_precision_gradients_of_a_key_only_one_row_looks_at(ops, D, gap):
     _check_all((out, *grads), w)
 
 
+# ---- infinities that are seen -------------------------------------------------------------------------------------------------------------
+def _infinite_values(v, rows):
+    """Copies of v with +inf in channel 3 and -inf in channel 5 of the given rows, and with zeros there."""
+    a, b = v.clone(), v.clone()
+    for x, p, m in ((a, math.inf, -math.inf), (b, 0.0, 0.0)):
+        for r in rows:
+            x[r][..., 3] = p
+            x[r][..., 5] = m
+    return a, b
+
+
+def _check_infinite(got, want, tol):
+    assert (got[..., 3] == math.inf).all() and (got[..., 5] == -math.inf).all()
+    rest = [c for c in range(got.shape[-1]) if c not in (3, 5)]
+    oracle.check(got[..., rest], want[..., rest], tol[..., rest], 'the other channels')
+
+
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('D', [64, 128])
+@pytest.mark.parametrize('keys', [31, 32, 33, 63, 64, 65, 128, 200])
+@pytest.mark.parametrize('queries', [1, 40])
+@pytest.mark.parametrize('train', [False, True])
+def test_an_infinite_value_every_query_sees(eng, ops, dtype, D, keys, queries, train):
+    H, G = 4, 2
+    q, k, v = _normal(21, queries, H, D, dtype=dtype), _normal(22, keys, G, D, dtype=dtype), _normal(23, keys, G, D, dtype=dtype)
+    inf, fin = _infinite_values(v, [10])
+    call = ops if train else eng
+    if train:
+        q = q.requires_grad_()
+    for causal in (False, True) if queries == 1 else (False,):
+        got = call.causal_attention(q, k, inf, _batch([queries]), kv_batch=_batch([keys]), causal_mask=causal).detach()
+        _check_infinite(got, *oracle.attention(q, k, fin, [queries], [keys], causal))
+
+
 # ---- parts without keys -------------------------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize('dtype', TYPES)
 @pytest.mark.parametrize('D', [64, 128])
