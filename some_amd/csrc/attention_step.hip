@@ -49,7 +49,7 @@ __global__ __launch_bounds__(NW * 64, (sizeof(T) == 4 && D == 128 ? 1 : 2)) void
     char* own = lds + wave * StepShape<T, D>::WAVE_B;
     const int ntiles = (max(0, hi_key - lo) + 31) / 32;
     frag kfr[KS], knext[KS];
-    auto fetch = [&](int t, int stage) {                                   // (rows past the chunk: copies of its last one)
+    auto fetch = [&](int t, int stage) {                                   // (rows past the chunk: copies of its last one, V's to be zeroed)
         const int key0 = lo + t * 32;
         const T* krow = reinterpret_cast<const T*>(kbase + (int64_t)min(key0 + l31, hi_key - 1) * kbytes) + 8 * hi;
 #pragma unroll
@@ -72,7 +72,13 @@ __global__ __launch_bounds__(NW * 64, (sizeof(T) == 4 && D == 128 ? 1 : 2)) void
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) kfr[ks] = knext[ks];
         if (t + NW < ntiles) fetch(t + NW, stage ^ 1);
-        const char* vt = own + stage * TILE_B;
+        char* vt = own + stage * TILE_B;
+        if (lo + t * 32 + 32 > hi_key) {                                   // values of places past the end: copies of the last one, which may be infinite
+#pragma unroll 1
+            for (int i = lane; i < 32 * TL::CHUNKS; i += 64)
+                if (lo + t * 32 + i / TL::CHUNKS >= hi_key) *reinterpret_cast<uint4*>(vt + i * 16) = uint4{0, 0, 0, 0};
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        }
         f32x16 s = zero16();
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) s = mma<T>(kfr[ks], qfr[ks], s);

@@ -200,6 +200,21 @@ def test_an_infinite_value_every_query_sees(eng, ops, dtype, D, keys, queries, t
         _check_infinite(got, *oracle.attention(q, k, fin, [queries], [keys], causal))
 
 
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('H,G,D', [(4, 2, 64), (2, 2, 128), (40, 1, 64)])
+@pytest.mark.parametrize('capacity', [40, 1000, 3000])
+def test_step_over_a_newest_frame_with_an_infinite_value(eng, dtype, H, G, D, capacity):
+    lens = [n for n in (1, 2, 31, 32, 33, 63, 64, 65, 127, 128, 129, 255, 256, 257, 1000, 2049, 3000) if n <= capacity]
+    B = len(lens)
+    q, kc, vc = _normal(31, B, H, D, dtype=dtype), _normal(32, B, capacity, G, D, dtype=dtype), _normal(33, B, capacity, G, D, dtype=dtype)
+    inf, fin = _infinite_values(vc, [(b, n - 1) for b, n in enumerate(lens)])
+    for b, n in enumerate(lens):
+        inf[b, n:] = kc[b, n:] = math.nan
+    got = eng.attention_step(q, kc, inf, torch.tensor(lens, dtype=torch.int32, device='cuda'))
+    k, v = (torch.cat([c[b, :n] for b, n in enumerate(lens)]) for c in (kc, fin))
+    _check_infinite(got, *oracle.attention(q, k, v, [1] * B, lens))
+
+
 # ---- parts without keys -------------------------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize('dtype', TYPES)
 @pytest.mark.parametrize('D', [64, 128])
