@@ -553,7 +553,7 @@ int some_train_qk_norm_rope_bwd(SomeHandle* h, int32_t dtype, int32_t head_dim, 
 /* out = softmax(scale q k^T) v per clip.  Clip b's queries are rows [q_offsets[b], q_offsets[b + 1]) and its keys rows [k_offsets[b], ...): with
  * causal != 0 the queries are the clip's LAST frames, i.e. query i of Tq sees keys j <= i + Tk - Tq (a chunk over what is cached already); with
  * causal = 0 every key.  A query that sees no key gets 0, and nothing in a masked place - infinities and NaN included - reaches an output.
- * scale > 0.  For the backward, each NULL if there is none: rest_dev [q_rows, heads, head_dim] of the type, what rounding to a 16-bit type took from out
+ * scale > 0, log2(e) scale finite.  For the backward, each NULL if there is none: rest_dev [q_rows, heads, head_dim] of the type, what rounding to a 16-bit type took from out
  * (f16: times 2^10; not used for fp32), and lse_dev fp32 [heads, q_rows] (base-2 log-sum-exp, -inf where no key is seen).  workspace_dev:
  * some_op_causal_attention_bytes bytes (0 unless few queries meet many keys), 16-byte aligned, not shared with a call that may run at the same time. */
 size_t some_op_causal_attention_bytes(const SomeHandle* h, int32_t dtype, int32_t heads, int32_t kv_heads, int32_t head_dim, int32_t B, int64_t q_rows,

@@ -61,7 +61,7 @@ __global__ __launch_bounds__(NW * 64, (sizeof(T) == 4 && D == 128 ? 1 : 2)) void
 #pragma unroll
     for (int d = 0; d < DB; ++d) o[d] = zero16();
     float m = -INFINITY, l = 0.f;
-    const float c2 = a.scale * 1.4426950408889634f, slack = kSlack / c2, drop = kDrop / c2;
+    const float c2 = a.scale * 1.4426950408889634f, slack = score_units(kSlack, c2), drop = score_units(kDrop, c2);
 
     if (wave < ntiles) fetch(wave, 0);
     int stage = 0;

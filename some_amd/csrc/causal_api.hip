@@ -34,6 +34,8 @@ bool laid_out(int dtype, const Rows3& x) {
 bool type_ok(int dtype, int head_dim) { return dtype >= 0 && dtype <= 2 && (head_dim == 64 || head_dim == 128); }
 bool heads_ok(int heads, int kv_heads) { return kv_heads > 0 && heads > 0 && heads <= kMaxHeads && heads % kv_heads == 0; }
 
+bool scale_ok(float scale) { return scale > 0.f && std::isfinite(scale * 1.4426950408889634f); }      // (the exponentials are of base 2)
+
 const char* kType = "dtype must be SOME_DTYPE_F32, F16 or BF16 and head_dim 64 or 128";
 const char* kHeadsMsg = "heads must be a multiple of kv_heads, at most 1024";
 const char* kLayout = "arrays must be 16-byte aligned, strides non-negative multiples of 16 bytes, rows below 16 MiB apart";
@@ -151,7 +153,7 @@ int some_op_causal_attention(SomeHandle* h, int32_t dtype, int32_t head_dim, con
     C_CHECK(type_ok(dtype, head_dim), kType);
     C_CHECK(heads_ok(heads, kv_heads), kHeadsMsg);
     C_CHECK(B >= 0 && q_rows >= 0 && k_rows >= 0 && q_rows < kMaxRows && k_rows < kMaxRows && B < kMaxRows, "clips and rows must be below 2^29");
-    C_CHECK(scale > 0.f && std::isfinite(scale), "scale must be finite and positive");
+    C_CHECK(scale_ok(scale), "scale must be positive and log2(e) times it finite");
     if (B == 0 || q_rows == 0) return SOME_OK;
     C_CHECK(q_dev && out_dev && q_offsets_dev && k_offsets_dev && (k_rows == 0 || (k_dev && v_dev)), "null pointer");
     CausalArgs a{};
@@ -183,7 +185,7 @@ int some_train_causal_attention_bwd(SomeHandle* h, int32_t dtype, int32_t head_d
     C_CHECK(type_ok(dtype, head_dim), kType);
     C_CHECK(heads_ok(heads, kv_heads), kHeadsMsg);
     C_CHECK(B >= 0 && q_rows >= 0 && k_rows >= 0 && q_rows < kMaxRows && k_rows < kMaxRows && B < kMaxRows, "clips and rows must be below 2^29");
-    C_CHECK(scale > 0.f && std::isfinite(scale), "scale must be finite and positive");
+    C_CHECK(scale_ok(scale), "scale must be positive and log2(e) times it finite");
     if (B == 0 || (q_rows == 0 && k_rows == 0)) return SOME_OK;
     C_CHECK(q_offsets_dev && k_offsets_dev && workspace_dev, "null pointer");
     C_CHECK(q_rows == 0 || (q_dev && out_dev && lse_dev && dout_dev && dq_dev), "null pointer");
@@ -228,7 +230,7 @@ int some_op_attention_step(SomeHandle* h, int32_t dtype, int32_t head_dim, const
     C_CHECK(heads_ok(heads, kv_heads), kHeadsMsg);
     C_CHECK(B >= 0 && B <= 65535, "at most 65535 streams");
     C_CHECK(max_length >= 0 && max_length < kMaxRows, "max_length must be below 2^29");
-    C_CHECK(scale > 0.f && std::isfinite(scale), "scale must be finite and positive");
+    C_CHECK(scale_ok(scale), "scale must be positive and log2(e) times it finite");
     if (B == 0) return SOME_OK;
     C_CHECK(q_dev && out_dev && lengths_dev && (max_length == 0 || (k_dev && v_dev)), "null pointer");
     StepArgs a{};

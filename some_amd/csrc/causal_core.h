@@ -236,6 +236,8 @@ template <typename T> __device__ __forceinline__ float row_base(float m, float c
     if constexpr (__is_same(T, f16_t)) return x - (__builtin_fabsf(x) < 0x1p20f ? 7.f : 0.f);
     else return x;
 }
+// a distance of exponents in units of the raw products; finite for scales next to nought too, or the first key would not pass it
+__device__ __forceinline__ float score_units(float x, float c2) { return x / fmaxf(c2, 0x1p-120f); }
 // whether a tile of maximum mx moves the running maximum m (the first visible key passes -inf; a sum m + slack would round up where scores are huge), and where to
 template <typename T> __device__ __forceinline__ bool max_moves(float mx, float m, float slack, float drop) {
     if constexpr (__is_same(T, f16_t)) return __builtin_fabsf(mx - m + 0.5f * (drop - slack)) > 0.5f * (drop + slack);

@@ -97,7 +97,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 ? (D == 64 ? 4 : 2) : (D == 64
 #pragma unroll
     for (int d = 0; d < DB; ++d) o[d] = zero16();
     float m = -INFINITY, l = 0.f, lost = 0.f;                // running maximum (of the raw products), this half's share of the sum, what rounding added to it last (f32)
-    const float c2 = a.scale * 1.4426950408889634f, slack = kSlack / c2, drop = kDrop / c2;
+    const float c2 = a.scale * 1.4426950408889634f, slack = score_units(kSlack, c2), drop = score_units(kDrop, c2);
     bool bad = false;
 
     if (t_begin < t_end) fetch(t_begin);

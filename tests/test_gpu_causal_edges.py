@@ -268,3 +268,18 @@ def test_gradients_of_long_runs_of_equal_frames(ops, dtype, D, causal):
     out = ops.causal_attention(*leaves, _batch(lens), causal_mask=causal)
     grads = torch.autograd.grad(out, leaves, dout)
     _check_all((out, *grads), oracle.attention(*(t.detach() for t in leaves), lens, lens, causal, dout=dout))
+
+
+# ---- scales far from 1 --------------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('scale', [2.0 ** -64, 2.0 ** -126, 2.0 ** -130])
+def test_a_scale_next_to_nought(ops, dtype, scale):
+    """All weights alike: the mean of what a row sees, and gradients to match."""
+    lens, H, G, D = [70, 3], 2, 1, 64
+    M = sum(lens)
+    q, k, v = _normal(71, M, H, D, dtype=dtype), _normal(72, M, G, D, dtype=dtype), _normal(73, M, G, D, dtype=dtype)
+    dout = _normal(74, M, H, D, dtype=dtype)
+    leaves = [t.requires_grad_() for t in (q, k, v)]
+    out = ops.causal_attention(*leaves, _batch(lens), scale=scale)
+    grads = torch.autograd.grad(out, leaves, dout)
+    _check_all((out, *grads), oracle.attention(q, k, v, lens, lens, scale=scale, dout=dout))
