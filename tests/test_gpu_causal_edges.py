@@ -283,3 +283,28 @@ def test_a_scale_next_to_nought(ops, dtype, scale):
     out = ops.causal_attention(*leaves, _batch(lens), scale=scale)
     grads = torch.autograd.grad(out, leaves, dout)
     _check_all((out, *grads), oracle.attention(q, k, v, lens, lens, scale=scale, dout=dout))
+
+
+# ---- norm + rotation of many rows -------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('M,H,G,D', [(30011, 13, 5, 64), (9001, 33, 7, 128), (60007, 16, 3, 64), (150001, 1, 6, 64)])
+def test_norm_rope_of_many_rows(ops, eng, dtype, M, H, G, D):
+    """Several heads a thread (a count that does not divide the heads), a launch of as many blocks as there may be, each of them over many rows."""
+    assert M * (H + G) * (D // 16) > 1 << 20
+    lib = _lib.load()
+    assert lib.some_train_qk_norm_rope_bytes(None, M, H, G, D) == 1536 * D * 4
+    fused = _normal(81, M, H + 2 * G, D, dtype=dtype, scale=1.7)
+    q, k = fused[:, :H], fused[:, H:H + G]
+    gq, gk = 1 + _normal(83, D, scale=0.3), 1 + _normal(84, D, scale=0.3)
+    pos = torch.randint(-50, 3000000, (M,), device='cuda', generator=torch.Generator(device='cuda').manual_seed(85))
+    dq, dk = _normal(86, M, H, D, dtype=dtype), _normal(87, M, G, D, dtype=dtype)
+    leaves = [t.detach().requires_grad_() for t in (q, k, gq, gk)]
+    yq, yk = ops.qk_norm_rope(*leaves, pos)
+    grads = torch.autograd.grad([yq, yk], leaves, [dq, dk])
+    sq, sk = eng.qk_norm_rope(q, k, gq, gk, pos)
+    assert torch.equal(sq, yq) and torch.equal(sk, yk)
+    for x, g, d, y, dx, dg in ((q, gq, dq, yq, grads[0], grads[2]), (k, gk, dk, yk, grads[1], grads[3])):
+        w = oracle.norm_rope(x, g, pos, dy=d)
+        oracle.check(y.detach(), *w[0:2], 'y')
+        oracle.check(dx, *w[2:4], 'dx')
+        oracle.check(dg, *w[4:6], 'dgamma')
