@@ -541,7 +541,8 @@ int some_op_qk_norm_rope(SomeHandle* h, int32_t dtype, int32_t head_dim, const v
                          const float* gamma_k_dev, const void* positions_dev, int32_t positions64, double theta, float eps, void* q_out_dev,
                          int64_t qo_row, int64_t qo_head, void* k_out_dev, int64_t ko_row, int64_t ko_head, void* stream);
 /* Its gradients: q / k are the forward's inputs, dqo / dko the gradients of its outputs; writes dq, dk (which may be dqo, dko) and - added to their
- * contents if accumulate != 0 - the fp32 gain gradients, summed in a fixed order.  scratch_dev: some_train_qk_norm_rope_bytes. */
+ * contents if accumulate != 0 - the fp32 gain gradients, two arrays that do not overlap (one gain for both: add them), summed in a fixed order.
+ * scratch_dev: some_train_qk_norm_rope_bytes. */
 size_t some_train_qk_norm_rope_bytes(const SomeHandle* h, int64_t rows, int32_t heads, int32_t kv_heads, int32_t head_dim);
 int some_train_qk_norm_rope_bwd(SomeHandle* h, int32_t dtype, int32_t head_dim, const void* q_dev, int64_t q_row, int64_t q_head, int32_t heads,
                                 const void* k_dev, int64_t k_row, int64_t k_head, int32_t kv_heads, int64_t rows, const float* gamma_q_dev,

@@ -120,6 +120,8 @@ int some_train_qk_norm_rope_bwd(SomeHandle* h, int32_t dtype, int32_t head_dim, 
     C_CHECK(fill_turns(a, theta, head_dim), "theta must be finite and positive");
     if (scratch_bytes < some_train_qk_norm_rope_bytes(h, rows, heads, kv_heads, head_dim))
         return cfail(h, SOME_ENOMEM, __func__, "scratch too small (some_train_qk_norm_rope_bytes)");
+    const uintptr_t gq = reinterpret_cast<uintptr_t>(dgamma_q_dev), gk = reinterpret_cast<uintptr_t>(dgamma_k_dev);
+    C_CHECK((gq < gk ? gk - gq : gq - gk) >= head_dim * sizeof(float), "gain gradients must not overlap (they are written, or added to, at the same time)");
     a.gamma_q = gamma_q_dev; a.gamma_k = gamma_k_dev; a.positions = positions_dev; a.positions64 = positions64;
     a.partial = static_cast<float*>(scratch_dev);
     a.rows = rows; a.heads = heads; a.kv_heads = kv_heads; a.eps = eps;
