@@ -329,13 +329,13 @@ __global__ __launch_bounds__(256, (D == 64 ? (sizeof(T) == 2 ? 3 : 2) : sizeof(T
 #pragma unroll
                 for (int i = 0; i < 4; ++i) dp[4 * r4 + i] = d4[i];
             }
-            products_first();
+            if constexpr (sizeof(T) == 2) products_first();
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
                 s = mma<T>(TL::row_frag(qt, nb * 32 + l31, ks, hi), kfr[ks], s);
                 dp = mma<T>(TL::row_frag(gt, nb * 32 + l31, ks, hi), vfr(ks), dp);
             }
-            products_done();
+            if constexpr (sizeof(T) == 2) products_done();
             const bool edge = qb0 + shift < kw + 31 || qb0 + 32 > Tq || kw + 32 > Tk;
 #pragma unroll
             for (int r4 = 0; r4 < 4; ++r4) {
@@ -366,7 +366,7 @@ __global__ __launch_bounds__(256, (D == 64 ? (sizeof(T) == 2 ? 3 : 2) : sizeof(T
 #pragma unroll
                 for (int r = 0; r < 16; ++r) dp[r] *= F * unit;
             }
-            products_first();
+            if constexpr (sizeof(T) == 2) products_first();
             if constexpr (sizeof(T) == 4) {
                 add_block<T, D>(dv, gt, nb * 32, s, lane);
                 add_block<T, D>(dk, qt, nb * 32, dp, lane);
@@ -381,7 +381,7 @@ __global__ __launch_bounds__(256, (D == 64 ? (sizeof(T) == 2 ? 3 : 2) : sizeof(T
                     }
                 }
             }
-            products_done();
+            if constexpr (sizeof(T) == 2) products_done();
         }
         g = gn;
         t = tn;

@@ -72,8 +72,9 @@ __device__ __forceinline__ f32x16 zero16() {
 }
 
 // Around a run of products: the wave goes before the others of its SIMD, whose exponentials then fill the gaps between the products instead of delaying them.
-// us without and with: backward, 8 x 2584 frames, 8/2 heads of 64: dK/dV bf16 146, 140, f16 170, 159, dQ 108, 106.5 and 120, 116; forward, 3 clips up to 8191,
-// 16/4 heads of 128, bf16: 340, 315, but 4 x 4096 frames in f32 1416, 1446 and heads of 64, bf16, 84.4, 86.6 - there the forward goes without.
+// us without and with: 8 x 2584 frames, 8/2 heads of 64: dK/dV bf16 146, 142, f16 189, 174, dQ 108.8, 108.3 and 119.9, 115.8; forward, 3 clips up to 8191, 16/4
+// heads of 128, bf16: 305, 286; 4 x 4096 frames, 8/2 heads of 64, f32: forward 661, 597, dQ 903, 845.  Not so the 16-bit forward at heads of 64 (bf16 87.6, 88.5,
+// f16 85.9, 87.6) and dK/dV in f32 (1212, 1270): those go without.
 __device__ __forceinline__ void products_first() { __builtin_amdgcn_s_setprio(1); }
 __device__ __forceinline__ void products_done() { __builtin_amdgcn_s_setprio(0); }
 
@@ -115,12 +116,6 @@ template <typename T> __device__ __forceinline__ typename Frag<T>::type load8(co
     } else {
         return *reinterpret_cast<const s16x8*>(p);
     }
-}
-template <typename T> __device__ __forceinline__ typename Frag<T>::type zero8() {
-    typename Frag<T>::type f;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) f[j] = 0;
-    return f;
 }
 
 // four neighbouring values of a row, rounded to the type once

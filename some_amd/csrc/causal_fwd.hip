@@ -110,7 +110,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 ? (D == 64 ? 4 : 2) : (D == 64
         const int key0 = t * KT;
         if (key0 >= seen_w) continue;
         f32x16 s[NB];
-        if constexpr (sizeof(T) == 2 && D == 128) products_first();
+        if constexpr (sizeof(T) == 4 || D == 128) products_first();
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
             s[nb] = zero16();
@@ -118,7 +118,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 ? (D == 64 ? 4 : 2) : (D == 64
             for (int ks = 0; ks < KS; ++ks) s[nb] = mma<T>(TL::row_frag(kt, nb * 32 + l31, ks, hi), qfr[ks], s[nb]);
         }
         if constexpr (sizeof(T) == 2) order_products<NB * KS, 1, 4>();
-        if constexpr (sizeof(T) == 2 && D == 128) products_done();
+        if constexpr (sizeof(T) == 4 || D == 128) products_done();
         if (key0 + KT > full_w) {                            // some masked place in here
             const int limit = min(q + shift, Tk - 1);
 #pragma unroll
@@ -162,7 +162,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 ? (D == 64 ? 4 : 2) : (D == 64
             if constexpr (sizeof(T) == 4) lost = (sum - l) - w;
             l = sum;
         }
-        if constexpr (sizeof(T) == 2 && D == 128) products_first();
+        if constexpr (sizeof(T) == 4 || D == 128) products_first();
         if constexpr (sizeof(T) == 4) {
             // (16-bit products add eight keys at a time, and far below their own rounding).  The block's sum is too much for two waves a SIMD at heads of 128: 59
             // registers spilled, 4 x 4096 frames, 8/2 heads, 1810 us, one wave 1375
@@ -179,7 +179,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 ? (D == 64 ? 4 : 2) : (D == 64
                 }
         }
         if constexpr (sizeof(T) == 2) order_products<NB * 2 * DB, 2, 3>();
-        if constexpr (sizeof(T) == 2 && D == 128) products_done();
+        if constexpr (sizeof(T) == 4 || D == 128) products_done();
     }
 
     // A wave that sees one tile in all: where a row sees few keys, nothing averages the rounding of P out of O (nor of the gradients' D), so what it took goes
