@@ -5,7 +5,7 @@
 //                   group are the columns of its products, so a key is read once for all of them.  Running maximum and sum per wave, the waves of a
 //                   block joined through LDS; one chunk in all: the output, otherwise a partial (O, m, l).
 //   join_kernel     joins a stream's chunks in chunk order (the result does not depend on which block finished first).
-// 32 streams of 8 x 128 (32 heads) in bf16, lengths up to 8192, take 68 + 4 us (4.7 TB/s); one of 517 frames, 8 x 64: 5.2 + 2.4 us, which is latency.  In f32 the
+// 32 streams of 8 x 128 (32 heads) in bf16, lengths up to 8192, take 69 + 5 us (4.6 TB/s); one of 517 frames, 8 x 64: 5.2 + 2.6 us, which is latency.  In f32 the
 // products bound short caches: of their 32 columns a group of 4 heads fills 4.
 #include "causal_core.h"
 
@@ -208,9 +208,10 @@ template <typename T, int D> hipError_t run(const StepArgs& a, hipStream_t s) {
 }  // namespace
 
 // Keys of a chunk (us of the launches alone).  Up to 64 KiB of keys a stream and kv head there are no chunks and no join, for the second launch also costs the
-// host 3.5 us: one stream of 8 x 64 in bf16, 512 frames whole 5.5, in chunks of 128 6.1; 1024 whole 7.7, in chunks of 256 6.7.  Beyond, a chunk has 128 frames
-// (256 where a row is 128 bytes: 2584 frames 7.4, in chunks of 128 7.5, of 512 7.9), and more as long as 256 blocks, one for each CU, remain (32 streams, 1024
-// frames: 256 blocks 13.3, 512: 16.8), but not above 1024, for the sake of unequal streams (32, up to 8192 frames: chunks of 1024 38, of 2048 57).
+// host 3.5 us: one stream of 8 x 64 in bf16, 512 frames whole 6.3, in chunks of 128 4.4 + 2.4; 1024 whole 8.5, in chunks of 256 5.2 + 2.4.  Beyond, a chunk has 128
+// frames (256 where a row is 128 bytes: one stream of 8 x 64, 2584 frames 5.3 + 3.3, in chunks of 128 4.7 + 3.8; two of 5000, 8/2 heads, 5.6 + 4.1 and 4.9 + 5.5),
+// and more as long as 256 blocks, one for each CU, remain (32 streams of 1024 frames, 32/8 heads of 128: 256 blocks 25, 512: 24 + 4), but not above 1024, for the
+// sake of unequal streams (the 32 up to 8192 frames above: chunks of 512 72 + 4, of 1024 71 + 5, of 2048 73 + 5).
 StepPlan step_plan(int dtype, int head_dim, int B, int kv_heads, int group, int max_len) {
     const int64_t units = (int64_t)B * kv_heads * ((group + 31) / 32);
     const int row = head_dim * (dtype == 0 ? 4 : 2);

@@ -5,8 +5,8 @@
 //   causal_dq_kernel   a wave owns 32 queries (a lane's column is a query), loops over the keys they see; writes D on the way in
 //   causal_dkv_kernel  a wave owns 32 keys of one kv head (a lane's column is a key), loops over the group's heads and the queries that see them
 // In both, the recomputed tile's registers are the B operand of the products that follow (causal_core.h).  Nine products of a pair instead of the formula's seven
-// are the price of the order.  8 x 2584 frames, 8/2 heads of 64, bf16: 106 + 140 us, 780 TF/s of what they compute (VALU 50 and 40 % busy, products 35 %);
-// 3 clips up to 8191, 16/4 heads of 128: 445 + 690 us, 860 TF/s, products 40 to 48 % busy at the clock the power limit leaves.
+// are the price of the order.  8 x 2584 frames, 8/2 heads of 64, bf16: 104 + 135 us, 800 TF/s of what they compute (VALU 51 and 42 % busy, products 36 %);
+// 3 clips up to 8191, 16/4 heads of 128: 411 + 613 us, 950 TF/s, products 48 and 40 % busy at the clock the power limit leaves.
 #include "causal_core.h"
 
 namespace {
@@ -493,8 +493,8 @@ template <typename T, int D> hipError_t run(const CausalBwdArgs& b, hipStream_t 
 
 // Parts the queries (and heads of a group) that a key tile meets are cut into: as many as bring the launch to 1200 workgroups - some rounds of the 512 to 768
 // that run at once, so that causal tiles of unequal work end together; every part costs a plane of partial sums -, at least 4 tiles of 64 queries each.
-// us of the kernel + the sum, bf16: 8 x 2584 frames, 8/2 heads of 64: 1 part 412, 2: 233 + 10, 3: 173 + 13, 4: 157 + 15, 5: 162 + 18; 8191 + 1326 frames,
-// 16/4 heads of 128: 1 part 1859, 2: 1057 + 16, 3: 782 + 22, 4: 751 + 27, 6: 747 + 39.  Lengths are on the device, so the averages over the batch decide.
+// us of the kernel + the sum, bf16: 8 x 2584 frames, 8/2 heads of 64: 1 part 327, 2: 192 + 9, 3: 144 + 12, 4: 142 + 15, 5: 146 + 17; 3 clips up to 8191,
+// 16/4 heads of 128: 1 part 1796, 2: 1016 + 16, 3: 772 + 22, 4: 726 + 27, 6: 732 + 38.  Lengths are on the device, so the averages over the batch decide.
 int causal_bwd_parts(int64_t q_rows, int64_t k_rows, int B, int heads, int kv_heads) {
     if (B <= 0 || q_rows <= 0 || k_rows <= 0) return 1;
     const int64_t tiles = (k_rows + KB - 1) / KB > B ? (k_rows + KB - 1) / KB : B;

@@ -5,8 +5,8 @@
 // group frames with all heads of a group, which read every key tile together -, a wave 32 of them; S^T = K Q^T puts a query in every lane's column, so its
 // maximum and sum are the lane's own registers plus one exchange with the other half, and P^T is already the B operand of O^T += V^T P^T (causal_core.h):
 // no probability touches LDS.  K and V tiles go global -> LDS by DMA into a ring; V is read transposed by ds_read_b64_tr_b16.
-// Bound by the products at heads of 128 - 2 clips up to 16384, 32/8 heads, bf16: 2.42 ms, 1040 TF/s, where a large matrix product reaches 1120 under the power
-// limit - and at heads of 64 by the exponentials and what stands around them (8 x 2584, 8/2 heads, bf16: 84 us, 650 TF/s, VALU 60 % and products 29 % busy).
+// Bound by the products at heads of 128 - 2 clips up to 16384, 32/8 heads, bf16: 2.32 ms, 1090 TF/s, where a large matrix product reaches 1120 under the power
+// limit - and at heads of 64 by the exponentials and what stands around them (8 x 2584, 8/2 heads, bf16: 83 us, 660 TF/s, VALU 60 % and products 29 % busy).
 #include "causal_core.h"
 
 namespace {
@@ -15,7 +15,7 @@ using namespace causal;
 constexpr int QB = 128;                          // queries per workgroup
 
 template <typename T, int D> struct Shape {
-    static constexpr int KT = sizeof(T) == 4 ? 32 : 64;      // keys per tile (f32, 8 x 520 frames, heads of 64: 64 keys 53 us, 32: 48)
+    static constexpr int KT = sizeof(T) == 4 ? 32 : 64;      // keys per tile (f32: one block, whose products are summed by themselves)
     static constexpr int TILE_B = KT * D * (int)sizeof(T);
     static constexpr int STAGES = 2;
     static constexpr int LDS_B = STAGES * 2 * TILE_B;
@@ -279,7 +279,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 ? (D == 64 ? 4 : 2) : (D == 64
 }
 
 // Joins the parts of the keys, in order, four channels a thread and four parts in flight (a clip's rows see keys in the first part or in none: it says so by
-// a sum of -1).  Bound by latency where parts are few: 4160 rows of 8 heads of 64 in two parts take 6 us in f32 and 5 in bf16.
+// a sum of -1).  Bound by latency where parts are few: 4160 rows of 8 heads of 64 in two parts take 6 us in f32.
 template <typename T, int D> __global__ __launch_bounds__(256) void causal_join_kernel(CausalArgs a) {
     const int heads = a.kv_heads * a.group;
     const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x, i0 = id / (D / 4), row = i0 / heads;
@@ -346,10 +346,10 @@ int64_t causal_fwd_blocks(const CausalArgs& a) { return causal::work_blocks(a.kv
 
 // Parts the keys are cut into: 1 unless the queries alone give too few workgroups AND the keys are long (256 of them per part at least in f32, 512 in the
 // 16-bit types).  Every part costs a plane of partial sums, so the launch is only brought to about 576 workgroups (2 per CU and a few more for balance): an f16
-// chunk of 766 frames, 16/4 heads of 128, over 20 000 cached ones takes 4 parts 164 + 9 us, 5: 143 + 11, 6: 135 + 13, 8: 152 + 16, 12: 137 + 22.  8 x 520
-// frames, 8 heads of 64: f32 1 part 63 us, 2: 48 + 6; bf16 17, 15 + 5.  2 x 1000, 8/1 heads of 128: f32 1 part 239, 3: 102 + 7; bf16 27, 22 + 6.  2 x 1500,
-// 8/2 heads of 64, bf16: 1 part 30, 2: 21 + 5, 3: 19 + 5.  The gradient of the queries takes the same parts (and a sum): 2 x 1000, 8/1 heads of 128, f32 1 part
-// 225, 3: 93 + 6; 2 x 2000, bf16 68, 2: 48 + 8.  Lengths are on the device, so the averages over the batch decide.
+// chunk of 766 frames, 16/4 heads of 128, over 20 000 cached ones takes 4 parts 146 + 6 us, 5: 132 + 7, 6: 128 + 8, 8: 147 + 10, 12: 132 + 13.  8 x 520
+// frames, 8 heads of 64, f32: 1 part 59 us, 2: 47 + 6.  2 x 1000, 8/1 heads of 128, f32: 1 part 167, 2: 92 + 6, 3: 69 + 7.  2 x 1500, 8/2 heads of 64, bf16:
+// 1 part 32, 2: 22 + 5; 2 x 2000, 8/1 heads of 128: 1 part 53, 2: 38 + 9.  The gradient of the queries takes the same parts (and a sum): 2 x 1000, 8/1 heads of
+// 128, f32: 1 part 229, 3: 95 + 6; 2 x 2000, bf16: 72, 2: 52 + 8.  Lengths are on the device, so the averages over the batch decide.
 int causal_fwd_parts(int dtype, int64_t q_rows, int64_t k_rows, int B, int heads, int kv_heads) {
     if (B <= 0 || q_rows <= 0) return 1;
     const int64_t queries = q_rows * (heads / kv_heads), tiles = (queries + 127) / 128 > B ? (queries + 127) / 128 : B;

@@ -745,7 +745,7 @@ class TrainOps:
 
     def causal_attention(self, q, k, v, batch, kv_batch=None, causal_mask: bool = True, scale: Optional[float] = None, head_dim: int = 0):
         """Attention over packed clips that looks back only, heads in groups (``Engine.causal_attention``), differentiable in q, k and v; takes and
-        returns float32, float16 or bfloat16 (in float16, gradients of any magnitude are carried at full precision).  To capture a backward pass
+        returns float32, float16 or bfloat16 (in float16 weights and gradients carry powers of two of their own, so those of any magnitude keep their bits).  To capture a backward pass
         into a graph, let no eager graph of the same leaves be alive: torch would wait inside the capture for the stream of that graph."""
         q3, _, _, kv = causal.check_attention(self.device, q, k, v, batch, kv_batch, head_dim)
         return self._apply(_CausalAttention, q, k, v, batch, kv, bool(causal_mask), causal.default_scale(scale, q3.shape[2]),
