@@ -187,12 +187,12 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 ? (D == 64 ? 4 : 2) : (D == 64
     if constexpr (sizeof(T) == 2) {
         const bool few = t_begin == 0 && t_end > 0 && t_end <= STAGES && seen_w > 0 && seen_w <= KT && !bad;
         if (few) {                                           // (the rest of a weight may be nought or negative: an infinity of V that is seen must not meet it)
-            bool lost = false;
+            bool inf = false;
 #pragma unroll
             for (int d = 0; d < DB; ++d)
 #pragma unroll
-                for (int r = 0; r < 16; ++r) lost |= o[d][r] - o[d][r] != 0.f;
-            bad = __any(lost);
+                for (int r = 0; r < 16; ++r) inf |= o[d][r] - o[d][r] != 0.f;
+            bad = __any(inf);
         }
         if (few && !bad) {
             const float mc = m == -INFINITY ? 0.f : row_base<T>(m, c2);
